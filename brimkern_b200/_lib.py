@@ -23,6 +23,9 @@ BRK_ERR_DEVICE = -5
 BRK_MAX_BATCH = 512
 BRK_KV_F16 = 0
 BRK_KV_I8 = 1
+BRK_T_F32 = 0
+BRK_T_F16 = 1
+ACTIVATIONS = {"none": 0, "silu": 1, "gelu": 2, "gelu_tanh": 3, "quick_gelu": 4}
 BRK_DECODE_STATIC_SCRATCH_BYTES = 8 << 20
 BRK_MAX_PEERS = 8
 BRK_PEER_HANDLE_BYTES = 64
@@ -91,6 +94,11 @@ SIGNATURES = [
     ("brk_attn_combine", _i, [_vp, _i, _i, _i, _vp, _vp, _sz, _vp, _vp]),
     ("brk_proj_qkv", _i, [_vp, _i, _i, _i, _i, _vp, _vp, _d, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     ("brk_proj_out", _i, [_vp, _i, _i, _i, _vp, _vp, _vp, _d, _i, _vp, _vp, _vp]),
+    ("brk_attn_decode_prefix", _i, [_vp, _vp, _i, _i, _vp, _i, _PARAMS, _i, _i, _i32p, _vp, _i, _vp, _i, _vp]),
+    ("brk_attn_step_prefix", _i, [_vp, _vp, _i, _i, _vp, _i, _PARAMS, _i, _i, _i32p, _vp, _vp, _vp, _vp, _vp, _i, _vp]),
+    ("brk_linear", _i, [_vp, _i, _i, _i, _vp, _vp, _vp, _i, _vp, _vp, _i, _vp]),
+    ("brk_ffn_gate_up", _i, [_vp, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _i, _vp, _vp]),
+    ("brk_ffn", _i, [_vp, _i, _i, _i, _vp, _vp, _d, _i, _vp, _vp, _vp, _vp, _i, _vp, _vp]),
     ("brk_peer_create", _i, [_vp, _i, _i, _i, _i, _pp]),
     ("brk_peer_handle", _i, [_vp, _vp, _sz]),
     ("brk_peer_open", _i, [_vp, _i, _vp, _sz]),

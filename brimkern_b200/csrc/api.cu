@@ -9,6 +9,7 @@
 #include <cstdlib>
 #include <cstring>
 #include <mutex>
+#include <new>
 #include <string>
 #include <vector>
 
@@ -304,6 +305,72 @@ int ensure_counters(brk_ctx *ctx, size_t n) {
     return BRK_OK;
 }
 
+// The scratch of `stream`, or of the capture it is in: a workspace of at least `bytes` and
+// n_counters zeroed counters.  Growing keeps the old buffers (queued kernels and captured graphs
+// may still use them) and neither synchronises nor disturbs a capture: the allocation runs in
+// relaxed capture mode, and the counters are zeroed on a stream of the context's own.
+int get_scratch(brk_ctx *ctx, cudaStream_t stream, size_t bytes, size_t n_counters, brk_scratch **out) {
+    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    BRK_CUDA(cudaStreamGetCaptureInfo(stream, &st, &id));
+    if (st == cudaStreamCaptureStatusInvalidated) return fail(BRK_ERR_CUDA, "the stream's capture is invalid");
+    const bool capture = st == cudaStreamCaptureStatusActive;
+    if (!capture) BRK_CUDA(cudaStreamGetId(stream, &id));
+    brk_scratch *sc = nullptr;
+    for (brk_scratch *x : ctx->scratch)
+        if (x->id == id && x->capture == capture) sc = x;
+    if (!sc) {
+        sc = new (std::nothrow) brk_scratch();
+        if (!sc) return fail(BRK_ERR_CUDA, "out of host memory");
+        sc->id = id;
+        sc->capture = capture;
+        try {
+            ctx->scratch.push_back(sc);
+        } catch (...) {
+            delete sc;
+            return fail(BRK_ERR_CUDA, "out of host memory");
+        }
+    }
+    *out = sc;
+    if (bytes <= sc->ws_bytes && n_counters <= sc->counters_n) return BRK_OK;
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    BRK_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
+    cudaError_t e = cudaSuccess;
+    try {
+        sc->retired.reserve(sc->retired.size() + 2);
+        if (bytes > sc->ws_bytes) {
+            const size_t want = (std::max(bytes, 2 * sc->ws_bytes) + 255) / 256 * 256;
+            void *p = nullptr;
+            e = cudaMalloc(&p, want);
+            if (e == cudaSuccess) {
+                if (sc->ws) sc->retired.push_back(sc->ws);
+                sc->ws = p;
+                sc->ws_bytes = want;
+            }
+        }
+        if (e == cudaSuccess && n_counters > sc->counters_n) {
+            const size_t want = std::max(std::max(n_counters, 2 * sc->counters_n), (size_t)4096);
+            void *p = nullptr;
+            e = cudaMalloc(&p, want * sizeof(int));
+            if (e == cudaSuccess && !ctx->aux) e = cudaStreamCreateWithFlags(&ctx->aux, cudaStreamNonBlocking);
+            if (e == cudaSuccess) e = cudaMemsetAsync(p, 0, want * sizeof(int), ctx->aux);
+            if (e == cudaSuccess) e = cudaStreamSynchronize(ctx->aux);
+            if (e == cudaSuccess) {
+                if (sc->counters) sc->retired.push_back(sc->counters);
+                sc->counters = static_cast<int *>(p);
+                sc->counters_n = want;
+            } else {
+                cudaFree(p);
+            }
+        }
+    } catch (...) {
+        e = cudaErrorMemoryAllocation;
+    }
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    if (e != cudaSuccess) return cuda_fail(e, "scratch allocation");
+    return BRK_OK;
+}
+
 // fixed_ws / fixed_bytes: when set, the split-KV scratch goes there and nothing is allocated
 // (brk_attn_decode_static); otherwise the context workspace is used and grown on demand.
 // pdl: the decode kernel is a programmatic dependent of the append launched just before it.
@@ -532,6 +599,13 @@ int brk_ctx_destroy(brk_ctx *ctx) {
     cudaFree(ctx->ws);
     cudaFree(ctx->stage);
     cudaFree(ctx->act);
+    for (brk_scratch *sc : ctx->scratch) {
+        cudaFree(sc->ws);
+        cudaFree(sc->counters);
+        for (void *p : sc->retired) cudaFree(p);
+        delete sc;
+    }
+    if (ctx->aux) cudaStreamDestroy(ctx->aux);
     delete ctx;
     return BRK_OK;
 }
@@ -546,6 +620,8 @@ int brk_ctx_check(brk_ctx *ctx, void *stream) {
         BRK_CUDA(cudaMemset(ctx->d_err, 0, sizeof(int)));
         // A kernel that gave up may have left split counters mid-count: start them from zero.
         if (ctx->counters) BRK_CUDA(cudaMemset(ctx->counters, 0, ctx->counters_n * sizeof(int)));
+        for (brk_scratch *sc : ctx->scratch)
+            if (sc->counters) BRK_CUDA(cudaMemset(sc->counters, 0, sc->counters_n * sizeof(int)));
         return fail(BRK_ERR_DEVICE, "a kernel gave up on a bounded wait (code %d)", err);
     }
     return BRK_OK;
@@ -1339,6 +1415,379 @@ int brk_proj_out(brk_ctx *ctx, int rows, int q_dim, int d_model, const float *at
     rc = run_proj(ctx, rows, q_dim, attn, nullptr, 0.0, 0, 1, n, w, out, bias, post_norm ? nullptr : x, st);
     if (rc || !post_norm) return rc;
     cudaError_t e = brk::launch_post_norm_residual(h, x, post_norm, (float)eps, norm_one_plus, rows, d_model, st);
+    if (e != cudaSuccess) return cuda_fail(e, "post-norm launch");
+    ++ctx->launches;
+    return BRK_OK;
+}
+
+namespace {
+size_t align256(size_t n) { return (n + 255) / 256 * 256; }
+
+bool aligned16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+// Splits of the prefix's key tiles over CTAs (one CTA per SM).  A CTA's fixed cost (q staging, ring
+// ramp, join, partial) is worth about four tiles, and every split adds a partial to the merge.
+int prefix_splits(const brk_ctx *ctx, int units, int ntiles) {
+    const int most = std::min(32, std::max(1, ntiles / 2));
+    double best = 1e30;
+    int best_n = 1;
+    for (int n = 1; n <= most; ++n) {
+        const int tps = (ntiles + n - 1) / n;
+        const long long waves = ((long long)units * n + ctx->num_sms - 1) / ctx->num_sms;
+        const double cost = (double)waves * (tps + 4) + 0.25 * n;
+        if (cost < best - 1e-9) {
+            best = cost;
+            best_n = n;
+        }
+    }
+    return best_n;
+}
+
+int check_prefix_call(const brk_ctx *ctx, const brk_kv *prefix, int prefix_seq, int prefix_len, const brk_kv *kv,
+                      int layer, const brk_attn_params *p, int batch, int n_tokens, const int32_t *past_len,
+                      const void *q, int q_type, const void *out, int out_type) {
+    int rc = check_call(ctx, kv, layer, p, batch, n_tokens, past_len);
+    if (rc) return rc;
+    if (!q || !out) return fail(BRK_ERR_INVALID, "null q or out");
+    if ((q_type != BRK_T_F32 && q_type != BRK_T_F16) || (out_type != BRK_T_F32 && out_type != BRK_T_F16))
+        return fail(BRK_ERR_INVALID, "q type %d / out type %d (BRK_T_F32 or BRK_T_F16)", q_type, out_type);
+    if (!aligned16(q) || !aligned16(out)) return fail(BRK_ERR_INVALID, "q and out must be 16-byte aligned");
+    if (prefix_len < 0) return fail(BRK_ERR_INVALID, "prefix_len %d < 0", prefix_len);
+    if (p->kv_offset != prefix_len)
+        return fail(BRK_ERR_INVALID, "kv_offset %d must be the prefix length %d (the own rows follow the prefix)",
+                    p->kv_offset, prefix_len);
+    if ((long long)n_tokens * (p->n_heads / p->n_kv_heads) > 64)
+        return fail(BRK_ERR_UNSUPPORTED, "shared-prefix attention covers decode (n_tokens * group <= 64)");
+    if (prefix_len > 0) {
+        if (!prefix) return fail(BRK_ERR_INVALID, "null prefix cache");
+        if (prefix->ctx != ctx) return fail(BRK_ERR_INVALID, "prefix cache belongs to another context");
+        if (prefix->desc.n_kv_heads != p->n_kv_heads || prefix->desc.head_dim != p->head_dim)
+            return fail(BRK_ERR_INVALID, "params (%d kv heads, dim %d) do not match the prefix cache (%d, %d)",
+                        p->n_kv_heads, p->head_dim, prefix->desc.n_kv_heads, prefix->desc.head_dim);
+        if (layer >= prefix->desc.n_layers)
+            return fail(BRK_ERR_INVALID, "layer %d outside the prefix cache's [0, %d)", layer, prefix->desc.n_layers);
+        if (prefix_seq < 0 || prefix_seq >= prefix->desc.batch)
+            return fail(BRK_ERR_INVALID, "prefix sequence %d outside [0, %d)", prefix_seq, prefix->desc.batch);
+        if (prefix_len > prefix->cap)
+            return fail(BRK_ERR_CAPACITY, "prefix of %d rows, its cache's capacity is %d", prefix_len, prefix->cap);
+    }
+    for (int b = 0; b < batch; ++b)
+        if ((long long)past_len[b] + n_tokens - p->kv_offset > kv->cap)
+            return fail(BRK_ERR_CAPACITY, "sequence %d needs %lld cache rows, capacity is %d (grow the cache)", b,
+                        (long long)past_len[b] + n_tokens - p->kv_offset, kv->cap);
+    return BRK_OK;
+}
+
+// The launches of brk_attn_decode_prefix (arguments checked, device current).  pdl: the first is a
+// programmatic dependent of the append launched just before.
+int run_decode_prefix(brk_ctx *ctx, const brk_kv *prefix, int prefix_seq, int prefix_len, const brk_kv *kv, int layer,
+                      const brk_attn_params *p, int batch, int n_tokens, const int32_t *past_len, const void *q,
+                      int q_type, void *out, int out_type, cudaStream_t st, bool pdl) {
+    const int D = p->head_dim, G = p->n_heads / p->n_kv_heads, Hkv = p->n_kv_heads;
+    const int window = p->window > 0 ? p->window : 0;
+    const size_t rows = (size_t)batch * n_tokens * p->n_heads;
+    const float scale = effective_scale(p);
+    const float softcap = p->softcap > 0.f ? p->softcap : 0.f;
+    const double log2e = 1.4426950408889634;
+    const float cap_k1 = softcap > 0.f ? (float)(2.0 * (double)scale * log2e / (double)softcap) : 0.f;
+    const float cap_k2 = softcap > 0.f ? (float)((double)softcap * log2e) : 0.f;
+
+    // Keys of the prefix that some row attends (int8: from a multiple of four, for the scales' loads).
+    int k_begin = 0;
+    if (window > 0) {
+        int first = past_len[0];
+        for (int b = 1; b < batch; ++b) first = std::min(first, past_len[b]);
+        k_begin = (int)std::min<long long>(prefix_len, std::max<long long>(0, (long long)first - window + 1));
+        if (prefix_len > 0 && prefix->q8()) k_begin = k_begin / 4 * 4;
+    }
+    const int keys = prefix_len - k_begin;
+    int splits = 0, tps = 0;
+    if (keys > 0) {
+        const int rb = brk::prefix_block_rows(D, batch * n_tokens * G);
+        const int ntiles = (keys + brk::prefix_tile_keys() - 1) / brk::prefix_tile_keys();
+        splits = prefix_splits(ctx, Hkv * ((batch * n_tokens * G + rb - 1) / rb), ntiles);
+        tps = (ntiles + splits - 1) / splits;
+        splits = (ntiles + tps - 1) / tps;  // no empty split
+    }
+    int nsplit = 1, kps = 0;
+    int rc = decode_split_plan(ctx, kv, p, batch, n_tokens, past_len, false, &nsplit, &kps);
+    if (rc) return rc;
+    if (nsplit > 32) {  // the merge takes in at most 32 of these and 32 of the prefix's partials
+        const int tk = brk::decode_stage_keys(D);
+        const int span = nsplit * kps;
+        kps = ((span + 31) / 32 + tk - 1) / tk * tk;
+        nsplit = (span + kps - 1) / kps;
+    }
+    const int rt = brk::decode_rows_per_tile();
+    const int mtiles = (n_tokens * G + rt - 1) / rt;
+    const int units = batch * Hkv * mtiles;
+
+    const size_t n_ml = rows * 2 * sizeof(float), n_o = rows * D * sizeof(float);
+    const size_t staged = keys > 0 && prefix->q8() ? (size_t)Hkv * keys * D * sizeof(__half) : 0;
+    const size_t off_o = align256(splits * n_ml), off_sml = off_o + align256(splits * n_o);
+    const size_t off_so = off_sml + (nsplit > 1 ? align256(nsplit * n_ml) : 0);
+    const size_t off_k = off_so + (nsplit > 1 ? align256(nsplit * n_o) : 0), off_v = off_k + align256(staged);
+    brk_scratch *sc = nullptr;
+    rc = get_scratch(ctx, st, off_v + align256(staged), (size_t)units, &sc);
+    if (rc) return rc;
+    char *ws = static_cast<char *>(sc->ws);
+
+    if (keys > 0) {
+        brk::PrefixArgs x;
+        memset(&x, 0, sizeof(x));
+        x.q = q_type == BRK_T_F32 ? static_cast<const float *>(q) : nullptr;
+        x.q16 = q_type == BRK_T_F16 ? static_cast<const __half *>(q) : nullptr;
+        x.part_ml = reinterpret_cast<float *>(ws);
+        x.part_o = reinterpret_cast<float *>(ws + off_o);
+        x.err = ctx->d_err;
+        x.B = batch, x.T = n_tokens, x.Hq = p->n_heads, x.Hkv = Hkv, x.G = G;
+        x.rows = batch * n_tokens * G;
+        x.k_begin = k_begin, x.k_end = prefix_len;
+        x.tiles_per_split = tps;
+        x.window = window;
+        x.scale_log2 = scale * (float)log2e;
+        x.softcap = softcap, x.cap_k1 = cap_k1, x.cap_k2 = cap_k2;
+        for (int b = 0; b < batch; ++b) x.past_len[b] = past_len[b];
+        const size_t seg0 = ((size_t)layer * prefix->desc.batch + prefix_seq) * Hkv;
+        CUtensorMap mk, mv;
+        const CUtensorMap *tk = &prefix->tm_pre_k, *tv = &prefix->tm_pre_v;
+        if (staged) {
+            __half *sk = reinterpret_cast<__half *>(ws + off_k), *sv = reinterpret_cast<__half *>(ws + off_v);
+            const size_t off = seg0 * prefix->cap * D;
+            cudaError_t e = brk::launch_codes_to_half(prefix->k8 + off, prefix->v8 + off, sk, sv, Hkv, D, prefix->cap,
+                                                      k_begin, keys, st);
+            if (e != cudaSuccess) return cuda_fail(e, "prefix code staging launch");
+            ++ctx->launches;
+            pdl = false;  // the staging kernel, an ordinary launch, is between the append and the prefix kernel
+            if ((rc = make_cache_map(&mk, sk, (uint64_t)Hkv * keys, D, brk::prefix_tile_keys()))) return rc;
+            if ((rc = make_cache_map(&mv, sv, (uint64_t)Hkv * keys, D, brk::prefix_tile_keys()))) return rc;
+            tk = &mk, tv = &mv;
+            x.scales = prefix->scales + seg0 * 2 * prefix->scale_pitch;
+            x.scale_pitch = prefix->scale_pitch;
+            x.row0 = -k_begin;
+            x.head_rows = keys;
+        } else {
+            x.row0 = (int)(seg0 * prefix->cap);
+            x.head_rows = prefix->cap;
+        }
+        cudaError_t e = brk::launch_prefix(D, *tk, *tv, x, splits, st, pdl);
+        if (e != cudaSuccess) return cuda_fail(e, "prefix kernel launch");
+        ++ctx->launches;
+    }
+
+    brk::DecodeArgs a;
+    memset(&a, 0, sizeof(a));
+    a.with_prefix = 1;
+    a.late_wait = keys > 0;
+    a.pre_parts = splits;
+    a.pre_ml = reinterpret_cast<const float *>(ws);
+    a.pre_o = reinterpret_cast<const float *>(ws + off_o);
+    a.q = q_type == BRK_T_F32 ? static_cast<const float *>(q) : nullptr;
+    a.q16 = q_type == BRK_T_F16 ? static_cast<const __half *>(q) : nullptr;
+    a.out = out_type == BRK_T_F32 ? static_cast<float *>(out) : nullptr;
+    a.out16 = out_type == BRK_T_F16 ? static_cast<__half *>(out) : nullptr;
+    a.err = ctx->d_err;
+    a.B = batch, a.T = n_tokens, a.Hq = p->n_heads, a.Hkv = Hkv, a.G = G;
+    a.layer = layer;
+    a.cap = kv->cap;
+    a.mtiles = mtiles;
+    a.nsplit = nsplit;
+    a.keys_per_split = kps;
+    a.kv_offset = p->kv_offset;
+    a.window = window;
+    a.scale = scale;
+    a.scale_log2 = scale * (float)log2e;
+    a.softcap = softcap, a.cap_k1 = cap_k1, a.cap_k2 = cap_k2;
+    a.part_ml = reinterpret_cast<float *>(ws + off_sml);
+    a.part_o = reinterpret_cast<float *>(ws + off_so);
+    a.counters = sc->counters;
+    for (int b = 0; b < batch; ++b) a.past_len[b] = past_len[b];
+    cudaError_t e = brk::launch_decode(kv->q8(), D, kv->tm_dec_k, kv->tm_dec_v, kv->q8() ? kv->tm_dec_s : kv->tm_dec_k,
+                                       a, nsplit, Hkv * mtiles, batch, st, keys > 0 || pdl);
+    if (e != cudaSuccess) return cuda_fail(e, "decode kernel launch");
+    ++ctx->launches;
+    return BRK_OK;
+}
+
+// One linear product (mats 1) or gate-up product (mats 2); arguments checked, device current.
+int run_linear(brk_ctx *ctx, int mats, int rows, int k, int n, const void *x, const uint16_t *const *w,
+               const float *const *bias, int act, const float *residual, void *out, int out_type, brk_scratch *sc,
+               size_t ws_off, cudaStream_t st, bool pdl) {
+    const brk::LinearPlan plan = brk::linear_plan(rows, k, n, mats, ctx->num_sms);
+    brk::LinearArgs a;
+    memset(&a, 0, sizeof(a));
+    a.M = rows, a.K = k, a.n = n;
+    a.nk = plan.nk;
+    a.tiles_m = plan.tiles_m;
+    a.tiles = plan.tiles;
+    a.residual = residual;
+    a.out = out;
+    a.out_half = out_type == BRK_T_F16;
+    a.act = act;
+    a.ws = reinterpret_cast<float *>(static_cast<char *>(sc->ws) + ws_off);
+    a.counters = sc->counters;
+    a.err = ctx->d_err;
+    CUtensorMap tx, tw[2];
+    int rc = make_map(&tx, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, x, (uint64_t)rows, (uint64_t)k, 64u, (uint32_t)plan.nt,
+                      CU_TENSOR_MAP_SWIZZLE_128B);
+    for (int i = 0; !rc && i < mats; ++i) {
+        a.bias[i] = bias[i];
+        rc = make_weight_map(&tw[i], w[i], n, k, 128);
+    }
+    if (rc) return rc;
+    cudaError_t e = brk::launch_linear(mats, plan, tx, tw, a, st, pdl);
+    if (e != cudaSuccess) return cuda_fail(e, "linear kernel launch");
+    ++ctx->launches;
+    return BRK_OK;
+}
+
+// Workspace bytes and counters of a linear product.
+size_t linear_ws(const brk_ctx *ctx, int mats, int rows, int k, int n, size_t *counters) {
+    const brk::LinearPlan plan = brk::linear_plan(rows, k, n, mats, ctx->num_sms);
+    *counters = std::max(*counters, (size_t)plan.tiles);
+    return align256(plan.ws_floats * sizeof(float));
+}
+
+int check_linear(const brk_ctx *ctx, int rows, int k, int n, int act, const char *what) {
+    if (!ctx) return fail(BRK_ERR_INVALID, "null context");
+    if (rows < 0) return fail(BRK_ERR_INVALID, "%s: rows %d < 0", what, rows);
+    if (k < 8 || k % 8) return fail(BRK_ERR_INVALID, "%s: inner width %d (a multiple of 8)", what, k);
+    if (n < 1) return fail(BRK_ERR_INVALID, "%s: width %d < 1", what, n);
+    if (act < BRK_ACT_NONE || act > BRK_ACT_QUICK_GELU) return fail(BRK_ERR_INVALID, "%s: activation %d", what, act);
+    if ((long long)((n + 127) / 128) * ((rows + 15) / 16) >= (1ll << 27))
+        return fail(BRK_ERR_CAPACITY, "%s: %d x %d outputs", what, rows, n);
+    return BRK_OK;
+}
+
+// Whether the byte ranges [a, a + na) and [b, b + nb) meet.
+bool overlap(const void *a, size_t na, const void *b, size_t nb) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return a && b && na && nb && x < y + nb && y < x + na;
+}
+}  // namespace
+
+int brk_attn_decode_prefix(brk_ctx *ctx, const brk_kv *prefix, int prefix_seq, int prefix_len, const brk_kv *kv,
+                           int layer, const brk_attn_params *p, int batch, int n_tokens, const int32_t *past_len,
+                           const void *q, int q_type, void *out, int out_type, void *stream) {
+    int rc = check_prefix_call(ctx, prefix, prefix_seq, prefix_len, kv, layer, p, batch, n_tokens, past_len, q, q_type,
+                               out, out_type);
+    if (rc) return rc;
+    const size_t elems = (size_t)batch * n_tokens * p->n_heads * p->head_dim;
+    if (overlap(q, elems * (q_type == BRK_T_F16 ? 2 : 4), out, elems * (out_type == BRK_T_F16 ? 2 : 4)))
+        return fail(BRK_ERR_INVALID, "out overlaps q");
+    DeviceGuard g(ctx->device);
+    return run_decode_prefix(ctx, prefix, prefix_seq, prefix_len, kv, layer, p, batch, n_tokens, past_len, q, q_type, out,
+                             out_type, static_cast<cudaStream_t>(stream), false);
+}
+
+int brk_attn_step_prefix(brk_ctx *ctx, const brk_kv *prefix, int prefix_seq, int prefix_len, brk_kv *kv, int layer,
+                         const brk_attn_params *p, int batch, int n_tokens, const int32_t *past_len,
+                         const float *q_in, const float *k_in, const float *v_in, float *q_work, void *out,
+                         int out_type, void *stream) {
+    if (!q_in || !k_in || !v_in || !q_work || !out) return fail(BRK_ERR_INVALID, "null tensor argument");
+    int rc = check_prefix_call(ctx, prefix, prefix_seq, prefix_len, kv, layer, p, batch, n_tokens, past_len, q_work,
+                               BRK_T_F32, out, out_type);
+    if (rc) return rc;
+    if (prefix == kv && prefix_len > 0)
+        return fail(BRK_ERR_INVALID, "the step appends to kv, which must not be the prefix cache");
+    const size_t elems = (size_t)batch * n_tokens * p->n_heads * p->head_dim;
+    if (overlap(q_work, elems * 4, out, elems * (out_type == BRK_T_F16 ? 2 : 4)))
+        return fail(BRK_ERR_INVALID, "out overlaps q_work");
+    rc = append_impl(ctx, kv, layer, p, batch, n_tokens, past_len, q_in, k_in, v_in, q_work, stream, true);
+    if (rc) return rc;
+    DeviceGuard g(ctx->device);
+    return run_decode_prefix(ctx, prefix, prefix_seq, prefix_len, kv, layer, p, batch, n_tokens, past_len, q_work,
+                             BRK_T_F32, out, out_type, static_cast<cudaStream_t>(stream), true);
+}
+
+int brk_linear(brk_ctx *ctx, int rows, int k, int n, const uint16_t *x, const uint16_t *w, const float *bias, int act,
+               const float *residual, void *out, int out_type, void *stream) {
+    int rc = check_linear(ctx, rows, k, n, act, "linear");
+    if (rc) return rc;
+    if (out_type != BRK_T_F32 && out_type != BRK_T_F16) return fail(BRK_ERR_INVALID, "out type %d", out_type);
+    if (rows == 0) return BRK_OK;
+    if (!x || !w || !out) return fail(BRK_ERR_INVALID, "null x, w or out");
+    if (!aligned16(x) || !aligned16(w)) return fail(BRK_ERR_INVALID, "x and w must be 16-byte aligned");
+    const size_t esz = out_type == BRK_T_F16 ? 2 : 4, no = (size_t)rows * n * esz;
+    if (reinterpret_cast<uintptr_t>(out) % esz) return fail(BRK_ERR_INVALID, "out is not aligned to its type");
+    if (overlap(out, no, x, (size_t)rows * k * 2) || overlap(out, no, w, (size_t)n * k * 2) ||
+        overlap(out, no, bias, (size_t)n * 4) ||
+        (overlap(out, no, residual, (size_t)rows * n * 4) && !(out == residual && out_type == BRK_T_F32)))
+        return fail(BRK_ERR_INVALID, "out overlaps an input");
+    DeviceGuard g(ctx->device);
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    size_t counters = 0;
+    const size_t bytes = linear_ws(ctx, 1, rows, k, n, &counters);
+    brk_scratch *sc = nullptr;
+    if ((rc = get_scratch(ctx, st, bytes, counters, &sc))) return rc;
+    return run_linear(ctx, 1, rows, k, n, x, &w, &bias, act, residual, out, out_type, sc, 0, st, false);
+}
+
+int brk_ffn_gate_up(brk_ctx *ctx, int rows, int d_model, int d_ff, const uint16_t *x, const uint16_t *w_gate,
+                    const uint16_t *w_up, const float *b_gate, const float *b_up, int act, uint16_t *hidden,
+                    void *stream) {
+    int rc = check_linear(ctx, rows, d_model, d_ff, act, "gate-up");
+    if (rc) return rc;
+    if (rows == 0) return BRK_OK;
+    if (!x || !w_gate || !w_up || !hidden) return fail(BRK_ERR_INVALID, "null x, weight or output");
+    if (!aligned16(x) || !aligned16(w_gate) || !aligned16(w_up))
+        return fail(BRK_ERR_INVALID, "x and the weights must be 16-byte aligned");
+    if (reinterpret_cast<uintptr_t>(hidden) % 2) return fail(BRK_ERR_INVALID, "hidden is not aligned to its type");
+    const size_t no = (size_t)rows * d_ff * 2, nw = (size_t)d_ff * d_model * 2;
+    if (overlap(hidden, no, x, (size_t)rows * d_model * 2) || overlap(hidden, no, w_gate, nw) ||
+        overlap(hidden, no, w_up, nw) || overlap(hidden, no, b_gate, (size_t)d_ff * 4) ||
+        overlap(hidden, no, b_up, (size_t)d_ff * 4))
+        return fail(BRK_ERR_INVALID, "hidden overlaps an input");
+    DeviceGuard g(ctx->device);
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    size_t counters = 0;
+    const size_t bytes = linear_ws(ctx, 2, rows, d_model, d_ff, &counters);
+    brk_scratch *sc = nullptr;
+    if ((rc = get_scratch(ctx, st, bytes, counters, &sc))) return rc;
+    const uint16_t *w[2] = {w_gate, w_up};
+    const float *b[2] = {b_gate, b_up};
+    return run_linear(ctx, 2, rows, d_model, d_ff, x, w, b, act, nullptr, hidden, BRK_T_F16, sc, 0, st, false);
+}
+
+int brk_ffn(brk_ctx *ctx, int rows, int d_model, int d_ff, const float *h, const float *ffn_norm, double eps,
+            int norm_one_plus, const uint16_t *w_gate, const uint16_t *w_up, const uint16_t *w_down,
+            const float *post_norm, int act, float *out, void *stream) {
+    int rc = check_linear(ctx, rows, d_model, d_ff, act, "ffn");
+    if (!rc) rc = check_linear(ctx, rows, d_ff, d_model, act, "ffn");
+    if (rc) return rc;
+    if (rows == 0) return BRK_OK;
+    if (!h || !w_gate || !w_up || !w_down || !out) return fail(BRK_ERR_INVALID, "null input, weight or output");
+    const void *al[] = {h, out, w_gate, w_up, w_down, ffn_norm, post_norm};
+    for (const void *q : al)
+        if (!aligned16(q)) return fail(BRK_ERR_INVALID, "tensors must be 16-byte aligned");
+    const size_t nh = (size_t)rows * d_model * 4, nw = (size_t)d_ff * d_model * 2;
+    if (overlap(out, nh, h, nh) || overlap(out, nh, w_gate, nw) || overlap(out, nh, w_up, nw) ||
+        overlap(out, nh, w_down, nw) || overlap(out, nh, ffn_norm, (size_t)d_model * 4) ||
+        overlap(out, nh, post_norm, (size_t)d_model * 4))
+        return fail(BRK_ERR_INVALID, "out overlaps an input");
+    DeviceGuard g(ctx->device);
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    size_t counters = 0;
+    const size_t ws = std::max(linear_ws(ctx, 2, rows, d_model, d_ff, &counters),
+                               linear_ws(ctx, 1, rows, d_ff, d_model, &counters));
+    const size_t off_x = ws, off_h = off_x + align256((size_t)rows * d_model * 2);
+    brk_scratch *sc = nullptr;
+    if ((rc = get_scratch(ctx, st, off_h + align256((size_t)rows * d_ff * 2), counters, &sc))) return rc;
+    __half *x16 = reinterpret_cast<__half *>(static_cast<char *>(sc->ws) + off_x);
+    __half *hid = reinterpret_cast<__half *>(static_cast<char *>(sc->ws) + off_h);
+    brk::ProjArgs none;
+    memset(&none, 0, sizeof(none));
+    cudaError_t e = brk::launch_norm_cast(h, ffn_norm, (float)eps, norm_one_plus ? 1 : 0, x16, rows, d_model, none, st);
+    if (e != cudaSuccess) return cuda_fail(e, "ffn norm launch");
+    ++ctx->launches;
+    const uint16_t *w[2] = {w_gate, w_up};
+    const float *b[2] = {nullptr, nullptr};
+    rc = run_linear(ctx, 2, rows, d_model, d_ff, x16, w, b, act, nullptr, hid, BRK_T_F16, sc, 0, st, true);
+    if (rc) return rc;
+    rc = run_linear(ctx, 1, rows, d_ff, d_model, hid, &w_down, b, BRK_ACT_NONE, post_norm ? nullptr : h, out, BRK_T_F32, sc,
+                    0, st, true);
+    if (rc || !post_norm) return rc;
+    e = brk::launch_post_norm_residual(out, h, post_norm, (float)eps, norm_one_plus ? 1 : 0, rows, d_model, st);
     if (e != cudaSuccess) return cuda_fail(e, "post-norm launch");
     ++ctx->launches;
     return BRK_OK;

@@ -259,8 +259,11 @@ __device__ __forceinline__ void patch_new_row(uint8_t *st, int rpos, const uint8
 }
 
 // F: the fused-append form (brk_attn_step with one token); a separate instantiation, so that the
-// plain kernel's code and registers stay as they are.
-template <bool Q8, int D, bool F>
+// plain kernel's code and registers stay as they are.  H: the own rows of sequences that share a
+// prefix (brk_attn_decode_prefix): q f32 or fp16, and the final merge takes the prefix kernel's
+// partials in; the cache streams while the prefix kernel still runs (a.late_wait: everything but
+// its partials was complete before this grid could start).
+template <bool Q8, int D, bool F, bool H = false>
 __global__ void __launch_bounds__(decode_threads<Q8, D, F>(), DecodeCfg<Q8, D>::kMinBlocks)
     decode_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
                    const __grid_constant__ CUtensorMap tms, const __grid_constant__ DecodeArgs a) {
@@ -372,7 +375,7 @@ __global__ void __launch_bounds__(decode_threads<Q8, D, F>(), DecodeCfg<Q8, D>::
             // finished; cache rows (and the fused append's inputs) may come from it or, as kernels
             // that trigger their dependents early wait for their own predecessors before they
             // finish, from anything the stream ran before.  The CTA's set-up has overlapped it.
-            griddep_wait();
+            if (!H || !a.late_wait) griddep_wait();
             if constexpr (F && !kRowWarp) {
                 if (writes_row) {
                     // The first ring stages (the new row's among them, unpatched, if it is that
@@ -422,7 +425,7 @@ __global__ void __launch_bounds__(decode_threads<Q8, D, F>(), DecodeCfg<Q8, D>::
         }
     }
 
-    griddep_wait();  // q (or, fused, q_in / k_in / v_in) may come from the preceding kernel
+    if (!H || !a.late_wait) griddep_wait();  // q (or, fused, q_in / k_in / v_in) may come from the preceding kernel
     const int kg = warp % KG;  // key group: keys [16 kg, 16 kg + 16) of every stage
     const int dh = warp / KG;  // head-dim slice [DH dh, DH dh + DH)
     const int qr = lane >> 2, qc = lane & 3;
@@ -490,7 +493,18 @@ __global__ void __launch_bounds__(decode_threads<Q8, D, F>(), DecodeCfg<Q8, D>::
     // Q^T fragments (B operand, column qr = query row row0 + qr), fp32 -> fp16: from global
     // memory, or (fused) from the staged rows.
     uint32_t qf[KS][2];
-    {
+    if (H && a.q16) {
+        // fp16 q: the fragments' pairs as they are.
+        const int rq = row0 + qr;
+        const __half *qrow =
+            rq < nrows ? a.q16 + (((size_t)b * T + rq / G) * a.Hq + kvh * G + rq % G) * D + dh * DH : nullptr;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            const int c0 = Q8 ? W * qc + 4 * ks : ks * 16 + 2 * qc, c1 = Q8 ? c0 + 2 : c0 + 8;
+            qf[ks][0] = qrow ? *reinterpret_cast<const uint32_t *>(qrow + c0) : 0u;
+            qf[ks][1] = qrow ? *reinterpret_cast<const uint32_t *>(qrow + c1) : 0u;
+        }
+    } else {
         const int rq = row0 + qr;
         const float *qrow = nullptr;
         if (rq < nrows)
@@ -808,7 +822,9 @@ __global__ void __launch_bounds__(decode_threads<Q8, D, F>(), DecodeCfg<Q8, D>::
     }
     named_barrier_sync(1, NC * 32);
 
-    if (a.cluster)
+    if constexpr (H)
+        decode_epilogue_prefix<D, KG, NC, kRT>(a, ring, row0, nrows, kvh, mtile, b, split);
+    else if (a.cluster)
         decode_epilogue_cluster<D, KG, NC, kRT>(a, ring, row0, nrows, kvh, b, split);
     else
         decode_epilogue<D, KG, NC, kRT>(a, ring, row0, nrows, kvh, mtile, b, split);
@@ -881,16 +897,16 @@ __global__ void combine_peers_kernel(const __grid_constant__ CombineArgs a, cons
     if (row < a.rows) combine_row(a, row, lane);
 }
 
-template <bool Q8, int D, bool F>
+template <bool Q8, int D, bool F, bool H = false>
 cudaError_t launch_t(const CUtensorMap &tmk, const CUtensorMap &tmv, const CUtensorMap &tms, const DecodeArgs &a,
                       dim3 grid, cudaStream_t s, bool pdl) {
     static unsigned long long configured = 0;  // one bit per device: the opt-in is per device
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev >= 64 || !(configured & (1ull << dev))) {
-        cudaError_t e = cudaFuncSetAttribute(decode_kernel<Q8, D, F>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        cudaError_t e = cudaFuncSetAttribute(decode_kernel<Q8, D, F, H>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                              DecodeLayout<Q8, D>::kSmemBytes);
-        if (e == cudaSuccess) e = cudaFuncSetAttribute(decode_kernel<Q8, D, F>,
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(decode_kernel<Q8, D, F, H>,
                                                        cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e != cudaSuccess) return e;
         if (dev < 64) configured |= 1ull << dev;
@@ -914,12 +930,15 @@ cudaError_t launch_t(const CUtensorMap &tmk, const CUtensorMap &tmv, const CUten
     }
     cfg.attrs = attr;
     cfg.numAttrs = n;
-    return cudaLaunchKernelEx(&cfg, decode_kernel<Q8, D, F>, tmk, tmv, tms, a);
+    return cudaLaunchKernelEx(&cfg, decode_kernel<Q8, D, F, H>, tmk, tmv, tms, a);
 }
 
 template <int D>
 cudaError_t launch_dt(bool q8, bool fused, const CUtensorMap &tmk, const CUtensorMap &tmv, const CUtensorMap &tms,
                       const DecodeArgs &a, dim3 grid, cudaStream_t s, bool pdl) {
+    if (a.with_prefix)
+        return q8 ? launch_t<true, D, false, true>(tmk, tmv, tms, a, grid, s, pdl)
+                  : launch_t<false, D, false, true>(tmk, tmv, tms, a, grid, s, pdl);
     if (q8) return fused ? launch_t<true, D, true>(tmk, tmv, tms, a, grid, s, pdl)
                          : launch_t<true, D, false>(tmk, tmv, tms, a, grid, s, pdl);
     return fused ? launch_t<false, D, true>(tmk, tmv, tms, a, grid, s, pdl)

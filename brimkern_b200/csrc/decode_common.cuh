@@ -199,6 +199,139 @@ __device__ __forceinline__ void decode_epilogue(const DecodeArgs &a, uint8_t *ri
     if (a.push_world) push_finish<NC>(a);
 }
 
+// The epilogue of the own rows of sequences that share a prefix (brk_attn_decode_prefix).  As in
+// decode_epilogue, but what merges a row -- the tile's only CTA, or with split-KV its last -- also
+// takes in the prefix kernel's pre_parts partials of that row and writes the final output, f32 or
+// fp16.  The partials are ordered, so the sums are the same whichever CTA is last.
+template <int D, int KG, int NC, int RT>
+__device__ __forceinline__ void decode_epilogue_prefix(const DecodeArgs &a, uint8_t *ring, int row0, int nrows, int kvh,
+                                                       int mt, int b, int split) {
+    float *cm = reinterpret_cast<float *>(ring);
+    float *cl = cm + KG * RT;
+    float *co = cl + KG * RT;
+    int *flag = reinterpret_cast<int *>(co + KG * RT * D);
+    float *row_l = reinterpret_cast<float *>(flag + 4);  // [RT]
+    float *row_m = row_l + RT;                            // [RT] weight of the rows in shared memory
+    float *wts = row_m + RT;                              // [RT][parts]
+    const int G = a.G, T = a.T;
+    const int nvalid = min(RT, nrows - row0);
+    const int rows_total = a.B * T * a.Hq;
+    auto global_row = [&](int r) {
+        const int rr = row0 + r;
+        return ((size_t)b * T + rr / G) * a.Hq + kvh * G + rr % G;
+    };
+    const bool split_kv = a.nsplit > 1;
+    if (split_kv) {
+        for (int idx = threadIdx.x; idx < nvalid * D; idx += NC * 32) {
+            const int r = idx / D, d = idx % D;
+            float M = -CUDART_INF_F;
+#pragma unroll
+            for (int w = 0; w < KG; ++w) M = fmaxf(M, cm[w * RT + r]);
+            float Lsum = 0.f, O = 0.f;
+            if (M != -CUDART_INF_F) {
+#pragma unroll
+                for (int w = 0; w < KG; ++w) {
+                    const float f = exp2f(cm[w * RT + r] - M);
+                    Lsum += cl[w * RT + r] * f;
+                    O += co[(w * RT + r) * D + d] * f;
+                }
+            }
+            const size_t PR = (size_t)split * rows_total + global_row(r);
+            a.part_o[PR * D + d] = O;
+            if (d == 0) {
+                a.part_ml[PR * 2] = M == -CUDART_INF_F ? -CUDART_INF_F : M * kLn2;
+                a.part_ml[PR * 2 + 1] = Lsum;
+            }
+        }
+        __threadfence();
+        named_barrier_sync(1, NC * 32);
+        if (threadIdx.x == 0) {
+            const int tile = (b * a.Hkv + kvh) * a.mtiles + mt;
+            const int prev = atomicAdd(&a.counters[tile], 1);
+            flag[0] = prev == a.nsplit - 1;
+            if (prev == a.nsplit - 1) a.counters[tile] = 0;  // ready for the next launch
+        }
+        named_barrier_sync(1, NC * 32);
+        if (!flag[0]) return;
+        __threadfence();
+    }
+    if (a.late_wait) griddep_wait();  // the prefix kernel's partials
+    // Partials in memory: the splits' (or none: the rows are in shared memory), then the prefix's.
+    const int nw = split_kv ? a.nsplit : 0, parts = nw + a.pre_parts;
+    auto part_ml = [&](int p, size_t R) {
+        return __ldcg(reinterpret_cast<const float2 *>(
+            p < nw ? &a.part_ml[((size_t)p * rows_total + R) * 2] : &a.pre_ml[((size_t)(p - nw) * rows_total + R) * 2]));
+    };
+    const int mw = threadIdx.x >> 5, ml = threadIdx.x & 31;
+    for (int r = mw; r < nvalid; r += NC) {
+        const size_t R = global_row(r);
+        // Lanes over the partials; the rows in shared memory (log2 units) by the key groups' lanes.
+        float M = -CUDART_INF_F;
+        float2 v[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            v[u] = ml + 32 * u < parts ? part_ml(ml + 32 * u, R) : make_float2(-CUDART_INF_F, 0.f);
+            M = fmaxf(M, v[u].x);
+        }
+        const float own = !split_kv && ml < KG ? cm[ml * RT + r] : -CUDART_INF_F;
+        if (own != -CUDART_INF_F) M = fmaxf(M, own * kLn2);
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
+        float l = 0.f;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const float w = v[u].x == -CUDART_INF_F ? 0.f : expf(v[u].x - M);
+            if (ml + 32 * u < parts) wts[r * parts + ml + 32 * u] = w;
+            l += w * v[u].y;
+        }
+        if (!split_kv && ml < KG) {
+            const float w = own == -CUDART_INF_F ? 0.f : expf(own * kLn2 - M);
+            l += w * cl[ml * RT + r];
+            cm[ml * RT + r] = w;  // from here on: the key group's weight
+        }
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+        if (ml == 0) row_l[r] = l;
+    }
+    named_barrier_sync(1, NC * 32);
+    // Outputs: a thread per (row, 4 head-dim values); eight partials' loads in flight at a time.
+    for (int idx = threadIdx.x; idx < nvalid * (D / 4); idx += NC * 32) {
+        const int r = idx / (D / 4), d4 = idx % (D / 4);
+        const size_t R = global_row(r);
+        float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (!split_kv) {
+#pragma unroll
+            for (int w = 0; w < KG; ++w) {
+                const float f = cm[w * RT + r];
+                const float4 x = *reinterpret_cast<const float4 *>(co + (w * RT + r) * D + 4 * d4);
+                O.x = fmaf(f, x.x, O.x), O.y = fmaf(f, x.y, O.y), O.z = fmaf(f, x.z, O.z), O.w = fmaf(f, x.w, O.w);
+            }
+        }
+        for (int p0 = 0; p0 < parts; p0 += 8) {
+            float4 v[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int p = p0 + u;
+                const float *src = p < nw ? a.part_o + ((size_t)p * rows_total + R) * D
+                                          : a.pre_o + ((size_t)(p - nw) * rows_total + R) * D;
+                v[u] = p < parts ? __ldcg(reinterpret_cast<const float4 *>(src) + d4) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const float w = p0 + u < parts ? wts[r * parts + p0 + u] : 0.f;
+                O.x = fmaf(w, v[u].x, O.x), O.y = fmaf(w, v[u].y, O.y), O.z = fmaf(w, v[u].z, O.z),
+                O.w = fmaf(w, v[u].w, O.w);
+            }
+        }
+        const float inv = 1.f / row_l[r];
+        O.x *= inv, O.y *= inv, O.z *= inv, O.w *= inv;
+        if (a.out16)
+            *reinterpret_cast<uint2 *>(a.out16 + R * D + 4 * d4) = make_uint2(pack_half2(O.x, O.y), pack_half2(O.z, O.w));
+        else
+            *reinterpret_cast<float4 *>(a.out + R * D + 4 * d4) = O;
+    }
+}
+
 // Split-KV merge across a thread-block cluster (the splits of one (sequence, kv head, row
 // tile) launched as one cluster, split = rank): each CTA keeps its split's (m, l, o) rows in its
 // own shared memory behind cm / cl / co, the cluster synchronises, every CTA merges a slice of

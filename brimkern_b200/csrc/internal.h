@@ -9,7 +9,23 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <vector>
+
 #include "brk_attn.h"
+
+// Scratch of one stream (or of one stream capture) for the operators that keep theirs apart by
+// stream: partials / staging, and arrival counters that are zero between launches.  Calls on two
+// streams, and graphs captured one by one, so never share it.  A buffer that has become too small
+// is kept until the context goes (queued kernels and captured graphs may still use it).
+struct brk_scratch {
+    unsigned long long id = 0;   // stream id, or capture id
+    bool capture = false;
+    void *ws = nullptr;
+    size_t ws_bytes = 0;
+    int *counters = nullptr;
+    size_t counters_n = 0;
+    std::vector<void *> retired;
+};
 
 struct brk_ctx {
     int device = 0;
@@ -28,6 +44,8 @@ struct brk_ctx {
     void *act = nullptr;       // fp16 activations of the projection GEMMs
     size_t act_bytes = 0;
     uint64_t launches = 0;     // kernels launched through this context
+    cudaStream_t aux = nullptr;  // zeroes new counters (never captured)
+    std::vector<brk_scratch *> scratch;
 };
 
 // This rank's exchange area for sequence-sharded decode over peer memory (brk_attn_decode_push /
@@ -147,6 +165,36 @@ struct DecodeArgs {
     const float *q_norm, *k_norm;
     double eps;
     int one_plus;
+    // Own rows of sequences that share a prefix (brk_attn_decode_prefix, decode_kernel's H form):
+    // q in fp16 (or a.q in f32), the prefix kernel's pre_parts partials [part][rows][2] and
+    // [part][rows][D], the fp16 output (or a.out), and whether the preceding kernel of this call
+    // is the prefix kernel, whose partials alone have to be waited for.
+    int with_prefix;
+    int late_wait;
+    int pre_parts;
+    const __half *q16;
+    const float *pre_ml, *pre_o;
+    __half *out16;
+    int past_len[BRK_MAX_BATCH];
+};
+
+// Attention of every sequence's query rows over one shared prefix (prefix.cu): partials only.
+struct PrefixArgs {
+    const float *q;       // [B][T][Hq][D] f32, or
+    const __half *q16;    //   fp16
+    float *part_ml;       // [split][B*T*Hq][2] (m natural-log units, l)
+    float *part_o;        // [split][B*T*Hq][D] unnormalised
+    const float *scales;  // int8 cache: this (layer, sequence)'s [kv head][2][scale_pitch], or nullptr
+    int scale_pitch;
+    int *err;
+    int B, T, Hq, Hkv, G;
+    int rows;             // query rows per kv head: B * T * G
+    int row0;             // map row of key 0 of kv head 0
+    int head_rows;        // map rows from one kv head to the next
+    int k_begin, k_end;   // keys some row attends
+    int tiles_per_split;
+    int window;
+    float scale_log2, softcap, cap_k1, cap_k2;
     int past_len[BRK_MAX_BATCH];
 };
 
@@ -180,6 +228,28 @@ struct ProjArgs {
     const float *residual;    // [M][n[0]] added to matrix 0 (or null)
     int splits, kps;          // split-K factor and k steps (of 64) per split (proj_plan)
     int *err;
+};
+
+// Linear operators (linear.cu): act(x W^T + bias) + residual, or act(x W0^T + b0) * (x W1^T + b1).
+struct LinearArgs {
+    int M, K, n;              // tokens, inner width, output features
+    int nk, tiles_m;          // k steps of 64; token tiles (a tile index is feature tile * tiles_m + token tile)
+    long long tiles;
+    const float *bias[2];     // [n] or null
+    const float *residual;    // [M][n] f32 or null
+    void *out;                // [M][n] f32, or fp16
+    int out_half;
+    int act;                  // BRK_ACT_*
+    float *ws;                // partial tiles [CTA][2][matrix][token][128]
+    int *counters;            // [tiles] finished pieces, zero between launches
+    int *err;
+};
+
+// How a linear product is cut: tokens per tile, tiles, k steps, CTAs, workspace floats.
+struct LinearPlan {
+    int nt, tiles_m, nk, grid;
+    long long tiles;
+    size_t ws_floats;
 };
 
 struct CombineArgs {
@@ -251,6 +321,22 @@ cudaError_t launch_post_norm_residual(float *h, const float *x, const float *gai
                                       int n, cudaStream_t s);
 cudaError_t launch_proj(int ntok, const CUtensorMap &tx, const CUtensorMap *tw, const CUtensorMap *to,
                         const ProjArgs &a, cudaStream_t s);
+
+// Linear operators (linear.cu); mats 1 or 2.  tx has boxes of plan.nt rows, tw of 128 rows.
+LinearPlan linear_plan(int rows, int k, int n, int mats, int sms);
+cudaError_t launch_linear(int mats, const LinearPlan &p, const CUtensorMap &tx, const CUtensorMap *tw,
+                          const LinearArgs &a, cudaStream_t s, bool pdl);
+
+// Shared-prefix attention partials (prefix.cu): maps with prefix_tile_keys()-row boxes over fp16
+// rows (for an int8 cache: its codes as fp16, staged by launch_codes_to_half).  Query rows per CTA
+// for a head dim and row count: prefix_block_rows().
+int prefix_tile_keys();
+int prefix_block_rows(int head_dim, int rows);
+cudaError_t launch_prefix(int head_dim, const CUtensorMap &tmk, const CUtensorMap &tmv, const PrefixArgs &a, int splits,
+                          cudaStream_t s, bool pdl);
+// Codes of rows [row0, row0 + rows) of every kv head of one (layer, sequence) as fp16 [Hkv][rows][D].
+cudaError_t launch_codes_to_half(const uint8_t *kc, const uint8_t *vc, __half *k, __half *v, int n_kv_heads,
+                                 int head_dim, int cap, int row0, int rows, cudaStream_t s);
 
 // Non-causal attention staging (full.cu): token-major f32 [B][L][H][D] K/V -> head-major fp16
 // [B][H][L][Dp] (zero-padded head dim), and f32 rows [rows][D] -> [rows][Dp] zero-padded.

@@ -41,6 +41,9 @@ def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
 
+_T_TYPES = {torch.float32: L.BRK_T_F32, torch.float16: L.BRK_T_F16}
+
+
 def _positions(past_len, batch: int):
     arr = (ctypes.c_int32 * batch)()
     vals = [int(past_len)] * batch if np.isscalar(past_len) else [int(x) for x in past_len]
@@ -632,6 +635,135 @@ class AttentionEngine:
         pos = _positions(past_len, B)
         check(L.lib().brk_attn_decode_partial(self.ctx.handle, kv.handle, layer, ctypes.byref(p), B, T, pos, _ptr(q),
                                               _ptr(part_ml), _ptr(part_o), _stream_ptr(stream)))
+
+    # ---- decode over a shared prefix, and the linear operators (extensions; the FFN of
+    # recordLayerKV, kernels.ts:1737-1744) ---------------------------------------------------
+    def _tensor(self, t: torch.Tensor, name: str, dtypes, shape) -> int:
+        """The address of a tensor that the kernels read or write as it is: on this engine's device,
+        of one of `dtypes`, contiguous, of `shape` (None: not checked)."""
+        if t.device != self.device:
+            raise BrkError(L.BRK_ERR_INVALID, f"{name} is on {t.device}, the engine on {self.device}")
+        if t.dtype not in dtypes:
+            raise BrkError(L.BRK_ERR_INVALID, f"{name} is {t.dtype}, not {' or '.join(map(str, dtypes))}")
+        if shape is not None and tuple(t.shape) != shape:
+            raise BrkError(L.BRK_ERR_INVALID, f"{name} has shape {tuple(t.shape)}, not {shape}")
+        if not t.is_contiguous():
+            raise BrkError(L.BRK_ERR_INVALID, f"{name} is not contiguous")
+        return t.data_ptr()
+
+    def _stream(self, stream: Optional[torch.cuda.Stream]) -> int:
+        """The given stream, or the current one of this engine's device."""
+        return (stream if stream is not None else torch.cuda.current_stream(self.device)).cuda_stream
+
+    @staticmethod
+    def _activation(act: str) -> int:
+        try:
+            return L.ACTIVATIONS[act]
+        except KeyError:
+            raise BrkError(L.BRK_ERR_INVALID, f"activation {act!r} (one of {', '.join(L.ACTIVATIONS)})") from None
+
+    def _prefix_tokens(self, kv: KvCache, cfg: AttnConfig, q: torch.Tensor, name: str) -> int:
+        per = kv.batch * cfg.n_heads * cfg.head_dim
+        if per < 1 or q.numel() % per or q.numel() == 0:
+            raise BrkError(L.BRK_ERR_INVALID, f"{name} has {q.numel()} elements, not a multiple of batch * heads * dim {per}")
+        return q.numel() // per
+
+    def decodePrefix(self, prefix: Optional[KvCache], prefix_len: int, kv: KvCache, layer: int, cfg: AttnConfig,
+                     q: torch.Tensor, out: torch.Tensor, past_len, prefix_seq: int = 0, stream=None) -> torch.Tensor:
+        """Decode attention of a batch over a prefix that all its sequences share (sequence
+        `prefix_seq` of the cache `prefix`, positions [0, prefix_len)) and each sequence's own rows
+        (`kv`, row r at position prefix_len + r; cfg.kv_offset == prefix_len).  q [B, T, Hq, D]
+        (rotated) f32 or fp16 -> out of the same shape, f32 or fp16."""
+        T = self._prefix_tokens(kv, cfg, q, "q")
+        qp = self._tensor(q, "q", _T_TYPES, None)
+        op = self._tensor(out, "out", _T_TYPES, None)
+        if out.numel() != q.numel():
+            raise BrkError(L.BRK_ERR_INVALID, f"out has {out.numel()} elements, q has {q.numel()}")
+        p = cfg.params()
+        check(L.lib().brk_attn_decode_prefix(self.ctx.handle, prefix.handle if prefix is not None else None,
+                                             int(prefix_seq), int(prefix_len), kv.handle, layer, ctypes.byref(p), kv.batch,
+                                             T, _positions(past_len, kv.batch), qp, _T_TYPES[q.dtype], op,
+                                             _T_TYPES[out.dtype], self._stream(stream)))
+        return out
+
+    def stepPrefix(self, prefix: Optional[KvCache], prefix_len: int, kv: KvCache, layer: int, cfg: AttnConfig,
+                   q_in: torch.Tensor, k_in: torch.Tensor, v_in: torch.Tensor, past_len, prefix_seq: int = 0,
+                   q_work: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                   stream=None) -> torch.Tensor:
+        """attentionLayer over a shared prefix: the new tokens' K / V appended to `kv` (QK-norm and
+        RoPE as appendKv), then decodePrefix.  q_in [B, T, Hq, D], k_in / v_in [B, T, Hkv, D] f32
+        projections; out f32 (default) or fp16."""
+        T = self._prefix_tokens(kv, cfg, q_in, "q_in")
+        f32, n_kv = (torch.float32,), kv.batch * T * cfg.n_kv_heads * cfg.head_dim
+        q_work = torch.empty_like(q_in) if q_work is None else q_work
+        out = torch.empty_like(q_in) if out is None else out
+        ptrs = [self._tensor(t, n, f32, None) for t, n in ((q_in, "q_in"), (k_in, "k_in"), (v_in, "v_in"), (q_work, "q_work"))]
+        op = self._tensor(out, "out", _T_TYPES, None)
+        for t, n, want in ((k_in, "k_in", n_kv), (v_in, "v_in", n_kv), (q_work, "q_work", q_in.numel()),
+                           (out, "out", q_in.numel())):
+            if t.numel() != want:
+                raise BrkError(L.BRK_ERR_INVALID, f"{n} has {t.numel()} elements, not {want}")
+        p = cfg.params()
+        check(L.lib().brk_attn_step_prefix(self.ctx.handle, prefix.handle if prefix is not None else None, int(prefix_seq),
+                                           int(prefix_len), kv.handle, layer, ctypes.byref(p), kv.batch, T,
+                                           _positions(past_len, kv.batch), *ptrs, op, _T_TYPES[out.dtype],
+                                           self._stream(stream)))
+        return out
+
+    def linear(self, x: torch.Tensor, w: torch.Tensor, out: torch.Tensor, bias: Optional[torch.Tensor] = None,
+               act: str = "none", residual: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
+        """out = act(x w^T + bias) + residual.  x [rows, k] fp16, w [n, k] fp16, bias [n] f32,
+        residual [rows, n] f32, out [rows, n] f32 or fp16 (f32: may be the residual itself)."""
+        f16, f32 = (torch.float16,), (torch.float32,)
+        if x.dim() != 2 or w.dim() != 2:
+            raise BrkError(L.BRK_ERR_INVALID, f"x and w are matrices, not {tuple(x.shape)} and {tuple(w.shape)}")
+        rows, k = x.shape
+        n = w.shape[0]
+        check(L.lib().brk_linear(self.ctx.handle, rows, k, n, self._tensor(x, "x", f16, None),
+                                 self._tensor(w, "w", f16, (n, k)),
+                                 None if bias is None else self._tensor(bias, "bias", f32, (n,)), self._activation(act),
+                                 None if residual is None else self._tensor(residual, "residual", f32, (rows, n)),
+                                 self._tensor(out, "out", _T_TYPES, (rows, n)), _T_TYPES[out.dtype],
+                                 self._stream(stream)))
+        return out
+
+    def ffnGateUp(self, x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, hidden: torch.Tensor,
+                  act: str = "silu", b_gate: Optional[torch.Tensor] = None, b_up: Optional[torch.Tensor] = None,
+                  stream=None) -> torch.Tensor:
+        """hidden = act(x w_gate^T + b_gate) * (x w_up^T + b_up).  x [rows, d] fp16, weights [ff, d]
+        fp16, biases [ff] f32, hidden [rows, ff] fp16."""
+        f16, f32 = (torch.float16,), (torch.float32,)
+        if x.dim() != 2 or w_gate.dim() != 2:
+            raise BrkError(L.BRK_ERR_INVALID, f"x and w_gate are matrices, not {tuple(x.shape)} and {tuple(w_gate.shape)}")
+        rows, d = x.shape
+        ff = w_gate.shape[0]
+        check(L.lib().brk_ffn_gate_up(self.ctx.handle, rows, d, ff, self._tensor(x, "x", f16, None),
+                                      self._tensor(w_gate, "w_gate", f16, (ff, d)),
+                                      self._tensor(w_up, "w_up", f16, (ff, d)),
+                                      None if b_gate is None else self._tensor(b_gate, "b_gate", f32, (ff,)),
+                                      None if b_up is None else self._tensor(b_up, "b_up", f32, (ff,)),
+                                      self._activation(act), self._tensor(hidden, "hidden", f16, (rows, ff)),
+                                      self._stream(stream)))
+        return hidden
+
+    def ffn(self, h: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor, out: torch.Tensor,
+            ffn_norm: Optional[torch.Tensor] = None, eps: float = 1e-6, one_plus: bool = False, act: str = "silu",
+            post_norm: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
+        """The feed-forward half of a layer: out = h + w_down (act(w_gate x) * (w_up x)) with
+        x = rmsnorm(h, ffn_norm) (Gemma-2: the block's output normed by post_norm before the add).
+        h / out [rows, d] f32, w_gate / w_up [ff, d] and w_down [d, ff] fp16."""
+        f16, f32 = (torch.float16,), (torch.float32,)
+        if h.dim() != 2 or w_gate.dim() != 2:
+            raise BrkError(L.BRK_ERR_INVALID, f"h and w_gate are matrices, not {tuple(h.shape)} and {tuple(w_gate.shape)}")
+        rows, d = h.shape
+        ff = w_gate.shape[0]
+        check(L.lib().brk_ffn(self.ctx.handle, rows, d, ff, self._tensor(h, "h", f32, None),
+                              None if ffn_norm is None else self._tensor(ffn_norm, "ffn_norm", f32, (d,)), float(eps),
+                              int(bool(one_plus)), self._tensor(w_gate, "w_gate", f16, (ff, d)),
+                              self._tensor(w_up, "w_up", f16, (ff, d)), self._tensor(w_down, "w_down", f16, (d, ff)),
+                              None if post_norm is None else self._tensor(post_norm, "post_norm", f32, (d,)),
+                              self._activation(act), self._tensor(out, "out", f32, (rows, d)), self._stream(stream)))
+        return out
 
     # ---- the projections either side of the operator (recordLayerKV, kernels.ts:1700-1736) -----
     def projQkv(self, x: torch.Tensor, wq: torch.Tensor, wk: torch.Tensor, wv: torch.Tensor,

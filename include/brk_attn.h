@@ -47,6 +47,14 @@ enum {
  * V (quantize_kv, shaders.ts:1673-1705), half the bytes of fp16. */
 enum { BRK_KV_F16 = 0, BRK_KV_I8 = 1 };
 
+/* Element types of the tensors that some entry points take in either. */
+enum { BRK_T_F32 = 0, BRK_T_F16 = 1 };
+
+/* Activations of the linear operators, in f32: silu x / (1 + e^-x) (LayerCfg.act "silu"), gelu
+ * x (1 + erf(x / sqrt 2)) / 2, gelu_tanh x (1 + tanh(sqrt(2 / pi) (x + 0.044715 x^3))) / 2 (Gemma's
+ * "gelu"), quick_gelu x / (1 + e^(-1.702 x)) (CLIP). */
+enum { BRK_ACT_NONE = 0, BRK_ACT_SILU = 1, BRK_ACT_GELU = 2, BRK_ACT_GELU_TANH = 3, BRK_ACT_QUICK_GELU = 4 };
+
 typedef struct brk_ctx brk_ctx;   /* one per GPU: device id, error flag, workspace */
 typedef struct brk_kv brk_kv;     /* persistent KV cache of n_layers layers (KvEntry, kernels.ts:93) */
 typedef struct brk_rope brk_rope; /* RoPE cos/sin table in HBM */
@@ -268,6 +276,58 @@ int brk_attn_decode_partial(brk_ctx *ctx, const brk_kv *kv, int layer,
  * N GPUs is combined with part_ml = buf, part_o = buf + 2*rows, part_stride = rows*(2+head_dim). */
 int brk_attn_combine(brk_ctx *ctx, int n_parts, int rows, int head_dim, const float *part_ml,
                      const float *part_o, size_t part_stride, float *out, void *stream);
+
+/* ---- decode over a shared prefix (extension, no reference counterpart) -----------------------
+ * Decode attention of a batch whose sequences all begin with the same prefix_len positions (a system
+ * prompt, one document, several answers to one question): the prefix's rows are held once, in
+ * sequence prefix_seq of the cache `prefix`, and read once for the whole batch; `kv` holds each
+ * sequence's own rows, row r at position prefix_len + r, so p->kv_offset must equal prefix_len (and
+ * brk_attn_append / brk_attn_step's append place the new rows with the same parameters).  Token t of
+ * sequence b sits at position past_len[b] + t (past_len counts the prefix) and attends the prefix
+ * and own rows [prefix_len, past_len[b] + t], or the last p->window of those positions.  The result
+ * is brk_attn_decode's over a cache that holds prefix and own rows one after the other, up to
+ * rounding.
+ *   - Both caches hold `layer`, with the same kv heads and head_dim; each may be fp16 or int8.
+ *     prefix may be NULL with prefix_len 0.  Rows of the prefix from the first attended position on
+ *     must be finite (a masked row's V still meets a probability of 0 in the product).
+ *   - q and out [batch][n_tokens][n_heads][head_dim], each f32 or fp16 by q_type / out_type (BRK_T_*),
+ *     16-byte aligned, not overlapping.  n_tokens * (n_heads / n_kv_heads) <= 64.
+ *   - Scratch (partials; for an int8 prefix its codes as fp16, 4 bytes per code of the attended
+ *     rows of one layer) belongs to the stream, or to the stream capture, that the call is made on:
+ *     calls on several streams, and graphs captured one after the other, may run at the same time.
+ *     It grows at the first call that needs more (also while capturing) and lives until
+ *     brk_ctx_destroy, which must come after the last replay of such graphs. */
+int brk_attn_decode_prefix(brk_ctx *ctx, const brk_kv *prefix, int prefix_seq, int prefix_len, const brk_kv *kv,
+                           int layer, const brk_attn_params *p, int batch, int n_tokens, const int32_t *past_len,
+                           const void *q, int q_type, void *out, int out_type, void *stream);
+/* One decode step of a layer over a shared prefix: brk_attn_append of the new tokens into kv (rotated
+ * q to q_work f32), then the above.  out f32 or fp16. */
+int brk_attn_step_prefix(brk_ctx *ctx, const brk_kv *prefix, int prefix_seq, int prefix_len, brk_kv *kv, int layer,
+                         const brk_attn_params *p, int batch, int n_tokens, const int32_t *past_len,
+                         const float *q_in, const float *k_in, const float *v_in, float *q_work, void *out,
+                         int out_type, void *stream);
+
+/* ---- linear operators on fp16 activations (the FFN of recordLayerKV, kernels.ts:1737-1744) -----
+ * Weights are the engine's fp16 matrices [n][k] (C = A W^T), activations x fp16 [rows][k], biases
+ * f32 [n] or NULL; sums in f32.  k is a multiple of 8, x and the weights 16-byte aligned; rows (0:
+ * nothing is done) and n are any size.  Results do not change from run to run.  Scratch as for
+ * brk_attn_decode_prefix: by stream or stream capture.  Outputs may not overlap inputs, except
+ * brk_linear's f32 out, which may be its residual.
+ *   brk_linear:      out = act(x w^T + bias) + residual    (residual f32 [rows][n] or NULL)
+ *                    out f32 or fp16 [rows][n] by out_type.
+ *   brk_ffn_gate_up: hidden = act(x w_gate^T + b_gate) * (x w_up^T + b_up), fp16 [rows][d_ff].
+ *   brk_ffn:         the whole block: out = h + ffn(rmsnorm(h, ffn_norm)), f32 [rows][d_model], with
+ *                    ffn(x) = w_down (act(w_gate x) * (w_up x)); with post_norm (Gemma-2) out = h +
+ *                    rmsnorm(ffn(...), post_norm).  ffn_norm NULL: no norm.  d_model and d_ff
+ *                    multiples of 8.  out may not alias h. */
+int brk_linear(brk_ctx *ctx, int rows, int k, int n, const uint16_t *x, const uint16_t *w, const float *bias, int act,
+               const float *residual, void *out, int out_type, void *stream);
+int brk_ffn_gate_up(brk_ctx *ctx, int rows, int d_model, int d_ff, const uint16_t *x, const uint16_t *w_gate,
+                    const uint16_t *w_up, const float *b_gate, const float *b_up, int act, uint16_t *hidden,
+                    void *stream);
+int brk_ffn(brk_ctx *ctx, int rows, int d_model, int d_ff, const float *h, const float *ffn_norm, double eps,
+            int norm_one_plus, const uint16_t *w_gate, const uint16_t *w_up, const uint16_t *w_down,
+            const float *post_norm, int act, float *out, void *stream);
 
 /* ---- the projections either side of the operator (recordLayerKV, kernels.ts:1700-1736) -------
  * The layer-input RMSNorm with the q / k / v projections that feed brk_attn_append / step, and
