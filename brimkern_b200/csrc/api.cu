@@ -1616,10 +1616,10 @@ int run_linear(brk_ctx *ctx, int mats, int rows, int k, int n, const void *x, co
     const brk::LinearPlan plan = brk::linear_plan(rows, k, n, mats, ctx->num_sms);
     brk::LinearArgs a;
     memset(&a, 0, sizeof(a));
-    a.M = rows, a.K = k, a.n = n;
-    a.nk = plan.nk;
-    a.tiles_m = plan.tiles_m;
-    a.tiles = plan.tiles;
+    a.M = rows, a.n = n;
+    a.nk = plan.nk, a.nt = plan.nt, a.tiles_m = plan.tiles_m;
+    a.half_cols = plan.half_cols;
+    a.tiles = plan.tiles, a.tiles_whole = plan.tiles_whole;
     a.residual = residual;
     a.out = out;
     a.out_half = out_type == BRK_T_F16;
@@ -1628,7 +1628,7 @@ int run_linear(brk_ctx *ctx, int mats, int rows, int k, int n, const void *x, co
     a.counters = sc->counters;
     a.err = ctx->d_err;
     CUtensorMap tx, tw[2];
-    int rc = make_map(&tx, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, x, (uint64_t)rows, (uint64_t)k, 64u, (uint32_t)plan.nt,
+    int rc = make_map(&tx, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, x, (uint64_t)rows, (uint64_t)k, 64u, (uint32_t)plan.x_rows,
                       CU_TENSOR_MAP_SWIZZLE_128B);
     for (int i = 0; !rc && i < mats; ++i) {
         a.bias[i] = bias[i];
@@ -1644,7 +1644,7 @@ int run_linear(brk_ctx *ctx, int mats, int rows, int k, int n, const void *x, co
 // Workspace bytes and counters of a linear product.
 size_t linear_ws(const brk_ctx *ctx, int mats, int rows, int k, int n, size_t *counters) {
     const brk::LinearPlan plan = brk::linear_plan(rows, k, n, mats, ctx->num_sms);
-    *counters = std::max(*counters, (size_t)plan.tiles);
+    *counters = std::max(*counters, plan.counters);
     return align256(plan.ws_floats * sizeof(float));
 }
 

@@ -232,24 +232,26 @@ struct ProjArgs {
 
 // Linear operators (linear.cu): act(x W^T + bias) + residual, or act(x W0^T + b0) * (x W1^T + b1).
 struct LinearArgs {
-    int M, K, n;              // tokens, inner width, output features
-    int nk, tiles_m;          // k steps of 64; token tiles (a tile index is feature tile * tiles_m + token tile)
-    long long tiles;
+    int M, n;                 // tokens, output features
+    int nk, nt, tiles_m;      // k steps of 64; tokens per tile; token tiles (tile = feature tile * tiles_m + token tile)
+    int half_cols;            // tokens of a tile that an epilogue warp takes (one or two per lane quarter)
+    long long tiles, tiles_whole;  // tiles; the first of them that are done whole, wave by wave
     const float *bias[2];     // [n] or null
     const float *residual;    // [M][n] f32 or null
     void *out;                // [M][n] f32, or fp16
     int out_half;
     int act;                  // BRK_ACT_*
     float *ws;                // partial tiles [CTA][2][matrix][token][128]
-    int *counters;            // [tiles] finished pieces, zero between launches
+    int *counters;            // [ranged tiles][CTAs per tile] finished pieces, zero between launches
     int *err;
 };
 
-// How a linear product is cut: tokens per tile, tiles, k steps, CTAs, workspace floats.
+// How a linear product is cut: the kernel's token tile, tokens per tile, rows of a TMA box of x,
+// tiles, k steps, CTAs, workspace floats and counters.
 struct LinearPlan {
-    int nt, tiles_m, nk, grid;
-    long long tiles;
-    size_t ws_floats;
+    int nt_kernel, nt, x_rows, half_cols, tiles_m, nk, ctas;
+    long long tiles, tiles_whole;
+    size_t ws_floats, counters;
 };
 
 struct CombineArgs {
@@ -322,7 +324,7 @@ cudaError_t launch_post_norm_residual(float *h, const float *x, const float *gai
 cudaError_t launch_proj(int ntok, const CUtensorMap &tx, const CUtensorMap *tw, const CUtensorMap *to,
                         const ProjArgs &a, cudaStream_t s);
 
-// Linear operators (linear.cu); mats 1 or 2.  tx has boxes of plan.nt rows, tw of 128 rows.
+// Linear operators (linear.cu); mats 1 or 2.  tx has boxes of plan.x_rows rows, tw of 128 rows.
 LinearPlan linear_plan(int rows, int k, int n, int mats, int sms);
 cudaError_t launch_linear(int mats, const LinearPlan &p, const CUtensorMap &tx, const CUtensorMap *tw,
                           const LinearArgs &a, cudaStream_t s, bool pdl);

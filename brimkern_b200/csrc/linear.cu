@@ -2,22 +2,27 @@
 // operator y = act(x W^T + b) + r and the gated feed-forward's first half
 // h = act(x Wg^T + bg) * (x Wu^T + bu) (the FFN of recordLayerKV, kernels.ts:1737-1744).
 //
-// linear_kernel<NT, MATS> computes D^T = W X^T on tcgen05: 128 weight rows (output features) on
-// the MMA's M, up to NT = 16 .. 128 tokens on its N, so a single token pads 15 MMA columns and
-// not 127 rows.  With MATS = 2 a CTA holds the gate and the up tile of the same 128 features in two
-// accumulators, and the product leaves through one epilogue.
+// linear_kernel<NT, MATS, PAIR, DRAIN> computes D^T = W X^T on tcgen05: weight rows (output features) on the
+// MMA's M, up to NT tokens on its N, so a single token pads 15 MMA columns and not 127 rows, and the
+// token tile follows the row count in steps of 16 (32).  PAIR: two SMs of a cluster work on one tile
+// (cta_group::2, M 256): each holds its 128 features' weights and half of the tokens, so a k step
+// costs an SM half the activation bytes.  With MATS = 2 a CTA holds the gate and the up tile of the
+// same features in two accumulators, and the product leaves through one epilogue.
 //
-// Few tokens are bound by streaming the weights once (2 n k bytes a matrix), so what counts is
-// that every SM streams all the time: the (tile, k step) units of the whole product are dealt to
-// one CTA per SM in equal contiguous ranges.  A range's first and last piece may cover part of a
-// tile's k range; such pieces leave f32 partials in the workspace, and the last CTA of a tile to
+// Work is dealt so that every SM has the same amount: first whole waves of tiles (neighbouring CTAs
+// on neighbouring token tiles, so they share weights in L2), the last one to two waves' tiles as
+// (tile, k step) units in equal contiguous ranges.  A range's first and last piece may cover part
+// of a tile's k; such pieces leave f32 partials in the workspace, and the last CTA of a tile to
 // finish adds them in k order (the same order whoever is last: results do not change from run to
-// run).
+// run).  The ranges come first, so that the joins run under the whole tiles.  Few tokens, bound by
+// streaming the weights once, have nothing but ranges.
 //
 // The tensor core's f32 accumulation truncates: its error is a bias that grows with k (measured on
-// N(0,1) operands against 64 bits: 3.1e-6 of the result at k 2560, 1.2e-5 at 10240).  Linear
-// outputs may be f32, so its accumulators are drained every kDrainSteps k steps and the parts added
-// in registers; gate-up outputs are fp16 (half a step 4.9e-4), which does not need it.
+// N(0,1) operands against 64 bits: 3.1e-6 of the result at k 2560, 1.2e-5 at 10240).  For f32
+// outputs (DRAIN) the accumulators are drained every kDrainSteps k steps and the parts added in
+// registers; fp16 outputs (half a step 4.9e-4) do not need it.
+#include <algorithm>
+
 #include "common.cuh"
 #include "internal.h"
 #include "tcgen05.cuh"
@@ -26,47 +31,96 @@ namespace brk {
 
 namespace {
 
-constexpr int kLF = 128;      // output features per tile (MMA M, TMEM lanes)
-constexpr int kLK = 64;       // k per step: one 128-byte swizzled row
-constexpr int kLThreads = 192;
-constexpr int kLProducer = 4, kLMma = 5;
+constexpr int kLF = 128;         // output features per CTA and tile (TMEM lanes)
+constexpr int kLK = 64;          // k per step: one 128-byte swizzled row
 constexpr int kDrainSteps = 16;  // 1024 of k per accumulator
 
-template <int NT, int MATS>
+template <int NT, int MATS, bool PAIR>
 struct LinearLayout {
+    static constexpr int kCtas = PAIR ? 2 : 1;
     static constexpr uint32_t kWBox = kLF * 128;
-    static constexpr uint32_t kXBox = NT * 128;
+    static constexpr uint32_t kXBox = NT / kCtas * 128;
     static constexpr uint32_t kStageBytes = MATS * kWBox + kXBox;
-    static constexpr int kFit = (200 * 1024) / kStageBytes;
+    static constexpr int kFit = (204 * 1024) / kStageBytes;
     static constexpr int kStages = kFit < 12 ? kFit : 12;
-    static constexpr uint32_t kCols = MATS * NT;                       // one accumulator set
-    static constexpr uint32_t kTmemCols = 2 * kCols < 32 ? 32 : 2 * kCols;  // double-buffered
+    static constexpr uint32_t kCols = MATS * NT;                  // one accumulator set
+    static constexpr int kBufs = 2 * kCols <= 512 ? 2 : 1;
+    static constexpr uint32_t kTmemCols = kBufs * kCols < 32 ? 32 : kBufs * kCols;
+    static constexpr int kHalves = NT >= 64 ? 2 : 1;              // epilogue warps per TMEM lane quarter
+    static constexpr int kEpiWarps = 4 * kHalves;
+    static constexpr int kEpiCols = NT / kHalves;                 // columns of an epilogue thread
+    static constexpr int kChunk = 16;                             // columns handled at a time
+    static constexpr int kProducer = kEpiWarps, kMma = kEpiWarps + 1;
+    static constexpr int kThreads = (kEpiWarps + 2) * 32;
     static constexpr uint32_t kBarOff = kStages * kStageBytes;
     static constexpr uint32_t kSmemBytes = 1024 + kBarOff + (2 * kStages + 4) * 8 + 16;
-    static constexpr int kSegSteps = MATS == 1 ? kDrainSteps : 1 << 30;
     static_assert(kTmemCols <= 512 && (kTmemCols & (kTmemCols - 1)) == 0, "TMEM columns");
-    static_assert(kSmemBytes <= 232448, "more than 227 KB of shared memory per CTA");
+    static_assert(kSmemBytes <= 232448 - 64, "more than 227 KB of shared memory per CTA");
 };
 
-// The unit ranges of the grid's CTAs: CTA c of G takes units [c U / G, (c + 1) U / G).
+// The unit ranges of the ranged tiles: worker c of g takes units [c U / g, (c + 1) U / g).
 __device__ __forceinline__ long long range_begin(long long units, int c, int g) { return units * c / g; }
-// The CTA whose range holds unit u (the largest c with range_begin(c) <= u).
-__device__ __forceinline__ int cta_of(long long units, long long u, int g) { return (int)(((u + 1) * g - 1) / units); }
+// The worker whose range holds unit u (the largest c with range_begin(c) <= u; g <= units).
+__device__ __forceinline__ int worker_of(long long units, long long u, int g) {
+    return (int)(((u + 1) * g - 1) / units);
+}
 
-}  // namespace
+// The pieces (tile, k steps [k0, k1)) of worker c, in the order every role walks them.
+struct Pieces {
+    long long u, u_hi, u_lo;
+    long long tile_next, tiles_whole, base;
+    int nk, g;
+    __device__ Pieces(const LinearArgs &a, int c, int workers) {
+        nk = a.nk, g = workers;
+        tiles_whole = a.tiles_whole;
+        base = a.tiles_whole;
+        const long long units = (a.tiles - a.tiles_whole) * nk;
+        u_lo = u = range_begin(units, c, g);
+        u_hi = range_begin(units, c + 1, g);
+        tile_next = c;
+    }
+    __device__ bool next(long long &tile, int &k0, int &k1) {
+        if (u < u_hi) {
+            tile = base + u / nk;
+            k0 = (int)(u % nk);
+            k1 = u_hi - u < nk - k0 ? k0 + (int)(u_hi - u) : nk;
+            u += k1 - k0;
+            return true;
+        }
+        if (tile_next < tiles_whole) {
+            tile = tile_next;
+            tile_next += g;
+            k0 = 0, k1 = nk;
+            return true;
+        }
+        return false;
+    }
+};
 
-// act(v) in f32 (BRK_ACT_*).
+// The k steps of all pieces, one after the other.
+struct Steps {
+    Pieces p;
+    long long tile = 0;
+    int k = -1, k1 = 0;
+    __device__ Steps(const Pieces &pieces) : p(pieces) {}
+    __device__ bool next() { return ++k < k1 || p.next(tile, k, k1); }
+};
+
+// v * 1 / (1 + e^-z): with the hardware's 2^x and reciprocal, a few 2^-23 of the result.
+__device__ __forceinline__ float times_sigmoid(float v, float z) {
+    return v * rcp_fast(1.f + ex2_fast(-1.4426950408889634f * z));
+}
+
+// act(v) in f32 (BRK_ACT_*); tanh y = 2 sigmoid(2 y) - 1 turns gelu_tanh into a sigmoid too.
 __device__ __forceinline__ float apply_act(float v, int act) {
     switch (act) {
-        case BRK_ACT_SILU: return v / (1.f + expf(-v));
+        case BRK_ACT_SILU: return times_sigmoid(v, v);
         case BRK_ACT_GELU: return 0.5f * v * (1.f + erff(v * 0.70710678118654752f));
-        case BRK_ACT_GELU_TANH: return 0.5f * v * (1.f + tanhf(0.79788456080286536f * (v + 0.044715f * v * v * v)));
-        case BRK_ACT_QUICK_GELU: return v / (1.f + expf(-1.702f * v));
+        case BRK_ACT_GELU_TANH: return times_sigmoid(v, 1.5957691216057308f * fmaf(0.044715f * v * v, v, v));
+        case BRK_ACT_QUICK_GELU: return times_sigmoid(v, 1.702f * v);
         default: return v;
     }
 }
-
-namespace {
 
 // 16 consecutive 32-bit TMEM columns of this thread's lane (no wait).
 __device__ __forceinline__ void tc_ld16_nowait(uint32_t taddr, uint32_t (&r)[16]) {
@@ -78,25 +132,71 @@ __device__ __forceinline__ void tc_ld16_nowait(uint32_t taddr, uint32_t (&r)[16]
         : "r"(taddr));
 }
 
-template <int NT, int MATS>
-__global__ void __launch_bounds__(kLThreads, 1)
+__device__ __forceinline__ void tc_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+
+// The address, in the cluster's shared memory, of `p`'s counterpart in CTA `rank`.
+__device__ __forceinline__ uint32_t cluster_addr(const void *p, uint32_t rank) {
+    uint32_t d;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(d) : "r"(smem_addr(p)), "r"(rank));
+    return d;
+}
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// 2-D tiled TMA load into this CTA's shared memory whose bytes count on a barrier of the CTA pair.
+__device__ __forceinline__ void tma_load_2d_pair(void *dst, const CUtensorMap *map, int x, int y, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
+        "[%4];" ::"r"(smem_addr(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void tc_mma_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                            bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"((uint32_t)accumulate)
+        : "memory");
+}
+// Arrives on `bar` (and its counterpart in the other CTA of the pair) when the MMAs so far are done.
+__device__ __forceinline__ void tc_commit_pair(uint64_t *bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            smem_addr(bar)),
+        "h"((uint16_t)3)
+        : "memory");
+}
+
+template <int NT, int MATS, bool PAIR, bool DRAIN>
+__global__ void __launch_bounds__(LinearLayout<NT, MATS, PAIR>::kThreads, 1)
     linear_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap tw0,
                   const __grid_constant__ CUtensorMap tw1, const __grid_constant__ LinearArgs a) {
-    using L = LinearLayout<NT, MATS>;
-    constexpr int S = L::kStages;
+    using L = LinearLayout<NT, MATS, PAIR>;
+    constexpr int S = L::kStages, CH = L::kChunk, CTAS = L::kCtas, BUFS = L::kBufs;
+    constexpr int EPI = L::kEpiWarps * 32;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint64_t *full = reinterpret_cast<uint64_t *>(smem + L::kBarOff);
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + L::kBarOff);  // PAIR: the even CTA's count
     uint64_t *empty = full + S;
     uint64_t *accfull = empty + S;
-    uint64_t *accfree = accfull + 2;
+    uint64_t *accfree = accfull + 2;                                   // PAIR: the even CTA's count
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(accfree + 2);
     __shared__ int s_last;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int nk = a.nk, g = gridDim.x, c = blockIdx.x;
-    const long long units = (long long)a.tiles * nk;
-    const long long u_lo = range_begin(units, c, g), u_hi = range_begin(units, c + 1, g);
+    const int rank = PAIR ? (int)(blockIdx.x & 1) : 0;
+    const int worker = blockIdx.x / CTAS, workers = gridDim.x / CTAS;
+    const int nt = a.nt;  // tokens per tile: the MMA's N
+    const Pieces pieces(a, worker, workers);
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < S; ++s) {
@@ -105,76 +205,105 @@ __global__ void __launch_bounds__(kLThreads, 1)
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&accfull[i], 1);
-            mbar_init(&accfree[i], 128);
+            mbar_init(&accfree[i], L::kEpiWarps * CTAS);  // a warp's arrival each
         }
         fence_barrier_init();
     }
-    if (warp == kLMma) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)),
-                     "r"(L::kTmemCols)
-                     : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    if (warp == L::kMma) {
+        if constexpr (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)),
+                         "r"(L::kTmemCols)
+                         : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)),
+                         "r"(L::kTmemCols)
+                         : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
     }
     tc_fence_before();
     __syncthreads();
+    if constexpr (PAIR) cluster_sync_all();  // both CTAs' barriers and TMEM are there
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
 
-    if (warp == kLProducer) {
+    if (warp == L::kProducer) {
         if (lane == 0) {
             tma_prefetch_desc(&tx);
             tma_prefetch_desc(&tw0);
             if constexpr (MATS == 2) tma_prefetch_desc(&tw1);
+            const uint32_t x_rows = (uint32_t)nt / CTAS;
+            const uint32_t stage_tx = (MATS * L::kWBox + x_rows * 128) * CTAS;  // both CTAs' bytes
+            auto arm = [&](int s) {
+                if (rank == 0) mbar_arrive_expect_tx(&full[s], stage_tx);
+            };
+            auto load = [&](void *dst, const CUtensorMap *map, int x, int y, int s) {
+                if constexpr (PAIR)
+                    tma_load_2d_pair(dst, map, x, y, cluster_addr(&full[s], 0));
+                else
+                    tma_load_2d(dst, map, x, y, &full[s]);
+            };
+            auto load_w = [&](const Steps &t, int s) {
+                uint8_t *st = smem + s * L::kStageBytes;
+                const int f0 = ((int)(t.tile / a.tiles_m) * CTAS + rank) * kLF;
+                load(st, &tw0, t.k * kLK, f0, s);
+                if constexpr (MATS == 2) load(st + L::kWBox, &tw1, t.k * kLK, f0, s);
+            };
+            auto load_x = [&](const Steps &t, int s) {
+                const int m0 = (int)(t.tile % a.tiles_m) * nt + rank * (int)x_rows;
+                load(smem + s * L::kStageBytes + MATS * L::kWBox, &tx, t.k * kLK, m0, s);
+            };
             // The weights of the first ring do not depend on the kernel before (which, in the same
             // call, writes the activations): they are in flight before the wait for it.
-            const long long n_all = u_hi - u_lo;
-            const int pre = (int)(n_all < S ? n_all : S);
-            auto load_w = [&](long long u, uint8_t *st, uint64_t *bar) {
-                const int tile = (int)(u / nk), kk = (int)(u % nk), f0 = tile / a.tiles_m * kLF;
-                tma_load_2d(st, &tw0, kk * kLK, f0, bar);
-                if constexpr (MATS == 2) tma_load_2d(st + L::kWBox, &tw1, kk * kLK, f0, bar);
-            };
-            auto load_x = [&](long long u, uint8_t *st, uint64_t *bar) {
-                const int tile = (int)(u / nk), kk = (int)(u % nk), m0 = tile % a.tiles_m * NT;
-                tma_load_2d(st + MATS * L::kWBox, &tx, kk * kLK, m0, bar);
-            };
-            for (int j = 0; j < pre; ++j) {
-                mbar_arrive_expect_tx(&full[j], L::kStageBytes);
-                load_w(u_lo + j, smem + j * L::kStageBytes, &full[j]);
+            Steps w(pieces), x(pieces);
+            long long j = 0;
+            bool more = true;
+            while (j < S && (more = w.next())) {
+                arm((int)j);
+                load_w(w, (int)j);
+                ++j;
             }
             griddep_wait();
-            for (int j = 0; j < pre; ++j) load_x(u_lo + j, smem + j * L::kStageBytes, &full[j]);
-            long long issued = pre;
-            for (long long j = pre; j < n_all; ++j) {
+            for (int i = 0; i < (int)j; ++i) {
+                x.next();
+                load_x(x, i);
+            }
+            while (more && w.next()) {
                 const int s = (int)(j % S);
                 if (!mbar_wait(&empty[s], (uint32_t)((j / S) - 1) & 1, a.err, kErrSlotTimeout)) break;
-                uint8_t *st = smem + s * L::kStageBytes;
-                mbar_arrive_expect_tx(&full[s], L::kStageBytes);
-                load_w(u_lo + j, st, &full[s]);
-                load_x(u_lo + j, st, &full[s]);
-                issued = j + 1;
+                arm(s);
+                load_w(w, s);
+                load_x(w, s);
+                ++j;
             }
             // The next kernel of the call may start streaming its weights (what ran before this one is
             // complete: the wait above).
             griddep_launch_dependents();
-            // No copy may still be in flight when the CTA exits.
-            for (long long j = issued > S ? issued - S : 0; j < issued; ++j)
-                mbar_wait(&full[j % S], (uint32_t)(j / S) & 1, a.err, kErrTmaTimeout);
+            // No copy may still be in flight when a CTA exits (the even CTA's barriers count both's).
+            for (long long i = j > S ? j - S : 0; rank == 0 && i < j; ++i)
+                mbar_wait(&full[i % S], (uint32_t)(i / S) & 1, a.err, kErrTmaTimeout);
         }
         __syncwarp();
-    } else if (warp == kLMma) {
-        if (lane == 0) {
-            constexpr uint32_t idesc = f16_idesc(kLF, NT, 0, 0);
-            long long j = 0;   // k steps consumed
-            int seg = 0;       // accumulator sets used
+    } else if (warp == L::kMma) {
+        if (lane == 0 && rank == 0) {
+            const uint32_t idesc = f16_idesc(kLF * CTAS, nt, 0, 0);
+            auto commit = [&](uint64_t *bar) {
+                if constexpr (PAIR)
+                    tc_commit_pair(bar);
+                else
+                    tc_commit(bar);
+            };
+            Pieces p = pieces;
+            long long tile, j = 0;  // k steps consumed
+            int k0, k1, seg = 0;    // accumulator sets used
+            constexpr int seg_steps = DRAIN ? kDrainSteps : 1 << 30;
             bool ok = true;
-            for (long long u = u_lo; ok && u < u_hi;) {
-                const int k0 = (int)(u % nk);
-                const int k1 = (int)(u_hi - u < nk - k0 ? k0 + (u_hi - u) : nk);
-                for (int ks = k0; ok && ks < k1; ks += L::kSegSteps) {
-                    const int ke = k1 - ks < L::kSegSteps ? k1 : ks + L::kSegSteps;
-                    const int buf = seg & 1;
-                    if (seg >= 2 && !mbar_wait(&accfree[buf], ((seg >> 1) - 1) & 1, a.err, kErrMmaTimeout)) {
+            while (ok && p.next(tile, k0, k1)) {
+                for (int ks = k0; ok && ks < k1; ks += seg_steps) {
+                    const int ke = k1 - ks < seg_steps ? k1 : ks + seg_steps;
+                    const int buf = seg % BUFS;
+                    if (seg >= BUFS && !mbar_wait(&accfree[buf], ((seg / BUFS) - 1) & 1, a.err, kErrMmaTimeout)) {
                         ok = false;
                         break;
                     }
@@ -191,154 +320,169 @@ __global__ void __launch_bounds__(kLThreads, 1)
 #pragma unroll
                         for (int e = 0; e < kLK / 16; ++e)
 #pragma unroll
-                            for (int m = 0; m < MATS; ++m)
-                                tc_mma(d + m * NT, sw128_desc(w + m * L::kWBox + e * 32, 16, 1024),
-                                       sw128_desc(x + e * 32, 16, 1024), idesc, kk > ks || e > 0);
-                        tc_commit(&empty[s]);
+                            for (int m = 0; m < MATS; ++m) {
+                                const uint64_t wd = sw128_desc(w + m * L::kWBox + e * 32, 16, 1024);
+                                const uint64_t xd = sw128_desc(x + e * 32, 16, 1024);
+                                if constexpr (PAIR)
+                                    tc_mma_pair(d + m * NT, wd, xd, idesc, kk > ks || e > 0);
+                                else
+                                    tc_mma(d + m * NT, wd, xd, idesc, kk > ks || e > 0);
+                            }
+                        commit(&empty[s]);
                     }
                     if (ok) {
-                        tc_commit(&accfull[buf]);
+                        commit(&accfull[buf]);
                         ++seg;
                     }
                 }
-                u += k1 - k0;
             }
-            // Every MMA this thread issued completes before TMEM is released (the epilogue waits
-            // for every set's commit; after a timeout the last sets are waited for here).
-            for (int b = 0; b < 2; ++b) {
-                const int used = (seg + 1 - b) / 2;  // sets committed on accumulator b
+            // Every MMA issued completes before TMEM is released: the last sets' commits.
+            for (int b = 0; b < BUFS; ++b) {
+                const int used = (seg + BUFS - 1 - b) / BUFS;  // sets committed on accumulator b
                 if (used > 0) mbar_wait(&accfull[b], (used - 1) & 1, a.err, kErrMmaTimeout);
             }
         }
         __syncwarp();
     } else {
-        // ---- epilogue warps: thread r <-> feature f0 + r (TMEM lane r), columns = tokens.
-        const int r = threadIdx.x;
-        const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
+        // ---- epilogue warps: TMEM lane r <-> feature, columns <-> tokens; two warps per lane quarter
+        // (NT >= 64) take half of the columns each.
+        const int r = (warp & 3) * 32 + lane;
+        const int col0 = (warp >> 2) * (L::kHalves == 1 ? 0 : a.half_cols);
+        const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
         griddep_wait();  // the residual may come from, and the output may be read by, what ran before
-        int seg = 0;
-        constexpr int CH = NT < 32 ? 16 : 32;  // columns handled at a time
-        auto ld_cols = [&](uint32_t col, uint32_t (&v)[CH]) {
-            if constexpr (CH == 16)
-                tc_ld16_nowait(tmem + lane_base + col, v);
-            else
-                tc_ld32_nowait(tmem + lane_base + col, v);
+        auto ld_cols = [&](uint32_t col, uint32_t (&v)[CH]) { tc_ld16_nowait(tmem + lane_base + col, v); };
+        auto st_cols = [&](uint32_t col, const uint32_t (&v)[CH]) { tc_st16(tmem + lane_base + col, v); };
+        auto release = [&](int buf) {  // the accumulator may be overwritten
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                if constexpr (PAIR)
+                    mbar_arrive_cluster(cluster_addr(&accfree[buf], 0));
+                else
+                    mbar_arrive(&accfree[buf]);
+            }
         };
+        Pieces p = pieces;
+        long long tile;
+        int k0, k1, seg = 0;
         bool ok = true;
-        for (long long u = u_lo; u < u_hi;) {
-            const int tile = (int)(u / nk), k0 = (int)(u % nk);
-            const int k1 = (int)(u_hi - u < nk - k0 ? k0 + (u_hi - u) : nk);
-            const int feat = tile / a.tiles_m * kLF + r, m0 = tile % a.tiles_m * NT;
-            const int ntok = min(NT, a.M - m0);
-            const bool whole = k0 == 0 && k1 == nk;
-            float *part = nullptr;  // this piece's partial: [MATS][NT][128]
-            if (!whole) part = a.ws + ((size_t)c * 2 + (u == u_lo ? 0 : 1)) * (MATS * NT * kLF) + r;
+        bool first_piece = true;
+        while (p.next(tile, k0, k1)) {
+            const bool at_lo = first_piece;  // a ranged piece that begins at the range's begin
+            first_piece = false;
+            const int feat = ((int)(tile / a.tiles_m) * CTAS + rank) * kLF + r;
+            const int m0 = (int)(tile % a.tiles_m) * nt + col0;     // token of this thread's first column
+            const int ntok = min(min(a.half_cols, nt - col0), a.M - m0);  // columns that count (may be <= 0)
+            const bool whole = k0 == 0 && k1 == a.nk;
+            const size_t slot_floats = (size_t)MATS * nt * kLF;
             const bool in = feat < a.n;
             const float b0 = in && a.bias[0] ? a.bias[0][feat] : 0.f;
             const float b1 = MATS == 2 && in && a.bias[1] ? a.bias[1][feat] : 0.f;
             // The finished values of CH tokens from column c0 on: act(v + b0) (* (w + b1)) (+ residual).
             auto finish = [&](int c0, const float (&v)[CH], const float (&w)[CH]) {
+                if (!in) return;
+                const size_t o0 = (size_t)(m0 + c0) * a.n + feat;
                 float res[CH];
+                if (MATS == 1 && a.residual) {
 #pragma unroll
-                for (int e = 0; e < CH; ++e)
-                    res[e] = MATS == 1 && a.residual && in && c0 + e < ntok
-                                 ? a.residual[(size_t)(m0 + c0 + e) * a.n + feat]
-                                 : 0.f;
+                    for (int e = 0; e < CH; ++e) res[e] = c0 + e < ntok ? a.residual[o0 + (size_t)e * a.n] : 0.f;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < CH; ++e) res[e] = 0.f;
+                }
 #pragma unroll
                 for (int e = 0; e < CH; ++e) {
-                    if (c0 + e < ntok && in) {
+                    if (c0 + e < ntok) {
                         float y = apply_act(v[e] + b0, a.act);
                         if constexpr (MATS == 2)
                             y *= w[e] + b1;
                         else
                             y += res[e];
-                        const size_t o = (size_t)(m0 + c0 + e) * a.n + feat;
                         if (a.out_half)
-                            static_cast<__half *>(a.out)[o] = __float2half_rn(y);
+                            static_cast<__half *>(a.out)[o0 + (size_t)e * a.n] = __float2half_rn(y);
                         else
-                            static_cast<float *>(a.out)[o] = y;
+                            static_cast<float *>(a.out)[o0 + (size_t)e * a.n] = y;
                     }
                 }
             };
-            if constexpr (MATS == 1) {
-                float acc[NT];
+            float *part = a.ws + ((size_t)blockIdx.x * 2 + (at_lo ? 0 : 1)) * slot_floats + (size_t)col0 * kLF + r;
+            if constexpr (DRAIN) {
+                // All accumulator sets of the piece but the last into registers; their sum goes back
+                // into the last one's columns.
+                if (k1 - k0 > kDrainSteps) {
+                    float acc[L::kEpiCols];
 #pragma unroll
-                for (int e = 0; e < NT; ++e) acc[e] = 0.f;
-                for (int ks = k0; ks < k1; ks += L::kSegSteps, ++seg) {
-                    const int buf = seg & 1;
-                    // After one timeout no further set is waited for (the error word is set).
-                    const bool got = ok && mbar_wait(&accfull[buf], (seg >> 1) & 1, a.err, kErrMmaTimeout);
-                    ok = __all_sync(0xffffffffu, got);
-                    tc_fence_after();
+                    for (int e = 0; e < L::kEpiCols; ++e) acc[e] = 0.f;
+                    for (int ks = k0; ks < k1; ks += kDrainSteps) {
+                        const int buf = seg % BUFS;
+                        const bool last = ks + kDrainSteps >= k1;
+                        const bool got = ok && mbar_wait(&accfull[buf], (seg / BUFS) & 1, a.err, kErrMmaTimeout);
+                        ok = __all_sync(0xffffffffu, got);
+                        tc_fence_after();
 #pragma unroll
-                    for (int c0 = 0; c0 < NT; c0 += CH) {
-                        if (c0 < ntok) {
-                            uint32_t v[CH];
-                            ld_cols(buf * L::kCols + c0, v);
-                            tc_wait_ld();
+                        for (int c0 = 0; c0 < L::kEpiCols; c0 += CH) {
+                            if (c0 < ntok) {
+                                uint32_t v[CH];
+                                ld_cols(buf * L::kCols + col0 + c0, v);
+                                tc_wait_ld();
 #pragma unroll
-                            for (int e = 0; e < CH; ++e) acc[c0 + e] += __uint_as_float(v[e]);
-                        }
-                    }
-                    tc_fence_before();
-                    mbar_arrive(&accfree[buf]);
-                }
+                                for (int e = 0; e < CH; ++e) acc[c0 + e] += __uint_as_float(v[e]);
+                                if (last) {
 #pragma unroll
-                for (int c0 = 0; c0 < NT; c0 += CH) {
-                    if (c0 < ntok) {
-                        if (whole) {
-                            float v[CH];
-#pragma unroll
-                            for (int e = 0; e < CH; ++e) v[e] = acc[c0 + e];
-                            finish(c0, v, v);
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < CH; ++e)
-                                if (c0 + e < ntok) __stcg(part + (c0 + e) * kLF, acc[c0 + e]);
-                        }
-                    }
-                }
-            } else {
-                const int buf = seg & 1;
-                const bool got = ok && mbar_wait(&accfull[buf], (seg >> 1) & 1, a.err, kErrMmaTimeout);
-                ok = __all_sync(0xffffffffu, got);
-                ++seg;
-                tc_fence_after();
-#pragma unroll 1
-                for (int c0 = 0; c0 < ntok; c0 += CH) {
-                    uint32_t vr[CH], wr[CH];
-                    ld_cols(buf * L::kCols + c0, vr);
-                    ld_cols(buf * L::kCols + NT + c0, wr);
-                    tc_wait_ld();
-                    float v[CH], w[CH];
-#pragma unroll
-                    for (int e = 0; e < CH; ++e) v[e] = __uint_as_float(vr[e]), w[e] = __uint_as_float(wr[e]);
-                    if (whole) {
-                        finish(c0, v, w);
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < CH; ++e)
-                            if (c0 + e < ntok) {
-                                __stcg(part + (c0 + e) * kLF, v[e]);
-                                __stcg(part + (NT + c0 + e) * kLF, w[e]);
+                                    for (int e = 0; e < CH; ++e) v[e] = __float_as_uint(acc[c0 + e]);
+                                    st_cols(buf * L::kCols + col0 + c0, v);
+                                }
                             }
+                        }
+                        if (!last) {
+                            release(buf);
+                            ++seg;
+                        }
                     }
+                    tc_wait_st();
                 }
-                tc_fence_before();
-                mbar_arrive(&accfree[buf]);
             }
-            if (!whole) {
-                // The last CTA of the tile to finish adds the pieces in k order.
-                __threadfence();
-                named_barrier_sync(2, 128);
-                const long long t0 = (long long)tile * nk;
-                const int c_first = cta_of(units, t0, g), c_last = cta_of(units, t0 + nk - 1, g);
-                if (threadIdx.x == 0) {
-                    const int prev = atomicAdd(&a.counters[tile], 1);
-                    s_last = prev == c_last - c_first;
-                    if (s_last) a.counters[tile] = 0;  // ready for the next launch
+            const int buf = seg % BUFS;
+            // After one timeout no further set is waited for (the error word is set).
+            const bool got = ok && mbar_wait(&accfull[buf], (seg / BUFS) & 1, a.err, kErrMmaTimeout);
+            ok = __all_sync(0xffffffffu, got);
+            ++seg;
+            tc_fence_after();
+#pragma unroll 1
+            for (int c0 = 0; c0 < ntok; c0 += CH) {
+                uint32_t vr[CH], wr[CH];
+                ld_cols(buf * L::kCols + col0 + c0, vr);
+                if constexpr (MATS == 2) ld_cols(buf * L::kCols + NT + col0 + c0, wr);
+                tc_wait_ld();
+                float v[CH], w[CH];
+#pragma unroll
+                for (int e = 0; e < CH; ++e) v[e] = __uint_as_float(vr[e]), w[e] = MATS == 2 ? __uint_as_float(wr[e]) : 0.f;
+                if (whole) {
+                    finish(c0, v, w);
+                } else {
+                    float *dst = part + (size_t)c0 * kLF;
+#pragma unroll
+                    for (int e = 0; e < CH; ++e)
+                        if (c0 + e < ntok) {
+                            __stcg(dst + e * kLF, v[e]);
+                            if constexpr (MATS == 2) __stcg(dst + (size_t)(nt + e) * kLF, w[e]);
+                        }
                 }
-                named_barrier_sync(2, 128);
+            }
+            release(buf);
+            if (!whole) {
+                // The last CTA of the tile (and rank) to finish adds the pieces in k order.
+                __threadfence();
+                named_barrier_sync(2, EPI);
+                const long long units = (a.tiles - a.tiles_whole) * a.nk, t0 = (tile - a.tiles_whole) * a.nk;
+                const int c_first = worker_of(units, t0, workers), c_last = worker_of(units, t0 + a.nk - 1, workers);
+                if (threadIdx.x == 0) {
+                    int *counter = a.counters + (tile - a.tiles_whole) * CTAS + rank;
+                    const int prev = atomicAdd(counter, 1);
+                    s_last = prev == c_last - c_first;
+                    if (s_last) *counter = 0;  // ready for the next launch
+                }
+                named_barrier_sync(2, EPI);
                 if (s_last) {
                     __threadfence();
 #pragma unroll 1
@@ -346,65 +490,102 @@ __global__ void __launch_bounds__(kLThreads, 1)
                         float v[CH], w[CH];
 #pragma unroll
                         for (int e = 0; e < CH; ++e) v[e] = w[e] = 0.f;
-                        for (int p = c_first; p <= c_last; ++p) {
-                            const int slot = range_begin(units, p, g) >= t0 ? 0 : 1;
-                            const float *src = a.ws + ((size_t)p * 2 + slot) * (MATS * NT * kLF) + r;
+                        // Two pieces' loads in flight at a time.
+#pragma unroll 1
+                        for (int q = c_first; q <= c_last; q += 2) {
+                            float x[2][MATS][CH];
 #pragma unroll
-                            for (int e = 0; e < CH; ++e)
-                                if (c0 + e < ntok) {
-                                    v[e] += __ldcg(src + (c0 + e) * kLF);
-                                    if constexpr (MATS == 2) w[e] += __ldcg(src + (NT + c0 + e) * kLF);
+                            for (int h = 0; h < 2; ++h) {
+                                const bool there = q + h <= c_last;
+                                const int slot = range_begin(units, q + h, workers) >= t0 ? 0 : 1;
+                                const float *src = a.ws + ((size_t)((q + h) * CTAS + rank) * 2 + slot) * slot_floats +
+                                                   (size_t)(col0 + c0) * kLF + r;
+#pragma unroll
+                                for (int m = 0; m < MATS; ++m)
+#pragma unroll
+                                    for (int e = 0; e < CH; ++e)
+                                        x[h][m][e] = there && c0 + e < ntok ? __ldcg(src + (size_t)(m * nt + e) * kLF) : 0.f;
+                            }
+#pragma unroll
+                            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                                for (int e = 0; e < CH; ++e) {
+                                    v[e] += x[h][0][e];
+                                    if constexpr (MATS == 2) w[e] += x[h][MATS - 1][e];
                                 }
                         }
                         finish(c0, v, w);
                     }
                 }
-                named_barrier_sync(2, 128);  // s_last is read before the next piece writes it
+                named_barrier_sync(2, EPI);  // s_last is read before the next piece writes it
             }
-            u += k1 - k0;
         }
     }
     tc_fence_before();
     __syncthreads();
+    if constexpr (PAIR) cluster_sync_all();  // no CTA leaves while the other's copies or commits reach it
     tc_fence_after();
-    if (warp == kLMma)
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(L::kTmemCols) : "memory");
+    if (warp == L::kMma) {
+        if constexpr (PAIR)
+            asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(L::kTmemCols) : "memory");
+        else
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(L::kTmemCols) : "memory");
+    }
 }
 
-template <int NT, int MATS>
-cudaError_t launch_linear_t(const CUtensorMap &tx, const CUtensorMap *tw, const LinearArgs &a, int grid, cudaStream_t s,
+template <int NT, int MATS, bool PAIR, bool DRAIN>
+cudaError_t launch_linear_k(const CUtensorMap &tx, const CUtensorMap *tw, const LinearArgs &a, int ctas, cudaStream_t s,
                             bool pdl) {
-    using L = LinearLayout<NT, MATS>;
+    using L = LinearLayout<NT, MATS, PAIR>;
     static unsigned long long configured = 0;  // one bit per device: the opt-in is per device
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev >= 64 || !(configured & (1ull << dev))) {
-        cudaError_t e = cudaFuncSetAttribute(linear_kernel<NT, MATS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        cudaError_t e = cudaFuncSetAttribute(linear_kernel<NT, MATS, PAIR, DRAIN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                              L::kSmemBytes);
         if (e != cudaSuccess) return e;
         if (dev < 64) configured |= 1ull << dev;
     }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(kLThreads);
+    cfg.gridDim = dim3(ctas);
+    cfg.blockDim = dim3(L::kThreads);
     cfg.dynamicSmemBytes = L::kSmemBytes;
     cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchAttribute attr[2];
+    int n = 0;
+    if (pdl) {
+        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[n++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (PAIR) {
+        attr[n].id = cudaLaunchAttributeClusterDimension;
+        attr[n].val.clusterDim.x = 2;
+        attr[n].val.clusterDim.y = 1;
+        attr[n++].val.clusterDim.z = 1;
+    }
     cfg.attrs = attr;
-    cfg.numAttrs = pdl ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, linear_kernel<NT, MATS>, tx, tw[0], tw[MATS - 1], a);
+    cfg.numAttrs = n;
+    return cudaLaunchKernelEx(&cfg, linear_kernel<NT, MATS, PAIR, DRAIN>, tx, tw[0], tw[MATS - 1], a);
+}
+
+// f32 outputs (linear only) drain their accumulators.
+template <int NT, int MATS, bool PAIR>
+cudaError_t launch_linear_t(const CUtensorMap &tx, const CUtensorMap *tw, const LinearArgs &a, int ctas, cudaStream_t s,
+                            bool pdl) {
+    if constexpr (MATS == 1)
+        if (!a.out_half) return launch_linear_k<NT, 1, PAIR, true>(tx, tw, a, ctas, s, pdl);
+    return launch_linear_k<NT, MATS, PAIR, false>(tx, tw, a, ctas, s, pdl);
 }
 
 template <int MATS>
-cudaError_t launch_linear_m(int nt, const CUtensorMap &tx, const CUtensorMap *tw, const LinearArgs &a, int grid,
+cudaError_t launch_linear_m(const LinearPlan &p, const CUtensorMap &tx, const CUtensorMap *tw, const LinearArgs &a,
                             cudaStream_t s, bool pdl) {
-    switch (nt) {
-        case 16: return launch_linear_t<16, MATS>(tx, tw, a, grid, s, pdl);
-        case 32: return launch_linear_t<32, MATS>(tx, tw, a, grid, s, pdl);
-        case 64: return launch_linear_t<64, MATS>(tx, tw, a, grid, s, pdl);
-        case 128: return launch_linear_t<128, MATS>(tx, tw, a, grid, s, pdl);
+    switch (p.nt_kernel) {
+        case 16: return launch_linear_t<16, MATS, false>(tx, tw, a, p.ctas, s, pdl);
+        case 32: return launch_linear_t<32, MATS, false>(tx, tw, a, p.ctas, s, pdl);
+        case 64: return launch_linear_t<64, MATS, false>(tx, tw, a, p.ctas, s, pdl);
+        case 128: return launch_linear_t<128, MATS, true>(tx, tw, a, p.ctas, s, pdl);
+        case 256: return launch_linear_t<256, MATS, true>(tx, tw, a, p.ctas, s, pdl);
         default: return cudaErrorInvalidValue;
     }
 }
@@ -413,20 +594,36 @@ cudaError_t launch_linear_m(int nt, const CUtensorMap &tx, const CUtensorMap *tw
 
 LinearPlan linear_plan(int rows, int k, int n, int mats, int sms) {
     LinearPlan p;
-    p.nt = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
-    p.tiles_m = (rows + p.nt - 1) / p.nt;
-    p.tiles = (long long)((n + kLF - 1) / kLF) * p.tiles_m;
+    const bool pair = rows > 64;
+    // Token tiles: as few as 256 rows each allow, of equal size.
+    p.tiles_m = (rows + 255) / 256;
+    const int per = (rows + p.tiles_m - 1) / p.tiles_m, unit = pair ? 32 : 16;
+    p.nt = (per + unit - 1) / unit * unit;
+    p.nt_kernel = p.nt <= 16 ? 16 : p.nt <= 32 ? 32 : p.nt <= 64 ? 64 : p.nt <= 128 ? 128 : 256;
+    if (!pair) p.nt = p.nt_kernel;
+    const int ctas = pair ? 2 : 1;
+    p.x_rows = p.nt / ctas;
+    p.half_cols = p.nt_kernel >= 64 ? (p.nt / 2 + 15) / 16 * 16 : p.nt;
+    const int feats = kLF * ctas;
+    p.tiles = (long long)((n + feats - 1) / feats) * p.tiles_m;
     p.nk = (k + kLK - 1) / kLK;
-    const long long units = p.tiles * p.nk;
-    p.grid = (int)(units < sms ? units : sms);
-    p.ws_floats = (size_t)p.grid * 2 * mats * p.nt * kLF;
+    // Workers: a CTA (pair) per SM (two), no more than there are units.
+    long long workers = sms / ctas;
+    if (workers < 1) workers = 1;
+    workers = std::min<long long>(workers, p.tiles * p.nk);
+    // Whole waves of tiles, leaving one to two waves' tiles to the ranges (or none when they divide).
+    long long waves = p.tiles / workers;
+    if (p.tiles % workers && waves > 0) --waves;
+    p.tiles_whole = waves * workers;
+    p.ctas = (int)workers * ctas;
+    p.counters = (size_t)(p.tiles - p.tiles_whole) * ctas;
+    p.ws_floats = p.tiles > p.tiles_whole ? (size_t)p.ctas * 2 * mats * p.nt * kLF : 0;
     return p;
 }
 
 cudaError_t launch_linear(int mats, const LinearPlan &p, const CUtensorMap &tx, const CUtensorMap *tw,
                           const LinearArgs &a, cudaStream_t s, bool pdl) {
-    return mats == 2 ? launch_linear_m<2>(p.nt, tx, tw, a, p.grid, s, pdl)
-                     : launch_linear_m<1>(p.nt, tx, tw, a, p.grid, s, pdl);
+    return mats == 2 ? launch_linear_m<2>(p, tx, tw, a, s, pdl) : launch_linear_m<1>(p, tx, tw, a, s, pdl);
 }
 
 }  // namespace brk
