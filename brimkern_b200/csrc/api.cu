@@ -1619,7 +1619,8 @@ int run_linear(brk_ctx *ctx, int mats, int rows, int k, int n, const void *x, co
     a.M = rows, a.n = n;
     a.nk = plan.nk, a.nt = plan.nt, a.tiles_m = plan.tiles_m;
     a.half_cols = plan.half_cols;
-    a.tiles = plan.tiles, a.tiles_whole = plan.tiles_whole;
+    a.tiles_whole = (int)plan.tiles_whole;
+    a.range_units = plan.range_units, a.range_extra = plan.range_extra;
     a.residual = residual;
     a.out = out;
     a.out_half = out_type == BRK_T_F16;
@@ -1651,7 +1652,8 @@ size_t linear_ws(const brk_ctx *ctx, int mats, int rows, int k, int n, size_t *c
 int check_linear(const brk_ctx *ctx, int rows, int k, int n, int act, const char *what) {
     if (!ctx) return fail(BRK_ERR_INVALID, "null context");
     if (rows < 0) return fail(BRK_ERR_INVALID, "%s: rows %d < 0", what, rows);
-    if (k < 8 || k % 8) return fail(BRK_ERR_INVALID, "%s: inner width %d (a multiple of 8)", what, k);
+    if (k < 8 || k % 8 || k > (1 << 24))
+        return fail(BRK_ERR_INVALID, "%s: inner width %d (a multiple of 8, at most 2^24)", what, k);
     if (n < 1) return fail(BRK_ERR_INVALID, "%s: width %d < 1", what, n);
     if (act < BRK_ACT_NONE || act > BRK_ACT_QUICK_GELU) return fail(BRK_ERR_INVALID, "%s: activation %d", what, act);
     if ((long long)((n + 127) / 128) * ((rows + 15) / 16) >= (1ll << 27))

@@ -235,7 +235,8 @@ struct LinearArgs {
     int M, n;                 // tokens, output features
     int nk, nt, tiles_m;      // k steps of 64; tokens per tile; token tiles (tile = feature tile * tiles_m + token tile)
     int half_cols;            // tokens of a tile that an epilogue warp takes (one or two per lane quarter)
-    long long tiles, tiles_whole;  // tiles; the first of them that are done whole, wave by wave
+    int tiles_whole;          // the first tiles, done whole, wave by wave; the others are ranged
+    int range_units, range_extra;  // (tile, k step) units of a worker's range; workers with one more
     const float *bias[2];     // [n] or null
     const float *residual;    // [M][n] f32 or null
     void *out;                // [M][n] f32, or fp16
@@ -251,6 +252,7 @@ struct LinearArgs {
 struct LinearPlan {
     int nt_kernel, nt, x_rows, half_cols, tiles_m, nk, ctas;
     long long tiles, tiles_whole;
+    int range_units, range_extra;
     size_t ws_floats, counters;
 };
 

@@ -48,7 +48,7 @@ struct LinearLayout {
     static constexpr uint32_t kTmemCols = kBufs * kCols < 32 ? 32 : kBufs * kCols;
     static constexpr int kHalves = NT >= 64 ? 2 : 1;              // epilogue warps per TMEM lane quarter
     static constexpr int kEpiWarps = 4 * kHalves;
-    static constexpr int kEpiCols = NT / kHalves;                 // columns of an epilogue thread
+    static constexpr int kEpiCols = NT / kHalves;                 // most columns of an epilogue thread
     static constexpr int kChunk = 16;                             // columns handled at a time
     static constexpr int kProducer = kEpiWarps, kMma = kEpiWarps + 1;
     static constexpr int kThreads = (kEpiWarps + 2) * 32;
@@ -58,52 +58,55 @@ struct LinearLayout {
     static_assert(kSmemBytes <= 232448 - 64, "more than 227 KB of shared memory per CTA");
 };
 
-// The unit ranges of the ranged tiles: worker c of g takes units [c U / g, (c + 1) U / g).
-__device__ __forceinline__ long long range_begin(long long units, int c, int g) { return units * c / g; }
-// The worker whose range holds unit u (the largest c with range_begin(c) <= u; g <= units).
-__device__ __forceinline__ int worker_of(long long units, long long u, int g) {
-    return (int)(((u + 1) * g - 1) / units);
+// The ranged tiles' units are dealt to the workers in contiguous ranges: the first a.range_extra
+// workers have a.range_units + 1, the others a.range_units.
+__device__ __forceinline__ int range_begin(const LinearArgs &a, int c) { return c * a.range_units + min(c, a.range_extra); }
+__device__ __forceinline__ int worker_of(const LinearArgs &a, int u) {
+    const int longer = a.range_extra * (a.range_units + 1);
+    return u < longer ? u / (a.range_units + 1) : a.range_extra + (u - longer) / a.range_units;
 }
 
-// The pieces (tile, k steps [k0, k1)) of worker c, in the order every role walks them.
+// The pieces (tile, k steps [k0, k1)) of worker c, in the order every role walks them, with the
+// tile's feature and token tile.
 struct Pieces {
-    long long u, u_hi, u_lo;
-    long long tile_next, tiles_whole, base;
-    int nk, g;
+    int u, u_hi, whole_next, whole_end, step, nk, tiles_m;
+    int tile, ftile, mtile, k0, k1;
     __device__ Pieces(const LinearArgs &a, int c, int workers) {
-        nk = a.nk, g = workers;
-        tiles_whole = a.tiles_whole;
-        base = a.tiles_whole;
-        const long long units = (a.tiles - a.tiles_whole) * nk;
-        u_lo = u = range_begin(units, c, g);
-        u_hi = range_begin(units, c + 1, g);
-        tile_next = c;
+        u = range_begin(a, c), u_hi = range_begin(a, c + 1);
+        whole_next = c, whole_end = a.tiles_whole, step = workers;
+        nk = a.nk, tiles_m = a.tiles_m;
     }
-    __device__ bool next(long long &tile, int &k0, int &k1) {
+    __device__ bool next() {
         if (u < u_hi) {
-            tile = base + u / nk;
-            k0 = (int)(u % nk);
-            k1 = u_hi - u < nk - k0 ? k0 + (int)(u_hi - u) : nk;
+            const int t = u / nk;
+            tile = whole_end + t;
+            k0 = u - t * nk;
+            k1 = min(nk, k0 + u_hi - u);
             u += k1 - k0;
-            return true;
-        }
-        if (tile_next < tiles_whole) {
-            tile = tile_next;
-            tile_next += g;
+        } else if (whole_next < whole_end) {
+            tile = whole_next;
+            whole_next += step;
             k0 = 0, k1 = nk;
-            return true;
+        } else {
+            return false;
         }
-        return false;
+        ftile = tile / tiles_m;
+        mtile = tile - ftile * tiles_m;
+        return true;
     }
 };
 
 // The k steps of all pieces, one after the other.
 struct Steps {
     Pieces p;
-    long long tile = 0;
-    int k = -1, k1 = 0;
-    __device__ Steps(const Pieces &pieces) : p(pieces) {}
-    __device__ bool next() { return ++k < k1 || p.next(tile, k, k1); }
+    int k = -1;
+    __device__ Steps(const Pieces &pieces) : p(pieces) { p.k1 = 0; }
+    __device__ bool next() {
+        if (++k < p.k1) return true;
+        if (!p.next()) return false;
+        k = p.k0;
+        return true;
+    }
 };
 
 // v * 1 / (1 + e^-z): with the hardware's 2^x and reciprocal, a few 2^-23 of the result.
@@ -111,14 +114,57 @@ __device__ __forceinline__ float times_sigmoid(float v, float z) {
     return v * rcp_fast(1.f + ex2_fast(-1.4426950408889634f * z));
 }
 
-// act(v) in f32 (BRK_ACT_*); tanh y = 2 sigmoid(2 y) - 1 turns gelu_tanh into a sigmoid too.
-__device__ __forceinline__ float apply_act(float v, int act) {
-    switch (act) {
-        case BRK_ACT_SILU: return times_sigmoid(v, v);
-        case BRK_ACT_GELU: return 0.5f * v * (1.f + erff(v * 0.70710678118654752f));
-        case BRK_ACT_GELU_TANH: return times_sigmoid(v, 1.5957691216057308f * fmaf(0.044715f * v * v, v, v));
-        case BRK_ACT_QUICK_GELU: return times_sigmoid(v, 1.702f * v);
-        default: return v;
+// act(v) in f32; tanh y = 2 sigmoid(2 y) - 1 turns gelu_tanh into a sigmoid too.
+template <int ACT>
+__device__ __forceinline__ float apply_act(float v) {
+    if constexpr (ACT == BRK_ACT_SILU) return times_sigmoid(v, v);
+    if constexpr (ACT == BRK_ACT_GELU) return 0.5f * v * (1.f + erff(v * 0.70710678118654752f));
+    if constexpr (ACT == BRK_ACT_GELU_TANH) return times_sigmoid(v, 1.5957691216057308f * fmaf(0.044715f * v * v, v, v));
+    if constexpr (ACT == BRK_ACT_QUICK_GELU) return times_sigmoid(v, 1.702f * v);
+    return v;
+}
+
+// The finished values of one feature for CH tokens, at out[o + e * n] (e < count): act(v + b0)
+// (* (w + b1)), + residual.
+template <int ACT, int MATS, int CH>
+__device__ __forceinline__ void finish_act(const LinearArgs &a, size_t o, int count, float b0, float b1,
+                                           const float (&v)[CH], const float (&w)[CH]) {
+    const size_t n = (size_t)a.n;
+    float y[CH];
+    if (MATS == 1 && a.residual) {
+        const float *res = a.residual + o;
+#pragma unroll
+        for (int e = 0; e < CH; ++e) y[e] = e < count ? res[e * n] : 0.f;
+    } else {
+#pragma unroll
+        for (int e = 0; e < CH; ++e) y[e] = 0.f;
+    }
+#pragma unroll
+    for (int e = 0; e < CH; ++e) {
+        const float x = apply_act<ACT>(v[e] + b0);
+        y[e] = MATS == 2 ? x * (w[e] + b1) : x + y[e];
+    }
+    if (a.out_half) {
+        __half *out = static_cast<__half *>(a.out) + o;
+#pragma unroll
+        for (int e = 0; e < CH; ++e)
+            if (e < count) out[e * n] = __float2half_rn(y[e]);
+    } else {
+        float *out = static_cast<float *>(a.out) + o;
+#pragma unroll
+        for (int e = 0; e < CH; ++e)
+            if (e < count) out[e * n] = y[e];
+    }
+}
+template <int MATS, int CH>
+__device__ __forceinline__ void finish(const LinearArgs &a, size_t o, int count, float b0, float b1, const float (&v)[CH],
+                                       const float (&w)[CH]) {
+    switch (a.act) {
+        case BRK_ACT_SILU: return finish_act<BRK_ACT_SILU, MATS, CH>(a, o, count, b0, b1, v, w);
+        case BRK_ACT_GELU: return finish_act<BRK_ACT_GELU, MATS, CH>(a, o, count, b0, b1, v, w);
+        case BRK_ACT_GELU_TANH: return finish_act<BRK_ACT_GELU_TANH, MATS, CH>(a, o, count, b0, b1, v, w);
+        case BRK_ACT_QUICK_GELU: return finish_act<BRK_ACT_QUICK_GELU, MATS, CH>(a, o, count, b0, b1, v, w);
+        default: return finish_act<BRK_ACT_NONE, MATS, CH>(a, o, count, b0, b1, v, w);
     }
 }
 
@@ -246,42 +292,42 @@ __global__ void __launch_bounds__(LinearLayout<NT, MATS, PAIR>::kThreads, 1)
             };
             auto load_w = [&](const Steps &t, int s) {
                 uint8_t *st = smem + s * L::kStageBytes;
-                const int f0 = ((int)(t.tile / a.tiles_m) * CTAS + rank) * kLF;
+                const int f0 = (t.p.ftile * CTAS + rank) * kLF;
                 load(st, &tw0, t.k * kLK, f0, s);
                 if constexpr (MATS == 2) load(st + L::kWBox, &tw1, t.k * kLK, f0, s);
             };
             auto load_x = [&](const Steps &t, int s) {
-                const int m0 = (int)(t.tile % a.tiles_m) * nt + rank * (int)x_rows;
+                const int m0 = t.p.mtile * nt + rank * (int)x_rows;
                 load(smem + s * L::kStageBytes + MATS * L::kWBox, &tx, t.k * kLK, m0, s);
             };
             // The weights of the first ring do not depend on the kernel before (which, in the same
             // call, writes the activations): they are in flight before the wait for it.
             Steps w(pieces), x(pieces);
-            long long j = 0;
+            int j = 0;  // k steps loaded
             bool more = true;
             while (j < S && (more = w.next())) {
-                arm((int)j);
-                load_w(w, (int)j);
+                arm(j);
+                load_w(w, j);
                 ++j;
             }
             griddep_wait();
-            for (int i = 0; i < (int)j; ++i) {
+            for (int i = 0; i < j; ++i) {
                 x.next();
                 load_x(x, i);
             }
-            while (more && w.next()) {
-                const int s = (int)(j % S);
-                if (!mbar_wait(&empty[s], (uint32_t)((j / S) - 1) & 1, a.err, kErrSlotTimeout)) break;
+            uint32_t phase = 0;
+            for (int s = 0; more && w.next(); ++j) {
+                if (!mbar_wait(&empty[s], phase, a.err, kErrSlotTimeout)) break;
                 arm(s);
                 load_w(w, s);
                 load_x(w, s);
-                ++j;
+                if (++s == S) s = 0, phase ^= 1;
             }
             // The next kernel of the call may start streaming its weights (what ran before this one is
             // complete: the wait above).
             griddep_launch_dependents();
             // No copy may still be in flight when a CTA exits (the even CTA's barriers count both's).
-            for (long long i = j > S ? j - S : 0; rank == 0 && i < j; ++i)
+            for (int i = j > S ? j - S : 0; rank == 0 && i < j; ++i)
                 mbar_wait(&full[i % S], (uint32_t)(i / S) & 1, a.err, kErrTmaTimeout);
         }
         __syncwarp();
@@ -295,13 +341,14 @@ __global__ void __launch_bounds__(LinearLayout<NT, MATS, PAIR>::kThreads, 1)
                     tc_commit(bar);
             };
             Pieces p = pieces;
-            long long tile, j = 0;  // k steps consumed
-            int k0, k1, seg = 0;    // accumulator sets used
+            int s = 0;              // ring stage, with its phase
+            uint32_t phase = 0;
+            int seg = 0;            // accumulator sets used
             constexpr int seg_steps = DRAIN ? kDrainSteps : 1 << 30;
             bool ok = true;
-            while (ok && p.next(tile, k0, k1)) {
-                for (int ks = k0; ok && ks < k1; ks += seg_steps) {
-                    const int ke = k1 - ks < seg_steps ? k1 : ks + seg_steps;
+            while (ok && p.next()) {
+                for (int ks = p.k0; ok && ks < p.k1; ks += seg_steps) {
+                    const int ke = p.k1 - ks < seg_steps ? p.k1 : ks + seg_steps;
                     const int buf = seg % BUFS;
                     if (seg >= BUFS && !mbar_wait(&accfree[buf], ((seg / BUFS) - 1) & 1, a.err, kErrMmaTimeout)) {
                         ok = false;
@@ -309,9 +356,8 @@ __global__ void __launch_bounds__(LinearLayout<NT, MATS, PAIR>::kThreads, 1)
                     }
                     tc_fence_after();
                     const uint32_t d = tmem + buf * L::kCols;
-                    for (int kk = ks; kk < ke; ++kk, ++j) {
-                        const int s = (int)(j % S);
-                        if (!mbar_wait(&full[s], (uint32_t)(j / S) & 1, a.err, kErrTmaTimeout)) {
+                    for (int kk = ks; kk < ke; ++kk) {
+                        if (!mbar_wait(&full[s], phase, a.err, kErrTmaTimeout)) {
                             ok = false;
                             break;
                         }
@@ -329,6 +375,7 @@ __global__ void __launch_bounds__(LinearLayout<NT, MATS, PAIR>::kThreads, 1)
                                     tc_mma(d + m * NT, wd, xd, idesc, kk > ks || e > 0);
                             }
                         commit(&empty[s]);
+                        if (++s == S) s = 0, phase ^= 1;
                     }
                     if (ok) {
                         commit(&accfull[buf]);
@@ -363,48 +410,22 @@ __global__ void __launch_bounds__(LinearLayout<NT, MATS, PAIR>::kThreads, 1)
             }
         };
         Pieces p = pieces;
-        long long tile;
-        int k0, k1, seg = 0;
+        int seg = 0;
         bool ok = true;
         bool first_piece = true;
-        while (p.next(tile, k0, k1)) {
+        while (p.next()) {
+            const int k0 = p.k0, k1 = p.k1;
             const bool at_lo = first_piece;  // a ranged piece that begins at the range's begin
             first_piece = false;
-            const int feat = ((int)(tile / a.tiles_m) * CTAS + rank) * kLF + r;
-            const int m0 = (int)(tile % a.tiles_m) * nt + col0;     // token of this thread's first column
+            const int feat = (p.ftile * CTAS + rank) * kLF + r;
+            const int m0 = p.mtile * nt + col0;                   // token of this thread's first column
             const int ntok = min(min(a.half_cols, nt - col0), a.M - m0);  // columns that count (may be <= 0)
             const bool whole = k0 == 0 && k1 == a.nk;
             const size_t slot_floats = (size_t)MATS * nt * kLF;
             const bool in = feat < a.n;
             const float b0 = in && a.bias[0] ? a.bias[0][feat] : 0.f;
             const float b1 = MATS == 2 && in && a.bias[1] ? a.bias[1][feat] : 0.f;
-            // The finished values of CH tokens from column c0 on: act(v + b0) (* (w + b1)) (+ residual).
-            auto finish = [&](int c0, const float (&v)[CH], const float (&w)[CH]) {
-                if (!in) return;
-                const size_t o0 = (size_t)(m0 + c0) * a.n + feat;
-                float res[CH];
-                if (MATS == 1 && a.residual) {
-#pragma unroll
-                    for (int e = 0; e < CH; ++e) res[e] = c0 + e < ntok ? a.residual[o0 + (size_t)e * a.n] : 0.f;
-                } else {
-#pragma unroll
-                    for (int e = 0; e < CH; ++e) res[e] = 0.f;
-                }
-#pragma unroll
-                for (int e = 0; e < CH; ++e) {
-                    if (c0 + e < ntok) {
-                        float y = apply_act(v[e] + b0, a.act);
-                        if constexpr (MATS == 2)
-                            y *= w[e] + b1;
-                        else
-                            y += res[e];
-                        if (a.out_half)
-                            static_cast<__half *>(a.out)[o0 + (size_t)e * a.n] = __float2half_rn(y);
-                        else
-                            static_cast<float *>(a.out)[o0 + (size_t)e * a.n] = y;
-                    }
-                }
-            };
+            const size_t o0 = (size_t)m0 * a.n + feat;
             float *part = a.ws + ((size_t)blockIdx.x * 2 + (at_lo ? 0 : 1)) * slot_floats + (size_t)col0 * kLF + r;
             if constexpr (DRAIN) {
                 // All accumulator sets of the piece but the last into registers; their sum goes back
@@ -458,7 +479,7 @@ __global__ void __launch_bounds__(LinearLayout<NT, MATS, PAIR>::kThreads, 1)
 #pragma unroll
                 for (int e = 0; e < CH; ++e) v[e] = __uint_as_float(vr[e]), w[e] = MATS == 2 ? __uint_as_float(wr[e]) : 0.f;
                 if (whole) {
-                    finish(c0, v, w);
+                    if (in) finish<MATS, CH>(a, o0 + (size_t)c0 * a.n, ntok - c0, b0, b1, v, w);
                 } else {
                     float *dst = part + (size_t)c0 * kLF;
 #pragma unroll
@@ -474,10 +495,10 @@ __global__ void __launch_bounds__(LinearLayout<NT, MATS, PAIR>::kThreads, 1)
                 // The last CTA of the tile (and rank) to finish adds the pieces in k order.
                 __threadfence();
                 named_barrier_sync(2, EPI);
-                const long long units = (a.tiles - a.tiles_whole) * a.nk, t0 = (tile - a.tiles_whole) * a.nk;
-                const int c_first = worker_of(units, t0, workers), c_last = worker_of(units, t0 + a.nk - 1, workers);
+                const int t0 = (p.tile - a.tiles_whole) * a.nk;
+                const int c_first = worker_of(a, t0), c_last = worker_of(a, t0 + a.nk - 1);
                 if (threadIdx.x == 0) {
-                    int *counter = a.counters + (tile - a.tiles_whole) * CTAS + rank;
+                    int *counter = a.counters + (p.tile - a.tiles_whole) * CTAS + rank;
                     const int prev = atomicAdd(counter, 1);
                     s_last = prev == c_last - c_first;
                     if (s_last) *counter = 0;  // ready for the next launch
@@ -497,7 +518,7 @@ __global__ void __launch_bounds__(LinearLayout<NT, MATS, PAIR>::kThreads, 1)
 #pragma unroll
                             for (int h = 0; h < 2; ++h) {
                                 const bool there = q + h <= c_last;
-                                const int slot = range_begin(units, q + h, workers) >= t0 ? 0 : 1;
+                                const int slot = range_begin(a, q + h) >= t0 ? 0 : 1;
                                 const float *src = a.ws + ((size_t)((q + h) * CTAS + rank) * 2 + slot) * slot_floats +
                                                    (size_t)(col0 + c0) * kLF + r;
 #pragma unroll
@@ -514,7 +535,7 @@ __global__ void __launch_bounds__(LinearLayout<NT, MATS, PAIR>::kThreads, 1)
                                     if constexpr (MATS == 2) w[e] += x[h][MATS - 1][e];
                                 }
                         }
-                        finish(c0, v, w);
+                        if (in) finish<MATS, CH>(a, o0 + (size_t)c0 * a.n, ntok - c0, b0, b1, v, w);
                     }
                 }
                 named_barrier_sync(2, EPI);  // s_last is read before the next piece writes it
@@ -616,6 +637,8 @@ LinearPlan linear_plan(int rows, int k, int n, int mats, int sms) {
     if (p.tiles % workers && waves > 0) --waves;
     p.tiles_whole = waves * workers;
     p.ctas = (int)workers * ctas;
+    const long long units = (p.tiles - p.tiles_whole) * p.nk;
+    p.range_units = (int)(units / workers), p.range_extra = (int)(units % workers);
     p.counters = (size_t)(p.tiles - p.tiles_whole) * ctas;
     p.ws_floats = p.tiles > p.tiles_whole ? (size_t)p.ctas * 2 * mats * p.nt * kLF : 0;
     return p;
