@@ -1609,44 +1609,56 @@ int run_decode_prefix(brk_ctx *ctx, const brk_kv *prefix, int prefix_seq, int pr
     return BRK_OK;
 }
 
+// fp16 rows [rows][k] for the linear kernel, boxes of box_rows rows and kb steps of 64 along k:
+// as [k / 64][row][64], or (flat: k not a multiple of 64, or for its own sake) as [1][row][k].
+int make_linear_map(CUtensorMap *m, const void *base, int rows, int k, int box_rows, int kb, bool flat) {
+    auto enc = tensor_map_encoder();
+    if (!enc) return fail(BRK_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+    cuuint64_t dims[3] = {flat ? (cuuint64_t)k : 64u, (cuuint64_t)rows, flat ? 1u : (cuuint64_t)(k / 64)};
+    cuuint64_t strides[2] = {(cuuint64_t)k * 2, flat ? (cuuint64_t)rows * k * 2 : 128u};
+    cuuint32_t box[3] = {64u, (cuuint32_t)box_rows, (cuuint32_t)kb};
+    cuuint32_t estr[3] = {1u, 1u, 1u};
+    CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void *>(base), dims, strides, box, estr,
+                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(BRK_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+    return BRK_OK;
+}
+
 // One linear product (mats 1) or gate-up product (mats 2); arguments checked, device current.
-int run_linear(brk_ctx *ctx, int mats, int rows, int k, int n, const void *x, const uint16_t *const *w,
-               const float *const *bias, int act, const float *residual, void *out, int out_type, brk_scratch *sc,
-               size_t ws_off, cudaStream_t st, bool pdl) {
-    const brk::LinearPlan plan = brk::linear_plan(rows, k, n, mats, ctx->num_sms);
+// early_w: a launch of the same call came before.
+int run_linear(brk_ctx *ctx, const brk::LinearPlan &plan, int mats, int rows, int k, int n, const void *x,
+               const uint16_t *const *w, const float *const *bias, int act, const float *residual, void *out,
+               int out_type, brk_scratch *sc, cudaStream_t st, bool early_w) {
     brk::LinearArgs a;
     memset(&a, 0, sizeof(a));
     a.M = rows, a.n = n;
     a.nk = plan.nk, a.nt = plan.nt, a.tiles_m = plan.tiles_m;
+    a.f_rows = plan.f_rows;
+    a.kb = plan.kb, a.stages = plan.stages, a.flat = plan.flat;
+    a.drain_steps = plan.drain_steps;
     a.half_cols = plan.half_cols;
     a.tiles_whole = (int)plan.tiles_whole;
     a.range_units = plan.range_units, a.range_extra = plan.range_extra;
+    a.early_w = early_w;
     a.residual = residual;
     a.out = out;
     a.out_half = out_type == BRK_T_F16;
     a.act = act;
-    a.ws = reinterpret_cast<float *>(static_cast<char *>(sc->ws) + ws_off);
+    a.ws = static_cast<float *>(sc->ws);
     a.counters = sc->counters;
     a.err = ctx->d_err;
     CUtensorMap tx, tw[2];
-    int rc = make_map(&tx, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, x, (uint64_t)rows, (uint64_t)k, 64u, (uint32_t)plan.x_rows,
-                      CU_TENSOR_MAP_SWIZZLE_128B);
+    int rc = make_linear_map(&tx, x, rows, k, plan.x_rows, plan.kb, plan.flat);
     for (int i = 0; !rc && i < mats; ++i) {
         a.bias[i] = bias[i];
-        rc = make_weight_map(&tw[i], w[i], n, k, 128);
+        rc = make_linear_map(&tw[i], w[i], n, k, plan.w_rows, plan.kb, plan.flat);
     }
     if (rc) return rc;
-    cudaError_t e = brk::launch_linear(mats, plan, tx, tw, a, st, pdl);
+    cudaError_t e = brk::launch_linear(mats, plan, tx, tw, a, st);
     if (e != cudaSuccess) return cuda_fail(e, "linear kernel launch");
     ++ctx->launches;
     return BRK_OK;
-}
-
-// Workspace bytes and counters of a linear product.
-size_t linear_ws(const brk_ctx *ctx, int mats, int rows, int k, int n, size_t *counters) {
-    const brk::LinearPlan plan = brk::linear_plan(rows, k, n, mats, ctx->num_sms);
-    *counters = std::max(*counters, plan.counters);
-    return align256(plan.ws_floats * sizeof(float));
 }
 
 int check_linear(const brk_ctx *ctx, int rows, int k, int n, int act, const char *what) {
@@ -1718,11 +1730,10 @@ int brk_linear(brk_ctx *ctx, int rows, int k, int n, const uint16_t *x, const ui
         return fail(BRK_ERR_INVALID, "out overlaps an input");
     DeviceGuard g(ctx->device);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    size_t counters = 0;
-    const size_t bytes = linear_ws(ctx, 1, rows, k, n, &counters);
+    const brk::LinearPlan plan = brk::linear_plan(rows, k, n, 1, ctx->num_sms);
     brk_scratch *sc = nullptr;
-    if ((rc = get_scratch(ctx, st, bytes, counters, &sc))) return rc;
-    return run_linear(ctx, 1, rows, k, n, x, &w, &bias, act, residual, out, out_type, sc, 0, st, false);
+    if ((rc = get_scratch(ctx, st, plan.ws_floats * sizeof(float), plan.counters, &sc))) return rc;
+    return run_linear(ctx, plan, 1, rows, k, n, x, &w, &bias, act, residual, out, out_type, sc, st, false);
 }
 
 int brk_ffn_gate_up(brk_ctx *ctx, int rows, int d_model, int d_ff, const uint16_t *x, const uint16_t *w_gate,
@@ -1742,13 +1753,12 @@ int brk_ffn_gate_up(brk_ctx *ctx, int rows, int d_model, int d_ff, const uint16_
         return fail(BRK_ERR_INVALID, "hidden overlaps an input");
     DeviceGuard g(ctx->device);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    size_t counters = 0;
-    const size_t bytes = linear_ws(ctx, 2, rows, d_model, d_ff, &counters);
+    const brk::LinearPlan plan = brk::linear_plan(rows, d_model, d_ff, 2, ctx->num_sms);
     brk_scratch *sc = nullptr;
-    if ((rc = get_scratch(ctx, st, bytes, counters, &sc))) return rc;
+    if ((rc = get_scratch(ctx, st, plan.ws_floats * sizeof(float), plan.counters, &sc))) return rc;
     const uint16_t *w[2] = {w_gate, w_up};
     const float *b[2] = {b_gate, b_up};
-    return run_linear(ctx, 2, rows, d_model, d_ff, x, w, b, act, nullptr, hidden, BRK_T_F16, sc, 0, st, false);
+    return run_linear(ctx, plan, 2, rows, d_model, d_ff, x, w, b, act, nullptr, hidden, BRK_T_F16, sc, st, false);
 }
 
 int brk_ffn(brk_ctx *ctx, int rows, int d_model, int d_ff, const float *h, const float *ffn_norm, double eps,
@@ -1769,9 +1779,10 @@ int brk_ffn(brk_ctx *ctx, int rows, int d_model, int d_ff, const float *h, const
         return fail(BRK_ERR_INVALID, "out overlaps an input");
     DeviceGuard g(ctx->device);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    size_t counters = 0;
-    const size_t ws = std::max(linear_ws(ctx, 2, rows, d_model, d_ff, &counters),
-                               linear_ws(ctx, 1, rows, d_ff, d_model, &counters));
+    const brk::LinearPlan up = brk::linear_plan(rows, d_model, d_ff, 2, ctx->num_sms);
+    const brk::LinearPlan down = brk::linear_plan(rows, d_ff, d_model, 1, ctx->num_sms);
+    const size_t counters = std::max(up.counters, down.counters);
+    const size_t ws = align256(std::max(up.ws_floats, down.ws_floats) * sizeof(float));
     const size_t off_x = ws, off_h = off_x + align256((size_t)rows * d_model * 2);
     brk_scratch *sc = nullptr;
     if ((rc = get_scratch(ctx, st, off_h + align256((size_t)rows * d_ff * 2), counters, &sc))) return rc;
@@ -1784,10 +1795,10 @@ int brk_ffn(brk_ctx *ctx, int rows, int d_model, int d_ff, const float *h, const
     ++ctx->launches;
     const uint16_t *w[2] = {w_gate, w_up};
     const float *b[2] = {nullptr, nullptr};
-    rc = run_linear(ctx, 2, rows, d_model, d_ff, x16, w, b, act, nullptr, hid, BRK_T_F16, sc, 0, st, true);
+    rc = run_linear(ctx, up, 2, rows, d_model, d_ff, x16, w, b, act, nullptr, hid, BRK_T_F16, sc, st, true);
     if (rc) return rc;
-    rc = run_linear(ctx, 1, rows, d_ff, d_model, hid, &w_down, b, BRK_ACT_NONE, post_norm ? nullptr : h, out, BRK_T_F32, sc,
-                    0, st, true);
+    rc = run_linear(ctx, down, 1, rows, d_ff, d_model, hid, &w_down, b, BRK_ACT_NONE, post_norm ? nullptr : h, out,
+                    BRK_T_F32, sc, st, true);
     if (rc || !post_norm) return rc;
     e = brk::launch_post_norm_residual(out, h, post_norm, (float)eps, norm_one_plus ? 1 : 0, rows, d_model, st);
     if (e != cudaSuccess) return cuda_fail(e, "post-norm launch");

@@ -233,24 +233,29 @@ struct ProjArgs {
 // Linear operators (linear.cu): act(x W^T + bias) + residual, or act(x W0^T + b0) * (x W1^T + b1).
 struct LinearArgs {
     int M, n;                 // tokens, output features
-    int nk, nt, tiles_m;      // k steps of 64; tokens per tile; token tiles (tile = feature tile * tiles_m + token tile)
+    int nk, nt, tiles_m;      // stages' worth of k; tokens per tile; token tiles (tile = feature tile * tiles_m + token tile)
+    int f_rows;               // features per CTA and tile
+    int kb, stages, flat;     // k steps of 64 per stage; ring stages; k along the maps' x (else along z)
+    int drain_steps;          // stages' worth of k per accumulator set (f32 outputs)
     int half_cols;            // tokens of a tile that an epilogue warp takes (one or two per lane quarter)
     int tiles_whole;          // the first tiles, done whole, wave by wave; the others are ranged
-    int range_units, range_extra;  // (tile, k step) units of a worker's range; workers with one more
+    int range_units, range_extra;  // (tile, stage of k) units of a worker's range; workers with one more
+    int early_w;              // the kernel before belongs to the same call: weights may load before the wait for it
     const float *bias[2];     // [n] or null
     const float *residual;    // [M][n] f32 or null
     void *out;                // [M][n] f32, or fp16
     int out_half;
     int act;                  // BRK_ACT_*
-    float *ws;                // partial tiles [CTA][2][matrix][token][128]
+    float *ws;                // partial tiles [CTA][2][matrix][token / 4][128][4]
     int *counters;            // [ranged tiles][CTAs per tile] finished pieces, zero between launches
     int *err;
 };
 
-// How a linear product is cut: the kernel's token tile, tokens per tile, rows of a TMA box of x,
-// tiles, k steps, CTAs, workspace floats and counters.
+// How a linear product is cut: the kernel's token tile, tokens per tile, rows of the TMA boxes of x
+// and w, tiles, k, CTAs, workspace floats and counters.
 struct LinearPlan {
-    int nt_kernel, nt, x_rows, half_cols, tiles_m, nk, ctas;
+    bool pair, ranged, flat;
+    int nt_kernel, nt, x_rows, w_rows, f_rows, half_cols, tiles_m, nk, kb, stages, drain_steps, ctas;
     long long tiles, tiles_whole;
     int range_units, range_extra;
     size_t ws_floats, counters;
@@ -326,10 +331,11 @@ cudaError_t launch_post_norm_residual(float *h, const float *x, const float *gai
 cudaError_t launch_proj(int ntok, const CUtensorMap &tx, const CUtensorMap *tw, const CUtensorMap *to,
                         const ProjArgs &a, cudaStream_t s);
 
-// Linear operators (linear.cu); mats 1 or 2.  tx has boxes of plan.x_rows rows, tw of 128 rows.
+// Linear operators (linear.cu); mats 1 or 2.  The maps: boxes of plan.x_rows (w_rows) rows and plan.kb
+// k steps over [k / 64][row][64] (plan.flat: one k step over [row][k]).
 LinearPlan linear_plan(int rows, int k, int n, int mats, int sms);
 cudaError_t launch_linear(int mats, const LinearPlan &p, const CUtensorMap &tx, const CUtensorMap *tw,
-                          const LinearArgs &a, cudaStream_t s, bool pdl);
+                          const LinearArgs &a, cudaStream_t s);
 
 // Shared-prefix attention partials (prefix.cu): maps with prefix_tile_keys()-row boxes over fp16
 // rows (for an int8 cache: its codes as fp16, staged by launch_codes_to_half).  Query rows per CTA

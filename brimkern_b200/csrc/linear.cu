@@ -2,25 +2,30 @@
 // operator y = act(x W^T + b) + r and the gated feed-forward's first half
 // h = act(x Wg^T + bg) * (x Wu^T + bu) (the FFN of recordLayerKV, kernels.ts:1737-1744).
 //
-// linear_kernel<NT, MATS, PAIR, DRAIN> computes D^T = W X^T on tcgen05: weight rows (output features) on the
-// MMA's M, up to NT tokens on its N, so a single token pads 15 MMA columns and not 127 rows, and the
-// token tile follows the row count in steps of 16 (32).  PAIR: two SMs of a cluster work on one tile
-// (cta_group::2, M 256): each holds its 128 features' weights and half of the tokens, so a k step
-// costs an SM half the activation bytes.  With MATS = 2 a CTA holds the gate and the up tile of the
-// same features in two accumulators, and the product leaves through one epilogue.
-//
-// Work is dealt so that every SM has the same amount: first whole waves of tiles (neighbouring CTAs
-// on neighbouring token tiles, so they share weights in L2), the last one to two waves' tiles as
-// (tile, k step) units in equal contiguous ranges.  A range's first and last piece may cover part
-// of a tile's k; such pieces leave f32 partials in the workspace, and the last CTA of a tile to
-// finish adds them in k order (the same order whoever is last: results do not change from run to
-// run).  The ranges come first, so that the joins run under the whole tiles.  Few tokens, bound by
-// streaming the weights once, have nothing but ranges.
+// linear_kernel computes D^T = W X^T on tcgen05: weight rows (output features) on the MMA's M, up to
+// NT tokens on its N, so a single token pads 15 MMA columns and not 127 rows, and the token tile
+// follows the row count in steps of 16 (32).  Three forms:
+//   - one CTA per tile, for few tokens, which are bound by streaming the weights once: the tile's
+//     feature count F (a multiple of 8, at most 128 of the MMA's rows) is chosen so that the tiles
+//     just fill the SMs and none has to be split along k; a stage of the ring holds several k steps
+//     when F is small (one TMA fetches them, [k step][row][64]);
+//   - PAIR: two SMs of a cluster work on one tile (cta_group::2, M 256), each with its 128 features'
+//     weights and half of the tokens, so that a k step costs an SM half the activation bytes: for
+//     many tokens, bound by the tensor cores;
+//   - products whose tiles do not fill whole waves: the last one to two waves' tiles are dealt as
+//     (tile, k step) units in equal contiguous ranges.  A range's first and last piece may cover part
+//     of a tile's k; such pieces leave f32 partials in the workspace, and the last CTA of a tile
+//     to finish adds them in k order (the same order whoever is last: results do not change from run
+//     to run).  The ranges come first, so that the joins run under the whole tiles.
+// Gate-up (MODE): a CTA holds the gate and the up tile of the same F features in two accumulators
+// (kTwoAcc); with PAIR they are interleaved, 64 gate rows and 64 up rows in one accumulator
+// (kInterleaved), which leaves TMEM for a second set: the epilogue of a tile runs under the next
+// tile's products, and its warps swap halves of a chunk through shared memory.
 //
 // The tensor core's f32 accumulation truncates: its error is a bias that grows with k (measured on
 // N(0,1) operands against 64 bits: 3.1e-6 of the result at k 2560, 1.2e-5 at 10240).  For f32
-// outputs (DRAIN) the accumulators are drained every kDrainSteps k steps and the parts added in
-// registers; fp16 outputs (half a step 4.9e-4) do not need it.
+// outputs (DRAIN) the accumulators are drained every 1024 of k and the parts added in registers;
+// fp16 outputs (half a step 4.9e-4) do not need it.
 #include <algorithm>
 
 #include "common.cuh"
@@ -31,29 +36,30 @@ namespace brk {
 
 namespace {
 
-constexpr int kLF = 128;         // output features per CTA and tile (TMEM lanes)
+constexpr int kLF = 128;         // MMA rows (TMEM lanes) per CTA
 constexpr int kLK = 64;          // k per step: one 128-byte swizzled row
-constexpr int kDrainSteps = 16;  // 1024 of k per accumulator
+constexpr int kDrainK = 16;      // k steps per accumulator set when draining
+constexpr uint32_t kRing = 208 * 1024;   // bytes of the load ring
+constexpr uint32_t kSlack = 16 * 1024;   // behind it: the MMA's rows past F, or the gate / up swap
+constexpr int kMaxStages = 16;
 
-template <int NT, int MATS, bool PAIR>
+enum : int { kLinear = 0, kTwoAcc = 1, kInterleaved = 2 };
+
+template <int NT, int MODE, bool PAIR>
 struct LinearLayout {
     static constexpr int kCtas = PAIR ? 2 : 1;
-    static constexpr uint32_t kWBox = kLF * 128;
-    static constexpr uint32_t kXBox = NT / kCtas * 128;
-    static constexpr uint32_t kStageBytes = MATS * kWBox + kXBox;
-    static constexpr int kFit = (204 * 1024) / kStageBytes;
-    static constexpr int kStages = kFit < 12 ? kFit : 12;
-    static constexpr uint32_t kCols = MATS * NT;                  // one accumulator set
+    static constexpr int kMats = MODE == kTwoAcc ? 2 : 1;         // accumulators of a set
+    static constexpr uint32_t kCols = kMats * NT;                 // TMEM columns of a set
     static constexpr int kBufs = 2 * kCols <= 512 ? 2 : 1;
     static constexpr uint32_t kTmemCols = kBufs * kCols < 32 ? 32 : kBufs * kCols;
     static constexpr int kHalves = NT >= 64 ? 2 : 1;              // epilogue warps per TMEM lane quarter
     static constexpr int kEpiWarps = 4 * kHalves;
     static constexpr int kEpiCols = NT / kHalves;                 // most columns of an epilogue thread
-    static constexpr int kChunk = 16;                             // columns handled at a time
+    static constexpr int kChunk = NT >= 64 && MODE == kLinear ? 32 : 16;  // columns handled at a time
     static constexpr int kProducer = kEpiWarps, kMma = kEpiWarps + 1;
     static constexpr int kThreads = (kEpiWarps + 2) * 32;
-    static constexpr uint32_t kBarOff = kStages * kStageBytes;
-    static constexpr uint32_t kSmemBytes = 1024 + kBarOff + (2 * kStages + 4) * 8 + 16;
+    static constexpr uint32_t kBarOff = kRing + kSlack;
+    static constexpr uint32_t kSmemBytes = 1024 + kBarOff + (2 * kMaxStages + 4) * 8 + 16;
     static_assert(kTmemCols <= 512 && (kTmemCols & (kTmemCols - 1)) == 0, "TMEM columns");
     static_assert(kSmemBytes <= 232448 - 64, "more than 227 KB of shared memory per CTA");
 };
@@ -125,24 +131,16 @@ __device__ __forceinline__ float apply_act(float v) {
 }
 
 // The finished values of one feature for CH tokens, at out[o + e * n] (e < count): act(v + b0)
-// (* (w + b1)), + residual.
-template <int ACT, int MATS, int CH>
+// * (w + b1) when GATED, else act(v + b0) + res.
+template <int ACT, bool GATED, int CH>
 __device__ __forceinline__ void finish_act(const LinearArgs &a, size_t o, int count, float b0, float b1,
                                            const float (&v)[CH], const float (&w)[CH]) {
     const size_t n = (size_t)a.n;
     float y[CH];
-    if (MATS == 1 && a.residual) {
-        const float *res = a.residual + o;
-#pragma unroll
-        for (int e = 0; e < CH; ++e) y[e] = e < count ? res[e * n] : 0.f;
-    } else {
-#pragma unroll
-        for (int e = 0; e < CH; ++e) y[e] = 0.f;
-    }
 #pragma unroll
     for (int e = 0; e < CH; ++e) {
         const float x = apply_act<ACT>(v[e] + b0);
-        y[e] = MATS == 2 ? x * (w[e] + b1) : x + y[e];
+        y[e] = GATED ? x * (w[e] + b1) : x + w[e];
     }
     if (a.out_half) {
         __half *out = static_cast<__half *>(a.out) + o;
@@ -156,15 +154,15 @@ __device__ __forceinline__ void finish_act(const LinearArgs &a, size_t o, int co
             if (e < count) out[e * n] = y[e];
     }
 }
-template <int MATS, int CH>
+template <bool GATED, int CH>
 __device__ __forceinline__ void finish(const LinearArgs &a, size_t o, int count, float b0, float b1, const float (&v)[CH],
                                        const float (&w)[CH]) {
     switch (a.act) {
-        case BRK_ACT_SILU: return finish_act<BRK_ACT_SILU, MATS, CH>(a, o, count, b0, b1, v, w);
-        case BRK_ACT_GELU: return finish_act<BRK_ACT_GELU, MATS, CH>(a, o, count, b0, b1, v, w);
-        case BRK_ACT_GELU_TANH: return finish_act<BRK_ACT_GELU_TANH, MATS, CH>(a, o, count, b0, b1, v, w);
-        case BRK_ACT_QUICK_GELU: return finish_act<BRK_ACT_QUICK_GELU, MATS, CH>(a, o, count, b0, b1, v, w);
-        default: return finish_act<BRK_ACT_NONE, MATS, CH>(a, o, count, b0, b1, v, w);
+        case BRK_ACT_SILU: return finish_act<BRK_ACT_SILU, GATED, CH>(a, o, count, b0, b1, v, w);
+        case BRK_ACT_GELU: return finish_act<BRK_ACT_GELU, GATED, CH>(a, o, count, b0, b1, v, w);
+        case BRK_ACT_GELU_TANH: return finish_act<BRK_ACT_GELU_TANH, GATED, CH>(a, o, count, b0, b1, v, w);
+        case BRK_ACT_QUICK_GELU: return finish_act<BRK_ACT_QUICK_GELU, GATED, CH>(a, o, count, b0, b1, v, w);
+        default: return finish_act<BRK_ACT_NONE, GATED, CH>(a, o, count, b0, b1, v, w);
     }
 }
 
@@ -196,13 +194,21 @@ __device__ __forceinline__ uint32_t cluster_addr(const void *p, uint32_t rank) {
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-// 2-D tiled TMA load into this CTA's shared memory whose bytes count on a barrier of the CTA pair.
-__device__ __forceinline__ void tma_load_2d_pair(void *dst, const CUtensorMap *map, int x, int y, uint32_t bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
-        "[%4];" ::"r"(smem_addr(dst)),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
-        : "memory");
+// 3-D tiled TMA load into this CTA's shared memory; PAIR: its bytes count on a barrier of the CTA pair.
+template <bool PAIR>
+__device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *map, int x, int y, int z, uint32_t bar) {
+    if constexpr (PAIR)
+        asm volatile(
+            "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
+            "%3, %4}], [%5];" ::"r"(smem_addr(dst)),
+            "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
+            : "memory");
+    else
+        asm volatile(
+            "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
+            "[%5];" ::"r"(smem_addr(dst)),
+            "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
+            : "memory");
 }
 __device__ __forceinline__ void tc_mma_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
                                             bool accumulate) {
@@ -222,18 +228,19 @@ __device__ __forceinline__ void tc_commit_pair(uint64_t *bar) {
         : "memory");
 }
 
-template <int NT, int MATS, bool PAIR, bool DRAIN>
-__global__ void __launch_bounds__(LinearLayout<NT, MATS, PAIR>::kThreads, 1)
+template <int NT, int MODE, bool PAIR, bool DRAIN>
+__global__ void __launch_bounds__(LinearLayout<NT, MODE, PAIR>::kThreads, 1)
     linear_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap tw0,
                   const __grid_constant__ CUtensorMap tw1, const __grid_constant__ LinearArgs a) {
-    using L = LinearLayout<NT, MATS, PAIR>;
-    constexpr int S = L::kStages, CH = L::kChunk, CTAS = L::kCtas, BUFS = L::kBufs;
+    using L = LinearLayout<NT, MODE, PAIR>;
+    constexpr int CTAS = L::kCtas, BUFS = L::kBufs, MATS = L::kMats, CH = L::kChunk;
     constexpr int EPI = L::kEpiWarps * 32;
+    constexpr bool GATED = MODE != kLinear;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t *full = reinterpret_cast<uint64_t *>(smem + L::kBarOff);  // PAIR: the even CTA's count
-    uint64_t *empty = full + S;
-    uint64_t *accfull = empty + S;
+    uint64_t *empty = full + kMaxStages;
+    uint64_t *accfull = empty + kMaxStages;
     uint64_t *accfree = accfull + 2;                                   // PAIR: the even CTA's count
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(accfree + 2);
     __shared__ int s_last;
@@ -241,8 +248,15 @@ __global__ void __launch_bounds__(LinearLayout<NT, MATS, PAIR>::kThreads, 1)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = PAIR ? (int)(blockIdx.x & 1) : 0;
     const int worker = blockIdx.x / CTAS, workers = gridDim.x / CTAS;
-    const int nt = a.nt;  // tokens per tile: the MMA's N
+    const int nt = a.nt;          // tokens per tile: the MMA's N
+    const int F = a.f_rows;       // features of this CTA's tile (per matrix)
+    const int S = a.stages, KB = PAIR ? 1 : a.kb;
     const Pieces pieces(a, worker, workers);
+    // A stage: W [matrix][k step][F rows][128 B] (interleaved: 64 gate rows, 64 up rows), then
+    // X [k step][token rows][128 B].
+    const uint32_t w_step = MODE == kInterleaved ? kLF * 128 : F * 128;  // bytes of one k step of an A operand
+    const uint32_t x_step = (uint32_t)(nt / CTAS) * 128;
+    const uint32_t x_off = MATS * KB * w_step, stage_bytes = x_off + KB * x_step;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < S; ++s) {
@@ -267,6 +281,10 @@ __global__ void __launch_bounds__(LinearLayout<NT, MATS, PAIR>::kThreads, 1)
                          : "memory");
             asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
         }
+    } else if (warp == L::kProducer && lane == 0) {
+        tma_prefetch_desc(&tx);
+        tma_prefetch_desc(&tw0);
+        if constexpr (GATED) tma_prefetch_desc(&tw1);
     }
     tc_fence_before();
     __syncthreads();
@@ -276,44 +294,51 @@ __global__ void __launch_bounds__(LinearLayout<NT, MATS, PAIR>::kThreads, 1)
 
     if (warp == L::kProducer) {
         if (lane == 0) {
-            tma_prefetch_desc(&tx);
-            tma_prefetch_desc(&tw0);
-            if constexpr (MATS == 2) tma_prefetch_desc(&tw1);
-            const uint32_t x_rows = (uint32_t)nt / CTAS;
-            const uint32_t stage_tx = (MATS * L::kWBox + x_rows * 128) * CTAS;  // both CTAs' bytes
+            const uint32_t stage_tx =
+                (GATED ? 2 : 1) * KB * (MODE == kInterleaved ? kLF / 2 : F) * 128u * CTAS + KB * x_step * CTAS;
             auto arm = [&](int s) {
-                if (rank == 0) mbar_arrive_expect_tx(&full[s], stage_tx);
+                if (rank == 0) mbar_arrive_expect_tx(&full[s], stage_tx);  // both CTAs' bytes
             };
-            auto load = [&](void *dst, const CUtensorMap *map, int x, int y, int s) {
-                if constexpr (PAIR)
-                    tma_load_2d_pair(dst, map, x, y, cluster_addr(&full[s], 0));
-                else
-                    tma_load_2d(dst, map, x, y, &full[s]);
-            };
+            auto bar_of = [&](int s) { return PAIR ? cluster_addr(&full[s], 0) : smem_addr(&full[s]); };
+            // k step t.k covers KB steps of 64; a flat map has k along x, the other along z.
             auto load_w = [&](const Steps &t, int s) {
-                uint8_t *st = smem + s * L::kStageBytes;
-                const int f0 = (t.p.ftile * CTAS + rank) * kLF;
-                load(st, &tw0, t.k * kLK, f0, s);
-                if constexpr (MATS == 2) load(st + L::kWBox, &tw1, t.k * kLK, f0, s);
+                uint8_t *st = smem + s * stage_bytes;
+                const int f0 = (t.p.ftile * CTAS + rank) * F;
+                const int x = a.flat ? t.k * kLK : 0, z = a.flat ? 0 : t.k * KB;
+                tma_load_3d<PAIR>(st, &tw0, x, f0, z, bar_of(s));
+                if constexpr (GATED)
+                    tma_load_3d<PAIR>(st + (MODE == kInterleaved ? kLF / 2 * 128 : KB * w_step), &tw1, x, f0, z, bar_of(s));
             };
             auto load_x = [&](const Steps &t, int s) {
-                const int m0 = t.p.mtile * nt + rank * (int)x_rows;
-                load(smem + s * L::kStageBytes + MATS * L::kWBox, &tx, t.k * kLK, m0, s);
+                const int m0 = t.p.mtile * nt + rank * (nt / CTAS);
+                tma_load_3d<PAIR>(smem + s * stage_bytes + x_off, &tx, a.flat ? t.k * kLK : 0, m0, a.flat ? 0 : t.k * KB,
+                                  bar_of(s));
             };
-            // The weights of the first ring do not depend on the kernel before (which, in the same
-            // call, writes the activations): they are in flight before the wait for it.
-            Steps w(pieces), x(pieces);
-            int j = 0;  // k steps loaded
+            Steps w(pieces);
+            int j = 0;  // stages loaded
             bool more = true;
-            while (j < S && (more = w.next())) {
-                arm(j);
-                load_w(w, j);
-                ++j;
-            }
-            griddep_wait();
-            for (int i = 0; i < j; ++i) {
-                x.next();
-                load_x(x, i);
+            if (a.early_w) {
+                // The weights of the first ring do not depend on the kernel before, which, in the same
+                // call, writes the activations: they are in flight before the wait for it.
+                Steps x(pieces);
+                while (j < S && (more = w.next())) {
+                    arm(j);
+                    load_w(w, j);
+                    ++j;
+                }
+                griddep_wait();
+                for (int i = 0; i < j; ++i) {
+                    x.next();
+                    load_x(x, i);
+                }
+            } else {
+                griddep_wait();
+                while (j < S && (more = w.next())) {
+                    arm(j);
+                    load_w(w, j);
+                    load_x(w, j);
+                    ++j;
+                }
             }
             uint32_t phase = 0;
             for (int s = 0; more && w.next(); ++j) {
@@ -323,8 +348,7 @@ __global__ void __launch_bounds__(LinearLayout<NT, MATS, PAIR>::kThreads, 1)
                 load_x(w, s);
                 if (++s == S) s = 0, phase ^= 1;
             }
-            // The next kernel of the call may start streaming its weights (what ran before this one is
-            // complete: the wait above).
+            // The next kernel may be scheduled (what ran before this one is complete: the wait above).
             griddep_launch_dependents();
             // No copy may still be in flight when a CTA exits (the even CTA's barriers count both's).
             for (int i = j > S ? j - S : 0; rank == 0 && i < j; ++i)
@@ -344,7 +368,7 @@ __global__ void __launch_bounds__(LinearLayout<NT, MATS, PAIR>::kThreads, 1)
             int s = 0;              // ring stage, with its phase
             uint32_t phase = 0;
             int seg = 0;            // accumulator sets used
-            constexpr int seg_steps = DRAIN ? kDrainSteps : 1 << 30;
+            const int seg_steps = DRAIN ? a.drain_steps : 1 << 30;
             bool ok = true;
             while (ok && p.next()) {
                 for (int ks = p.k0; ok && ks < p.k1; ks += seg_steps) {
@@ -362,18 +386,22 @@ __global__ void __launch_bounds__(LinearLayout<NT, MATS, PAIR>::kThreads, 1)
                             break;
                         }
                         tc_fence_after();
-                        const uint32_t w = smem_addr(smem + s * L::kStageBytes), x = w + MATS * L::kWBox;
+                        uint32_t w = smem_addr(smem) + s * stage_bytes, x = w + x_off;
+#pragma unroll 1
+                        for (int b = 0; b < KB; ++b, w += w_step, x += x_step) {
 #pragma unroll
-                        for (int e = 0; e < kLK / 16; ++e)
+                            for (int e = 0; e < kLK / 16; ++e)
 #pragma unroll
-                            for (int m = 0; m < MATS; ++m) {
-                                const uint64_t wd = sw128_desc(w + m * L::kWBox + e * 32, 16, 1024);
-                                const uint64_t xd = sw128_desc(x + e * 32, 16, 1024);
-                                if constexpr (PAIR)
-                                    tc_mma_pair(d + m * NT, wd, xd, idesc, kk > ks || e > 0);
-                                else
-                                    tc_mma(d + m * NT, wd, xd, idesc, kk > ks || e > 0);
-                            }
+                                for (int m = 0; m < MATS; ++m) {
+                                    const uint64_t wd = sw128_desc(w + m * KB * w_step + e * 32, 16, 1024);
+                                    const uint64_t xd = sw128_desc(x + e * 32, 16, 1024);
+                                    const bool acc = kk > ks || b > 0 || e > 0;
+                                    if constexpr (PAIR)
+                                        tc_mma_pair(d + m * NT, wd, xd, idesc, acc);
+                                    else
+                                        tc_mma(d + m * NT, wd, xd, idesc, acc);
+                                }
+                        }
                         commit(&empty[s]);
                         if (++s == S) s = 0, phase ^= 1;
                     }
@@ -391,14 +419,27 @@ __global__ void __launch_bounds__(LinearLayout<NT, MATS, PAIR>::kThreads, 1)
         }
         __syncwarp();
     } else {
-        // ---- epilogue warps: TMEM lane r <-> feature, columns <-> tokens; two warps per lane quarter
-        // (NT >= 64) take half of the columns each.
-        const int r = (warp & 3) * 32 + lane;
+        // ---- epilogue warps: TMEM lane <-> feature, columns <-> tokens; two warps per lane quarter
+        // (NT >= 64) take half of the columns each.  Interleaved: lanes 0-63 gate, 64-127 up.
+        const int quarter = warp & 3;
+        const int lrow = quarter * 32 + lane;
+        const int r = MODE == kInterleaved ? lrow & 63 : lrow;  // feature of the CTA's tile
         const int col0 = (warp >> 2) * (L::kHalves == 1 ? 0 : a.half_cols);
-        const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
+        const bool idle = MODE != kInterleaved && quarter * 32 >= F;  // a warp without features
         griddep_wait();  // the residual may come from, and the output may be read by, what ran before
-        auto ld_cols = [&](uint32_t col, uint32_t (&v)[CH]) { tc_ld16_nowait(tmem + lane_base + col, v); };
-        auto st_cols = [&](uint32_t col, const uint32_t (&v)[CH]) { tc_st16(tmem + lane_base + col, v); };
+        auto ld_cols = [&](uint32_t col, uint32_t (&v)[CH]) {
+            if constexpr (CH == 32)
+                tc_ld32_nowait(tmem + lane_base + col, v);
+            else
+                tc_ld16_nowait(tmem + lane_base + col, v);
+        };
+        auto st_cols = [&](uint32_t col, const uint32_t (&v)[CH]) {
+            if constexpr (CH == 32)
+                tc_st32(tmem + lane_base + col, v);
+            else
+                tc_st16(tmem + lane_base + col, v);
+        };
         auto release = [&](int buf) {  // the accumulator may be overwritten
             tc_fence_before();
             __syncwarp();
@@ -409,6 +450,10 @@ __global__ void __launch_bounds__(LinearLayout<NT, MATS, PAIR>::kThreads, 1)
                     mbar_arrive(&accfree[buf]);
             }
         };
+        // Interleaved: a gate warp and the up warp of the same features swap halves of a chunk, in
+        // two buffers in turn, so that each finishes 8 of its 16 tokens.
+        float *swap = reinterpret_cast<float *>(smem + kRing) + (size_t)((warp >> 2) * 2 + (quarter & 1)) * 2 * 512;
+        int swaps = 0;
         Pieces p = pieces;
         int seg = 0;
         bool ok = true;
@@ -417,26 +462,47 @@ __global__ void __launch_bounds__(LinearLayout<NT, MATS, PAIR>::kThreads, 1)
             const int k0 = p.k0, k1 = p.k1;
             const bool at_lo = first_piece;  // a ranged piece that begins at the range's begin
             first_piece = false;
-            const int feat = (p.ftile * CTAS + rank) * kLF + r;
-            const int m0 = p.mtile * nt + col0;                   // token of this thread's first column
-            const int ntok = min(min(a.half_cols, nt - col0), a.M - m0);  // columns that count (may be <= 0)
+            const int feat = (p.ftile * CTAS + rank) * F + r;
+            const int m0 = p.mtile * nt + col0;                    // token of this thread's first column
+            const int ntok = idle ? 0 : min(min(a.half_cols, nt - col0), a.M - m0);  // columns that count (may be <= 0)
             const bool whole = k0 == 0 && k1 == a.nk;
+            // A partial tile: [matrix][token / 4][128 lanes][4].
             const size_t slot_floats = (size_t)MATS * nt * kLF;
-            const bool in = feat < a.n;
+            const bool in = r < F && feat < a.n;
             const float b0 = in && a.bias[0] ? a.bias[0][feat] : 0.f;
-            const float b1 = MATS == 2 && in && a.bias[1] ? a.bias[1][feat] : 0.f;
+            const float b1 = GATED && in && a.bias[1] ? a.bias[1][feat] : 0.f;
             const size_t o0 = (size_t)m0 * a.n + feat;
-            float *part = a.ws + ((size_t)blockIdx.x * 2 + (at_lo ? 0 : 1)) * slot_floats + (size_t)col0 * kLF + r;
+            auto load_res = [&](int c0, float (&res)[CH]) {
+                const float *src = a.residual + o0 + (size_t)c0 * a.n;
+#pragma unroll
+                for (int e = 0; e < CH; ++e) res[e] = in && c0 + e < ntok ? src[(size_t)e * a.n] : 0.f;
+            };
+            const bool has_res = !GATED && a.residual;
+            float res[CH];
+#pragma unroll
+            for (int e = 0; e < CH; ++e) res[e] = 0.f;
+            if (has_res) {
+                // The residual on its way to L2 while the products run: a thread per 128-byte line of
+                // the CTA's tile.
+                const int f0 = (p.ftile * CTAS + rank) * F, fn = min(F, a.n - f0);
+                const int lines = (fn * 4 + 127) / 128, t0 = p.mtile * nt, tn = min(nt, a.M - t0);
+                for (int i = threadIdx.x; i < lines * tn; i += EPI) {
+                    const float *src = a.residual + (size_t)(t0 + i / lines) * a.n + f0 + i % lines * 32;
+                    asm volatile("prefetch.global.L2 [%0];" ::"l"(src));
+                }
+            }
+            if (!DRAIN && has_res && whole) load_res(0, res);
+            float *part = a.ws + ((size_t)blockIdx.x * 2 + (at_lo ? 0 : 1)) * slot_floats + (size_t)col0 * kLF + lrow * 4;
             if constexpr (DRAIN) {
                 // All accumulator sets of the piece but the last into registers; their sum goes back
                 // into the last one's columns.
-                if (k1 - k0 > kDrainSteps) {
+                if (k1 - k0 > a.drain_steps) {
                     float acc[L::kEpiCols];
 #pragma unroll
                     for (int e = 0; e < L::kEpiCols; ++e) acc[e] = 0.f;
-                    for (int ks = k0; ks < k1; ks += kDrainSteps) {
+                    for (int ks = k0; ks < k1; ks += a.drain_steps) {
                         const int buf = seg % BUFS;
-                        const bool last = ks + kDrainSteps >= k1;
+                        const bool last = ks + a.drain_steps >= k1;
                         const bool got = ok && mbar_wait(&accfull[buf], (seg / BUFS) & 1, a.err, kErrMmaTimeout);
                         ok = __all_sync(0xffffffffu, got);
                         tc_fence_after();
@@ -469,73 +535,120 @@ __global__ void __launch_bounds__(LinearLayout<NT, MATS, PAIR>::kThreads, 1)
             ok = __all_sync(0xffffffffu, got);
             ++seg;
             tc_fence_after();
+            if (DRAIN && has_res && whole) load_res(0, res);
 #pragma unroll 1
             for (int c0 = 0; c0 < ntok; c0 += CH) {
                 uint32_t vr[CH], wr[CH];
                 ld_cols(buf * L::kCols + col0 + c0, vr);
                 if constexpr (MATS == 2) ld_cols(buf * L::kCols + NT + col0 + c0, wr);
                 tc_wait_ld();
-                float v[CH], w[CH];
-#pragma unroll
-                for (int e = 0; e < CH; ++e) v[e] = __uint_as_float(vr[e]), w[e] = MATS == 2 ? __uint_as_float(wr[e]) : 0.f;
                 if (whole) {
-                    if (in) finish<MATS, CH>(a, o0 + (size_t)c0 * a.n, ntok - c0, b0, b1, v, w);
-                } else {
-                    float *dst = part + (size_t)c0 * kLF;
+                    float v[CH], w[CH];
+                    if constexpr (MODE == kInterleaved) {
+                        const bool up = quarter >= 2;
+                        float *buf_g = swap + (swaps & 1) * 512, *buf_u = buf_g + 256;
+                        ++swaps;
+                        // Gate warps give tokens 8-15 and take the up values of 0-7; up warps the reverse.
 #pragma unroll
-                    for (int e = 0; e < CH; ++e)
-                        if (c0 + e < ntok) {
-                            __stcg(dst + e * kLF, v[e]);
-                            if constexpr (MATS == 2) __stcg(dst + (size_t)(nt + e) * kLF, w[e]);
+                        for (int e = 0; e < 8; ++e) {
+                            if (up)
+                                buf_u[e * 32 + lane] = __uint_as_float(vr[e]);
+                            else
+                                buf_g[e * 32 + lane] = __uint_as_float(vr[8 + e]);
                         }
+                        named_barrier_sync(3 + (warp >> 2) * 2 + (quarter & 1), 64);
+                        float g8[8], u8[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            g8[e] = up ? buf_g[e * 32 + lane] : __uint_as_float(vr[e]);
+                            u8[e] = up ? __uint_as_float(vr[8 + e]) : buf_u[e * 32 + lane];
+                        }
+                        const int c8 = c0 + (up ? 8 : 0);
+                        if (in) finish<true, 8>(a, o0 + (size_t)c8 * a.n, ntok - c8, b0, b1, g8, u8);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < CH; ++e) {
+                            v[e] = __uint_as_float(vr[e]);
+                            w[e] = MATS == 2 ? __uint_as_float(wr[e]) : res[e];
+                        }
+                        if (has_res && c0 + CH < ntok) load_res(c0 + CH, res);  // the next chunk's
+                        if (in) finish<GATED, CH>(a, o0 + (size_t)c0 * a.n, ntok - c0, b0, b1, v, w);
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < CH; e += 4) {
+                        if (c0 + e >= ntok) break;
+                        float *dst = part + (size_t)(c0 + e) * kLF;
+                        __stcg(reinterpret_cast<uint4 *>(dst), make_uint4(vr[e], vr[e + 1], vr[e + 2], vr[e + 3]));
+                        if constexpr (MATS == 2)
+                            __stcg(reinterpret_cast<uint4 *>(dst + (size_t)nt * kLF),
+                                   make_uint4(wr[e], wr[e + 1], wr[e + 2], wr[e + 3]));
+                    }
                 }
             }
             release(buf);
             if (!whole) {
                 // The last CTA of the tile (and rank) to finish adds the pieces in k order.
-                __threadfence();
                 named_barrier_sync(2, EPI);
                 const int t0 = (p.tile - a.tiles_whole) * a.nk;
                 const int c_first = worker_of(a, t0), c_last = worker_of(a, t0 + a.nk - 1);
                 if (threadIdx.x == 0) {
                     int *counter = a.counters + (p.tile - a.tiles_whole) * CTAS + rank;
+                    __threadfence();  // the CTA's partial (ordered before by the barrier) before the count
                     const int prev = atomicAdd(counter, 1);
                     s_last = prev == c_last - c_first;
                     if (s_last) *counter = 0;  // ready for the next launch
+                    __threadfence();
                 }
                 named_barrier_sync(2, EPI);
                 if (s_last) {
-                    __threadfence();
+                    // Interleaved: the gate warps join the even chunks, the up warps the odd ones.
+                    constexpr int STEP = MODE == kInterleaved ? 2 * CH : CH;
+                    const int c_begin = MODE == kInterleaved && quarter >= 2 ? CH : 0;
 #pragma unroll 1
-                    for (int c0 = 0; c0 < ntok; c0 += CH) {
+                    for (int c0 = c_begin; c0 < ntok; c0 += STEP) {
                         float v[CH], w[CH];
+                        if (has_res) {
+                            load_res(c0, w);
+                        } else {
 #pragma unroll
-                        for (int e = 0; e < CH; ++e) v[e] = w[e] = 0.f;
+                            for (int e = 0; e < CH; ++e) w[e] = 0.f;
+                        }
+#pragma unroll
+                        for (int e = 0; e < CH; ++e) v[e] = 0.f;
                         // Two pieces' loads in flight at a time.
 #pragma unroll 1
                         for (int q = c_first; q <= c_last; q += 2) {
-                            float x[2][MATS][CH];
+                            float4 x[2][GATED ? 2 : 1][CH / 4];
 #pragma unroll
                             for (int h = 0; h < 2; ++h) {
                                 const bool there = q + h <= c_last;
                                 const int slot = range_begin(a, q + h) >= t0 ? 0 : 1;
                                 const float *src = a.ws + ((size_t)((q + h) * CTAS + rank) * 2 + slot) * slot_floats +
-                                                   (size_t)(col0 + c0) * kLF + r;
+                                                   (size_t)(col0 + c0) * kLF + r * 4;
+                                const size_t other = MODE == kInterleaved ? 64 * 4 : (size_t)nt * kLF;
 #pragma unroll
-                                for (int m = 0; m < MATS; ++m)
-#pragma unroll
-                                    for (int e = 0; e < CH; ++e)
-                                        x[h][m][e] = there && c0 + e < ntok ? __ldcg(src + (size_t)(m * nt + e) * kLF) : 0.f;
+                                for (int e = 0; e < CH / 4; ++e) {
+                                    const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+                                    x[h][0][e] = there && c0 + 4 * e < ntok ? __ldcg(reinterpret_cast<const float4 *>(src + e * 4 * kLF)) : zero;
+                                    if constexpr (GATED)
+                                        x[h][1][e] =
+                                            there && c0 + 4 * e < ntok ? __ldcg(reinterpret_cast<const float4 *>(src + other + e * 4 * kLF)) : zero;
+                                }
                             }
 #pragma unroll
                             for (int h = 0; h < 2; ++h)
 #pragma unroll
-                                for (int e = 0; e < CH; ++e) {
-                                    v[e] += x[h][0][e];
-                                    if constexpr (MATS == 2) w[e] += x[h][MATS - 1][e];
+                                for (int e = 0; e < CH / 4; ++e) {
+                                    v[4 * e] += x[h][0][e].x, v[4 * e + 1] += x[h][0][e].y;
+                                    v[4 * e + 2] += x[h][0][e].z, v[4 * e + 3] += x[h][0][e].w;
+                                    if constexpr (GATED) {
+                                        w[4 * e] += x[h][1][e].x, w[4 * e + 1] += x[h][1][e].y;
+                                        w[4 * e + 2] += x[h][1][e].z, w[4 * e + 3] += x[h][1][e].w;
+                                    }
                                 }
                         }
-                        if (in) finish<MATS, CH>(a, o0 + (size_t)c0 * a.n, ntok - c0, b0, b1, v, w);
+                        if (in) finish<GATED, CH>(a, o0 + (size_t)c0 * a.n, ntok - c0, b0, b1, v, w);
                     }
                 }
                 named_barrier_sync(2, EPI);  // s_last is read before the next piece writes it
@@ -554,16 +667,15 @@ __global__ void __launch_bounds__(LinearLayout<NT, MATS, PAIR>::kThreads, 1)
     }
 }
 
-template <int NT, int MATS, bool PAIR, bool DRAIN>
-cudaError_t launch_linear_k(const CUtensorMap &tx, const CUtensorMap *tw, const LinearArgs &a, int ctas, cudaStream_t s,
-                            bool pdl) {
-    using L = LinearLayout<NT, MATS, PAIR>;
+template <int NT, int MODE, bool PAIR, bool DRAIN>
+cudaError_t launch_linear_k(const CUtensorMap &tx, const CUtensorMap *tw, const LinearArgs &a, int ctas, cudaStream_t s) {
+    using L = LinearLayout<NT, MODE, PAIR>;
     static unsigned long long configured = 0;  // one bit per device: the opt-in is per device
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev >= 64 || !(configured & (1ull << dev))) {
-        cudaError_t e = cudaFuncSetAttribute(linear_kernel<NT, MATS, PAIR, DRAIN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             L::kSmemBytes);
+        cudaError_t e = cudaFuncSetAttribute(linear_kernel<NT, MODE, PAIR, DRAIN>,
+                                             cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmemBytes);
         if (e != cudaSuccess) return e;
         if (dev < 64) configured |= 1ull << dev;
     }
@@ -572,81 +684,136 @@ cudaError_t launch_linear_k(const CUtensorMap &tx, const CUtensorMap *tw, const 
     cfg.blockDim = dim3(L::kThreads);
     cfg.dynamicSmemBytes = L::kSmemBytes;
     cfg.stream = s;
+    // A programmatic dependent of whatever ran before: the CTAs' set-up overlaps its tail, and every
+    // access to memory (but the weights, when an earlier launch of the same call comes before) waits
+    // for it.
     cudaLaunchAttribute attr[2];
-    int n = 0;
-    if (pdl) {
-        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[n++].val.programmaticStreamSerializationAllowed = 1;
-    }
-    if (PAIR) {
-        attr[n].id = cudaLaunchAttributeClusterDimension;
-        attr[n].val.clusterDim.x = 2;
-        attr[n].val.clusterDim.y = 1;
-        attr[n++].val.clusterDim.z = 1;
-    }
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = 2;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = n;
-    return cudaLaunchKernelEx(&cfg, linear_kernel<NT, MATS, PAIR, DRAIN>, tx, tw[0], tw[MATS - 1], a);
+    cfg.numAttrs = PAIR ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, linear_kernel<NT, MODE, PAIR, DRAIN>, tx, tw[0], tw[MODE == kLinear ? 0 : 1], a);
 }
 
 // f32 outputs (linear only) drain their accumulators.
-template <int NT, int MATS, bool PAIR>
-cudaError_t launch_linear_t(const CUtensorMap &tx, const CUtensorMap *tw, const LinearArgs &a, int ctas, cudaStream_t s,
-                            bool pdl) {
-    if constexpr (MATS == 1)
-        if (!a.out_half) return launch_linear_k<NT, 1, PAIR, true>(tx, tw, a, ctas, s, pdl);
-    return launch_linear_k<NT, MATS, PAIR, false>(tx, tw, a, ctas, s, pdl);
+template <int NT, bool PAIR>
+cudaError_t launch_linear_t(int mats, const CUtensorMap &tx, const CUtensorMap *tw, const LinearArgs &a, int ctas,
+                            cudaStream_t s) {
+    if (mats == 2) return launch_linear_k<NT, PAIR ? kInterleaved : kTwoAcc, PAIR, false>(tx, tw, a, ctas, s);
+    return a.out_half ? launch_linear_k<NT, kLinear, PAIR, false>(tx, tw, a, ctas, s)
+                      : launch_linear_k<NT, kLinear, PAIR, true>(tx, tw, a, ctas, s);
 }
 
-template <int MATS>
-cudaError_t launch_linear_m(const LinearPlan &p, const CUtensorMap &tx, const CUtensorMap *tw, const LinearArgs &a,
-                            cudaStream_t s, bool pdl) {
-    switch (p.nt_kernel) {
-        case 16: return launch_linear_t<16, MATS, false>(tx, tw, a, p.ctas, s, pdl);
-        case 32: return launch_linear_t<32, MATS, false>(tx, tw, a, p.ctas, s, pdl);
-        case 64: return launch_linear_t<64, MATS, false>(tx, tw, a, p.ctas, s, pdl);
-        case 128: return launch_linear_t<128, MATS, true>(tx, tw, a, p.ctas, s, pdl);
-        case 256: return launch_linear_t<256, MATS, true>(tx, tw, a, p.ctas, s, pdl);
-        default: return cudaErrorInvalidValue;
-    }
-}
+int round_up(int v, int m) { return (v + m - 1) / m * m; }
 
 }  // namespace
 
+// The cheapest cut by a model in SM cycles.  A k step of a tile costs the larger of its products
+// (nt / 2 cycles for each 16 of k and accumulator) and its bytes through L2 (48 per cycle and SM
+// measured with every SM loading); the whole product at least its weights from HBM (3390 bytes a
+// cycle).  On top: launch, ramp and the last tile's epilogue, and for ranged tiles the partials'
+// way through L2.
 LinearPlan linear_plan(int rows, int k, int n, int mats, int sms) {
-    LinearPlan p;
-    const bool pair = rows > 64;
-    // Token tiles: as few as 256 rows each allow, of equal size.
-    p.tiles_m = (rows + 255) / 256;
-    const int per = (rows + p.tiles_m - 1) / p.tiles_m, unit = pair ? 32 : 16;
-    p.nt = (per + unit - 1) / unit * unit;
-    p.nt_kernel = p.nt <= 16 ? 16 : p.nt <= 32 ? 32 : p.nt <= 64 ? 64 : p.nt <= 128 ? 128 : 256;
-    if (!pair) p.nt = p.nt_kernel;
-    const int ctas = pair ? 2 : 1;
+    const int nkb = (k + kLK - 1) / kLK;
+    const double hbm = 2.0 * mats * n * (double)k / 3390.0;
+    LinearPlan best;
+    double best_cost = 1e300;
+    auto consider = [&](bool pair, int tiles_m, int f, bool ranged) {
+        LinearPlan p;
+        const int unit = pair ? 32 : 16, ctas = pair ? 2 : 1;
+        p.pair = pair;
+        p.tiles_m = tiles_m;
+        p.nt = round_up((rows + tiles_m - 1) / tiles_m, unit);
+        if (p.nt > 256) return;
+        p.nt_kernel = p.nt <= 16 ? 16 : p.nt <= 32 ? 32 : p.nt <= 64 ? 64 : p.nt <= 128 ? 128 : 256;
+        if (pair && p.nt_kernel < 128) p.nt_kernel = 128;
+        p.f_rows = f;
+        const long long ftiles = (n + (long long)f * ctas - 1) / (f * ctas);
+        p.tiles = ftiles * tiles_m;
+        const long long slots = std::max(1, sms / ctas);
+        const int lanes = pair ? kLF : f * mats;  // weight rows of a k step and CTA
+        const double step = std::max((pair ? 1 : mats) * 4.0 * std::max(p.nt / 2, 32), (lanes + p.nt / ctas) * 128 / 48.0);
+        const double epilogue = 800.0 + p.nt * 24.0;
+        double cost;
+        if (ranged) {
+            const double join = 6000.0 + p.nt * 60.0;
+            cost = (double)p.tiles * nkb / slots * step + join + epilogue;
+        } else {
+            cost = (double)((p.tiles + slots - 1) / slots) * nkb * step + epilogue;
+        }
+        cost = std::max(cost, hbm) + (pair ? 5000.0 : 4000.0);
+        if (cost < best_cost) {
+            best_cost = cost;
+            p.ranged = ranged;
+            best = p;
+        }
+    };
+    const int tm0 = (rows + 255) / 256;
+    for (int tm = tm0; tm <= tm0 + 2; ++tm) {
+        if (tm > tm0 && tm > rows) break;
+        // One CTA per tile: the feature count that makes the tiles fill one, two, ... waves.
+        for (int w = 1; w <= 4; ++w) {
+            const long long ft = (long long)sms * w / tm;
+            if (ft < 1) continue;
+            const int f = round_up((int)((n + ft - 1) / ft), 8);
+            if (f <= kLF) {
+                consider(false, tm, f, false);
+                break;
+            }
+        }
+        consider(false, tm, kLF, true);
+        if (rows > 32) {
+            consider(true, tm, mats == 2 ? kLF / 2 : kLF, false);
+            consider(true, tm, mats == 2 ? kLF / 2 : kLF, true);
+        }
+    }
+    LinearPlan &p = best;
+    const int ctas = p.pair ? 2 : 1;
     p.x_rows = p.nt / ctas;
-    p.half_cols = p.nt_kernel >= 64 ? (p.nt / 2 + 15) / 16 * 16 : p.nt;
-    const int feats = kLF * ctas;
-    p.tiles = (long long)((n + feats - 1) / feats) * p.tiles_m;
-    p.nk = (k + kLK - 1) / kLK;
-    // Workers: a CTA (pair) per SM (two), no more than there are units.
-    long long workers = sms / ctas;
-    if (workers < 1) workers = 1;
-    workers = std::min<long long>(workers, p.tiles * p.nk);
-    // Whole waves of tiles, leaving one to two waves' tiles to the ranges (or none when they divide).
-    long long waves = p.tiles / workers;
-    if (p.tiles % workers && waves > 0) --waves;
-    p.tiles_whole = waves * workers;
+    p.half_cols = p.nt_kernel >= 64 ? round_up((p.nt + 1) / 2, 16) : p.nt;
+    p.w_rows = p.f_rows;
+    // k steps per stage: one TMA fetches up to eight (k a multiple of 64), a stage about 32 KB.
+    const bool by_step = k % kLK == 0 && !p.pair;
+    const int step_rows = (p.pair ? kLF : p.f_rows * mats) + p.x_rows;
+    p.kb = 1;
+    while (by_step && p.kb < 8 && 2 * p.kb * step_rows * 128 <= 40 * 1024 && nkb >= 4 * p.kb) p.kb *= 2;
+    p.flat = p.kb == 1;
+    p.stages = std::min<int>(kMaxStages, kRing / (p.kb * step_rows * 128));
+    p.nk = (nkb + p.kb - 1) / p.kb;
+    p.drain_steps = kDrainK / p.kb;
+    // Workers: a CTA (pair) per SM (two), no more than there is work for.
+    long long workers = std::max(1, sms / ctas);
+    workers = std::min<long long>(workers, p.ranged ? p.tiles * p.nk : p.tiles);
+    // Ranged: whole waves of tiles, but for the last one to two waves' (unless they divide).
+    p.tiles_whole = p.tiles;
+    if (p.ranged && p.tiles % workers) {
+        const long long waves = p.tiles / workers;
+        p.tiles_whole = waves > 0 ? (waves - 1) * workers : 0;
+    }
     p.ctas = (int)workers * ctas;
     const long long units = (p.tiles - p.tiles_whole) * p.nk;
     p.range_units = (int)(units / workers), p.range_extra = (int)(units % workers);
     p.counters = (size_t)(p.tiles - p.tiles_whole) * ctas;
-    p.ws_floats = p.tiles > p.tiles_whole ? (size_t)p.ctas * 2 * mats * p.nt * kLF : 0;
+    p.ws_floats = p.tiles > p.tiles_whole ? (size_t)p.ctas * 2 * (p.pair ? 1 : mats) * p.nt * kLF : 0;
     return p;
 }
 
 cudaError_t launch_linear(int mats, const LinearPlan &p, const CUtensorMap &tx, const CUtensorMap *tw,
-                          const LinearArgs &a, cudaStream_t s, bool pdl) {
-    return mats == 2 ? launch_linear_m<2>(p, tx, tw, a, s, pdl) : launch_linear_m<1>(p, tx, tw, a, s, pdl);
+                          const LinearArgs &a, cudaStream_t s) {
+    if (p.pair)
+        return p.nt_kernel == 128 ? launch_linear_t<128, true>(mats, tx, tw, a, p.ctas, s)
+                                  : launch_linear_t<256, true>(mats, tx, tw, a, p.ctas, s);
+    switch (p.nt_kernel) {
+        case 16: return launch_linear_t<16, false>(mats, tx, tw, a, p.ctas, s);
+        case 32: return launch_linear_t<32, false>(mats, tx, tw, a, p.ctas, s);
+        case 64: return launch_linear_t<64, false>(mats, tx, tw, a, p.ctas, s);
+        case 128: return launch_linear_t<128, false>(mats, tx, tw, a, p.ctas, s);
+        default: return launch_linear_t<256, false>(mats, tx, tw, a, p.ctas, s);
+    }
 }
 
 }  // namespace brk
