@@ -1632,7 +1632,24 @@ int run_linear(brk_ctx *ctx, const brk::LinearPlan &plan, int mats, int rows, in
                int out_type, brk_scratch *sc, cudaStream_t st, bool early_w) {
     brk::LinearArgs a;
     memset(&a, 0, sizeof(a));
-    a.M = rows, a.n = n;
+    a.M = rows, a.n = n, a.K = k;
+    a.early_w = early_w;
+    a.residual = residual;
+    a.out = out;
+    a.out_half = out_type == BRK_T_F16;
+    a.act = act;
+    a.err = ctx->d_err;
+    if (rows <= brk::linear_rows_max()) {
+        a.x = static_cast<const __half *>(x);
+        for (int i = 0; i < mats; ++i) {
+            a.w[i] = reinterpret_cast<const __half *>(w[i]);
+            a.bias[i] = bias[i];
+        }
+        cudaError_t e = brk::launch_linear_rows(mats, a, st);
+        if (e != cudaSuccess) return cuda_fail(e, "linear kernel launch");
+        ++ctx->launches;
+        return BRK_OK;
+    }
     a.nk = plan.nk, a.nt = plan.nt, a.tiles_m = plan.tiles_m;
     a.f_rows = plan.f_rows;
     a.kb = plan.kb, a.stages = plan.stages, a.flat = plan.flat;
@@ -1640,14 +1657,8 @@ int run_linear(brk_ctx *ctx, const brk::LinearPlan &plan, int mats, int rows, in
     a.half_cols = plan.half_cols;
     a.tiles_whole = (int)plan.tiles_whole;
     a.range_units = plan.range_units, a.range_extra = plan.range_extra;
-    a.early_w = early_w;
-    a.residual = residual;
-    a.out = out;
-    a.out_half = out_type == BRK_T_F16;
-    a.act = act;
     a.ws = static_cast<float *>(sc->ws);
     a.counters = sc->counters;
-    a.err = ctx->d_err;
     CUtensorMap tx, tw[2];
     int rc = make_linear_map(&tx, x, rows, k, plan.x_rows, plan.kb, plan.flat);
     for (int i = 0; !rc && i < mats; ++i) {

@@ -241,6 +241,8 @@ struct LinearArgs {
     int tiles_whole;          // the first tiles, done whole, wave by wave; the others are ranged
     int range_units, range_extra;  // (tile, stage of k) units of a worker's range; workers with one more
     int early_w;              // the kernel before belongs to the same call: weights may load before the wait for it
+    const __half *x, *w[2];   // rows_kernel: [M][K] activations, [n][K] weights
+    int K;
     const float *bias[2];     // [n] or null
     const float *residual;    // [M][n] f32 or null
     void *out;                // [M][n] f32, or fp16
@@ -336,6 +338,10 @@ cudaError_t launch_proj(int ntok, const CUtensorMap &tx, const CUtensorMap *tw, 
 LinearPlan linear_plan(int rows, int k, int n, int mats, int sms);
 cudaError_t launch_linear(int mats, const LinearPlan &p, const CUtensorMap &tx, const CUtensorMap *tw,
                           const LinearArgs &a, cudaStream_t s);
+// At most linear_rows_max() tokens: without tiles, maps or workspace (M, K, n, x, w, the epilogue's
+// fields and early_w of the arguments).
+int linear_rows_max();
+cudaError_t launch_linear_rows(int mats, const LinearArgs &a, cudaStream_t s);
 
 // Shared-prefix attention partials (prefix.cu): maps with prefix_tile_keys()-row boxes over fp16
 // rows (for an int8 cache: its codes as fp16, staged by launch_codes_to_half).  Query rows per CTA

@@ -699,6 +699,116 @@ cudaError_t launch_linear_k(const CUtensorMap &tx, const CUtensorMap *tw, const 
     return cudaLaunchKernelEx(&cfg, linear_kernel<NT, MODE, PAIR, DRAIN>, tx, tw[0], tw[MODE == kLinear ? 0 : 1], a);
 }
 
+// Up to four tokens (linear_rows_max): no tile at all.  A warp takes WROWS weight rows (two neighbouring features, or
+// the gate and the up row of one), each lane 16 bytes of a 512-byte chunk, with the loads of U chunks
+// in flight; products and sums in f32 pairs, then a tree over the lanes.  The MMA form would read 128
+// rows of shared memory for every 16 of k whatever it needs of them, and its ring, TMEM and barriers
+// cost more than these products.
+template <int R, int WROWS, bool GATED>
+__global__ void __launch_bounds__(128) rows_kernel(const __grid_constant__ LinearArgs a) {
+    constexpr int U = R == 1 ? 8 : 4;
+    const int lane = threadIdx.x & 31;
+    const int unit = blockIdx.x * 4 + (threadIdx.x >> 5);
+    const int f = GATED ? unit : unit * WROWS;
+    if (!a.early_w) griddep_wait();
+    if (f >= a.n) {
+        if (a.early_w) griddep_wait();
+        griddep_launch_dependents();
+        return;
+    }
+    const uint4 *w[WROWS];
+#pragma unroll
+    for (int i = 0; i < WROWS; ++i) {
+        const int row = GATED ? f : min(f + i, a.n - 1);
+        w[i] = reinterpret_cast<const uint4 *>(a.w[GATED ? i : 0] + (size_t)row * a.K) + lane;
+    }
+    const uint4 *x[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+        x[r] = reinterpret_cast<const uint4 *>(a.x + (size_t)min(r, a.M - 1) * a.K) + lane;
+    const int chunks = (a.K + 255) / 256, k8 = a.K / 8 - lane;  // this lane's pieces: chunk * 32 < k8
+    float2 acc[WROWS][R];
+#pragma unroll
+    for (int i = 0; i < WROWS; ++i)
+#pragma unroll
+        for (int r = 0; r < R; ++r) acc[i][r] = make_float2(0.f, 0.f);
+    bool waited = !a.early_w;
+    for (int c = 0; c < chunks; c += U) {
+        uint4 wv[U][WROWS], xv[U][R];
+        const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int i = 0; i < WROWS; ++i) wv[u][i] = (c + u) * 32 < k8 ? __ldcs(w[i] + (c + u) * 32) : zero;
+        if (!waited) {
+            griddep_wait();
+            waited = true;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int r = 0; r < R; ++r) xv[u][r] = (c + u) * 32 < k8 ? x[r][(c + u) * 32] : zero;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            float2 wf[WROWS][4];
+#pragma unroll
+            for (int i = 0; i < WROWS; ++i) {
+                const __half2 *h = reinterpret_cast<const __half2 *>(&wv[u][i]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) wf[i][e] = __half22float2(h[e]);
+            }
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const __half2 *h = reinterpret_cast<const __half2 *>(&xv[u][r]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float2 xf = __half22float2(h[e]);
+#pragma unroll
+                    for (int i = 0; i < WROWS; ++i) acc[i][r] = ffma2(wf[i][e], xf, acc[i][r]);
+                }
+            }
+        }
+    }
+    griddep_launch_dependents();
+    // Lane r + R i ends up with the sum of (row i, token r).
+    float mine = 0.f, other = 0.f;  // GATED: every lane r gets both rows of its token
+#pragma unroll
+    for (int i = 0; i < WROWS; ++i)
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            float v = acc[i][r].x + acc[i][r].y;
+#pragma unroll
+            for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+            if (GATED) {
+                if (lane == r) (i ? other : mine) = v;
+            } else if (lane == r + R * i) {
+                mine = v;
+            }
+        }
+    const int r = GATED ? lane : lane % R, feat = GATED ? f : f + lane / R;
+    if (lane < (GATED ? R : R * WROWS) && r < a.M && feat < a.n) {
+        const size_t o = (size_t)r * a.n + feat;
+        const float v[1] = {mine};
+        const float w1[1] = {GATED ? other : a.residual ? a.residual[o] : 0.f};
+        finish<GATED, 1>(a, o, 1, a.bias[0] ? a.bias[0][feat] : 0.f, GATED && a.bias[1] ? a.bias[1][feat] : 0.f, v, w1);
+    }
+}
+
+template <int R, int WROWS, bool GATED>
+cudaError_t launch_rows_t(const LinearArgs &a, cudaStream_t s) {
+    cudaLaunchConfig_t cfg = {};
+    const int units = GATED ? a.n : (a.n + WROWS - 1) / WROWS;
+    cfg.gridDim = dim3((units + 3) / 4);
+    cfg.blockDim = dim3(128);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, rows_kernel<R, WROWS, GATED>, a);
+}
+
 // f32 outputs (linear only) drain their accumulators.
 template <int NT, bool PAIR>
 cudaError_t launch_linear_t(int mats, const CUtensorMap &tx, const CUtensorMap *tw, const LinearArgs &a, int ctas,
@@ -800,6 +910,16 @@ LinearPlan linear_plan(int rows, int k, int n, int mats, int sms) {
     p.counters = (size_t)(p.tiles - p.tiles_whole) * ctas;
     p.ws_floats = p.tiles > p.tiles_whole ? (size_t)p.ctas * 2 * (p.pair ? 1 : mats) * p.nt * kLF : 0;
     return p;
+}
+
+int linear_rows_max() { return 4; }
+
+cudaError_t launch_linear_rows(int mats, const LinearArgs &a, cudaStream_t s) {
+    if (mats == 2)
+        return a.M == 1 ? launch_rows_t<1, 2, true>(a, s)
+                        : a.M == 2 ? launch_rows_t<2, 2, true>(a, s) : launch_rows_t<4, 2, true>(a, s);
+    return a.M == 1 ? launch_rows_t<1, 1, false>(a, s)
+                    : a.M == 2 ? launch_rows_t<2, 2, false>(a, s) : launch_rows_t<4, 2, false>(a, s);
 }
 
 cudaError_t launch_linear(int mats, const LinearPlan &p, const CUtensorMap &tx, const CUtensorMap *tw,
