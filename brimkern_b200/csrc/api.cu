@@ -1652,6 +1652,7 @@ int run_linear(brk_ctx *ctx, const brk::LinearPlan &plan, int mats, int rows, in
     }
     a.nk = plan.nk, a.nt = plan.nt, a.tiles_m = plan.tiles_m;
     a.f_rows = plan.f_rows;
+    a.cs = plan.cs;
     a.kb = plan.kb, a.stages = plan.stages, a.flat = plan.flat;
     a.drain_steps = plan.drain_steps;
     a.half_cols = plan.half_cols;

@@ -235,6 +235,7 @@ struct LinearArgs {
     int M, n;                 // tokens, output features
     int nk, nt, tiles_m;      // stages' worth of k; tokens per tile; token tiles (tile = feature tile * tiles_m + token tile)
     int f_rows;               // features per CTA and tile
+    int cs;                   // parts that a cluster splits a tile's k into (1: none)
     int kb, stages, flat;     // k steps of 64 per stage; ring stages; k along the maps' x (else along z)
     int drain_steps;          // stages' worth of k per accumulator set (f32 outputs)
     int half_cols;            // tokens of a tile that an epilogue warp takes (one or two per lane quarter)
@@ -257,7 +258,7 @@ struct LinearArgs {
 // and w, tiles, k, CTAs, workspace floats and counters.
 struct LinearPlan {
     bool pair, ranged, flat;
-    int nt_kernel, nt, x_rows, w_rows, f_rows, half_cols, tiles_m, nk, kb, stages, drain_steps, ctas;
+    int cs, nt_kernel, nt, x_rows, w_rows, f_rows, half_cols, tiles_m, nk, kb, stages, drain_steps, ctas;
     long long tiles, tiles_whole;
     int range_units, range_extra;
     size_t ws_floats, counters;

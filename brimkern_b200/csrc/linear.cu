@@ -12,11 +12,14 @@
 //   - PAIR: two SMs of a cluster work on one tile (cta_group::2, M 256), each with its 128 features'
 //     weights and half of the tokens, so that a k step costs an SM half the activation bytes: for
 //     many tokens, bound by the tensor cores;
+//   - few tiles over a long k: a cluster of `cs` CTAs (pairs) splits the k of one tile and joins the
+//     parts through distributed shared memory, each CTA finishing a share of the tokens, so that the
+//     SMs stream without a way through global memory;
 //   - products whose tiles do not fill whole waves: the last one to two waves' tiles are dealt as
 //     (tile, k step) units in equal contiguous ranges.  A range's first and last piece may cover part
 //     of a tile's k; such pieces leave f32 partials in the workspace, and the last CTA of a tile
 //     to finish adds them in k order (the same order whoever is last: results do not change from run
-//     to run).  The ranges come first, so that the joins run under the whole tiles.
+//     to run; so does the cluster's join).  The ranges come first, so that the joins run under the whole tiles.
 // Gate-up (MODE): a CTA holds the gate and the up tile of the same F features in two accumulators
 // (kTwoAcc); with PAIR they are interleaved, 64 gate rows and 64 up rows in one accumulator
 // (kInterleaved), which leaves TMEM for a second set: the epilogue of a tile runs under the next
@@ -75,12 +78,14 @@ __device__ __forceinline__ int worker_of(const LinearArgs &a, int u) {
 // The pieces (tile, k steps [k0, k1)) of worker c, in the order every role walks them, with the
 // tile's feature and token tile.
 struct Pieces {
-    int u, u_hi, whole_next, whole_end, step, nk, tiles_m;
+    int u, u_hi, whole_next, whole_end, step, nk, tiles_m, kw0, kw1;
     int tile, ftile, mtile, k0, k1;
-    __device__ Pieces(const LinearArgs &a, int c, int workers) {
+    // split: the CTA's (pair's) part of a tile's k, of a.cs.
+    __device__ Pieces(const LinearArgs &a, int c, int workers, int split) {
         u = range_begin(a, c), u_hi = range_begin(a, c + 1);
         whole_next = c, whole_end = a.tiles_whole, step = workers;
         nk = a.nk, tiles_m = a.tiles_m;
+        kw0 = nk * split / a.cs, kw1 = nk * (split + 1) / a.cs;
     }
     __device__ bool next() {
         if (u < u_hi) {
@@ -92,7 +97,7 @@ struct Pieces {
         } else if (whole_next < whole_end) {
             tile = whole_next;
             whole_next += step;
-            k0 = 0, k1 = nk;
+            k0 = kw0, k1 = kw1;
         } else {
             return false;
         }
@@ -191,6 +196,14 @@ __device__ __forceinline__ uint32_t cluster_addr(const void *p, uint32_t rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(d) : "r"(smem_addr(p)), "r"(rank));
     return d;
 }
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(addr)
+                 : "memory");
+    return v;
+}
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
@@ -219,12 +232,13 @@ __device__ __forceinline__ void tc_mma_pair(uint32_t d_tmem, uint64_t a_desc, ui
         "l"(a_desc), "l"(b_desc), "r"(idesc), "r"((uint32_t)accumulate)
         : "memory");
 }
-// Arrives on `bar` (and its counterpart in the other CTA of the pair) when the MMAs so far are done.
-__device__ __forceinline__ void tc_commit_pair(uint64_t *bar) {
+// Arrives on `bar` in both CTAs of the pair (their bits of the cluster in `pair_mask`) when the MMAs so
+// far are done.
+__device__ __forceinline__ void tc_commit_pair(uint64_t *bar, uint16_t pair_mask) {
     asm volatile(
         "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
             smem_addr(bar)),
-        "h"((uint16_t)3)
+        "h"(pair_mask)
         : "memory");
 }
 
@@ -246,12 +260,15 @@ __global__ void __launch_bounds__(LinearLayout<NT, MODE, PAIR>::kThreads, 1)
     __shared__ int s_last;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int rank = PAIR ? (int)(blockIdx.x & 1) : 0;
-    const int worker = blockIdx.x / CTAS, workers = gridDim.x / CTAS;
+    const int cs = a.cs;                                        // parts of a tile's k across the cluster
+    const int crank = PAIR || cs > 1 ? (int)blockIdx.x % (CTAS * cs) : 0;
+    const int rank = PAIR ? crank & 1 : 0, split = crank / CTAS;
+    const uint32_t lead = crank - rank;                         // the pair's even CTA in the cluster
+    const int worker = blockIdx.x / (CTAS * cs), workers = gridDim.x / (CTAS * cs);
     const int nt = a.nt;          // tokens per tile: the MMA's N
     const int F = a.f_rows;       // features of this CTA's tile (per matrix)
     const int S = a.stages, KB = PAIR ? 1 : a.kb;
-    const Pieces pieces(a, worker, workers);
+    const Pieces pieces(a, worker, workers, split);
     // A stage: W [matrix][k step][F rows][128 B] (interleaved: 64 gate rows, 64 up rows), then
     // X [k step][token rows][128 B].
     const uint32_t w_step = MODE == kInterleaved ? kLF * 128 : F * 128;  // bytes of one k step of an A operand
@@ -299,7 +316,7 @@ __global__ void __launch_bounds__(LinearLayout<NT, MODE, PAIR>::kThreads, 1)
             auto arm = [&](int s) {
                 if (rank == 0) mbar_arrive_expect_tx(&full[s], stage_tx);  // both CTAs' bytes
             };
-            auto bar_of = [&](int s) { return PAIR ? cluster_addr(&full[s], 0) : smem_addr(&full[s]); };
+            auto bar_of = [&](int s) { return PAIR ? cluster_addr(&full[s], lead) : smem_addr(&full[s]); };
             // k step t.k covers KB steps of 64; a flat map has k along x, the other along z.
             auto load_w = [&](const Steps &t, int s) {
                 uint8_t *st = smem + s * stage_bytes;
@@ -360,7 +377,7 @@ __global__ void __launch_bounds__(LinearLayout<NT, MODE, PAIR>::kThreads, 1)
             const uint32_t idesc = f16_idesc(kLF * CTAS, nt, 0, 0);
             auto commit = [&](uint64_t *bar) {
                 if constexpr (PAIR)
-                    tc_commit_pair(bar);
+                    tc_commit_pair(bar, (uint16_t)(3u << lead));
                 else
                     tc_commit(bar);
             };
@@ -445,7 +462,7 @@ __global__ void __launch_bounds__(LinearLayout<NT, MODE, PAIR>::kThreads, 1)
             __syncwarp();
             if (lane == 0) {
                 if constexpr (PAIR)
-                    mbar_arrive_cluster(cluster_addr(&accfree[buf], 0));
+                    mbar_arrive_cluster(cluster_addr(&accfree[buf], lead));
                 else
                     mbar_arrive(&accfree[buf]);
             }
@@ -465,7 +482,7 @@ __global__ void __launch_bounds__(LinearLayout<NT, MODE, PAIR>::kThreads, 1)
             const int feat = (p.ftile * CTAS + rank) * F + r;
             const int m0 = p.mtile * nt + col0;                    // token of this thread's first column
             const int ntok = idle ? 0 : min(min(a.half_cols, nt - col0), a.M - m0);  // columns that count (may be <= 0)
-            const bool whole = k0 == 0 && k1 == a.nk;
+            const bool whole = cs > 1 || (k0 == 0 && k1 == a.nk);
             // A partial tile: [matrix][token / 4][128 lanes][4].
             const size_t slot_floats = (size_t)MATS * nt * kLF;
             const bool in = r < F && feat < a.n;
@@ -491,7 +508,7 @@ __global__ void __launch_bounds__(LinearLayout<NT, MODE, PAIR>::kThreads, 1)
                     asm volatile("prefetch.global.L2 [%0];" ::"l"(src));
                 }
             }
-            if (!DRAIN && has_res && whole) load_res(0, res);
+            if (!DRAIN && has_res && whole && cs == 1) load_res(0, res);
             float *part = a.ws + ((size_t)blockIdx.x * 2 + (at_lo ? 0 : 1)) * slot_floats + (size_t)col0 * kLF + lrow * 4;
             if constexpr (DRAIN) {
                 // All accumulator sets of the piece but the last into registers; their sum goes back
@@ -535,14 +552,26 @@ __global__ void __launch_bounds__(LinearLayout<NT, MODE, PAIR>::kThreads, 1)
             ok = __all_sync(0xffffffffu, got);
             ++seg;
             tc_fence_after();
-            if (DRAIN && has_res && whole) load_res(0, res);
+            if (DRAIN && has_res && whole && cs == 1) load_res(0, res);
 #pragma unroll 1
             for (int c0 = 0; c0 < ntok; c0 += CH) {
                 uint32_t vr[CH], wr[CH];
                 ld_cols(buf * L::kCols + col0 + c0, vr);
                 if constexpr (MATS == 2) ld_cols(buf * L::kCols + NT + col0 + c0, wr);
                 tc_wait_ld();
-                if (whole) {
+                if (cs > 1) {
+                    // This CTA's part [matrix][token / 4][128 lanes][4], in the ring (its copies and the
+                    // products that read them are complete).
+                    float *dst = reinterpret_cast<float *>(smem) + (size_t)(col0 + c0) * kLF + lrow * 4;
+#pragma unroll
+                    for (int e = 0; e < CH; e += 4) {
+                        if (c0 + e >= ntok) break;
+                        *reinterpret_cast<uint4 *>(dst + e * kLF) = make_uint4(vr[e], vr[e + 1], vr[e + 2], vr[e + 3]);
+                        if constexpr (MATS == 2)
+                            *reinterpret_cast<uint4 *>(dst + (size_t)nt * kLF + e * kLF) =
+                                make_uint4(wr[e], wr[e + 1], wr[e + 2], wr[e + 3]);
+                    }
+                } else if (whole) {
                     float v[CH], w[CH];
                     if constexpr (MODE == kInterleaved) {
                         const bool up = quarter >= 2;
@@ -655,9 +684,54 @@ __global__ void __launch_bounds__(LinearLayout<NT, MODE, PAIR>::kThreads, 1)
             }
         }
     }
+    if (cs > 1) {
+        __syncwarp();
+        cluster_sync_all();  // every part is in its CTA's shared memory
+        if (warp < L::kEpiWarps) {
+            // Groups of four tokens dealt over the cluster's CTAs and their warps; the parts added in k
+            // order.  Interleaved: the gate warps and the up warps take different groups.
+            Pieces p = pieces;
+            p.next();
+            const int quarter = warp & 3, lrow = quarter * 32 + lane;
+            const int r = MODE == kInterleaved ? lrow & 63 : lrow;
+            const int feat = (p.ftile * CTAS + rank) * F + r, m0 = p.mtile * nt, ntok = min(nt, a.M - m0);
+            constexpr int SHARES = L::kHalves * (MODE == kInterleaved ? 2 : 1);
+            const int share = (warp >> 2) * (MODE == kInterleaved ? 2 : 1) + (MODE == kInterleaved ? quarter >> 1 : 0);
+            const bool in = r < F && feat < a.n;
+            const float b0 = in && a.bias[0] ? a.bias[0][feat] : 0.f;
+            const float b1 = GATED && in && a.bias[1] ? a.bias[1][feat] : 0.f;
+            const uint32_t other = MODE == kInterleaved ? 64 * 16 : (uint32_t)nt * kLF * 4;
+#pragma unroll 1
+            for (int g = split * SHARES + share; 4 * g < ntok && in; g += cs * SHARES) {
+                const size_t o = (size_t)(m0 + 4 * g) * a.n + feat;
+                float v[4] = {0.f, 0.f, 0.f, 0.f}, w[4] = {0.f, 0.f, 0.f, 0.f};
+                if (!GATED && a.residual) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) w[e] = 4 * g + e < ntok ? a.residual[o + (size_t)e * a.n] : 0.f;
+                }
+                const float *src = reinterpret_cast<const float *>(smem) + (size_t)g * 4 * kLF + r * 4;
+                float4 x[8][GATED ? 2 : 1];
+#pragma unroll
+                for (int q = 0; q < 8; ++q)
+                    if (q < cs) {
+                        const uint32_t at = cluster_addr(src, q * CTAS + rank);
+                        x[q][0] = ld_cluster_f32x4(at);
+                        if constexpr (GATED) x[q][1] = ld_cluster_f32x4(at + other);
+                    }
+#pragma unroll
+                for (int q = 0; q < 8; ++q)
+                    if (q < cs) {
+                        v[0] += x[q][0].x, v[1] += x[q][0].y, v[2] += x[q][0].z, v[3] += x[q][0].w;
+                        if constexpr (GATED) w[0] += x[q][1].x, w[1] += x[q][1].y, w[2] += x[q][1].z, w[3] += x[q][1].w;
+                    }
+                finish<GATED, 4>(a, o, ntok - 4 * g, b0, b1, v, w);
+            }
+        }
+        __syncwarp();
+    }
     tc_fence_before();
     __syncthreads();
-    if constexpr (PAIR) cluster_sync_all();  // no CTA leaves while the other's copies or commits reach it
+    if (PAIR || cs > 1) cluster_sync_all();  // no CTA leaves while another's copies, commits or reads reach it
     tc_fence_after();
     if (warp == L::kMma) {
         if constexpr (PAIR)
@@ -691,11 +765,11 @@ cudaError_t launch_linear_k(const CUtensorMap &tx, const CUtensorMap *tw, const 
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = 2;
+    attr[1].val.clusterDim.x = L::kCtas * a.cs;
     attr[1].val.clusterDim.y = 1;
     attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = PAIR ? 2 : 1;
+    cfg.numAttrs = L::kCtas * a.cs > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, linear_kernel<NT, MODE, PAIR, DRAIN>, tx, tw[0], tw[MODE == kLinear ? 0 : 1], a);
 }
 
@@ -822,36 +896,74 @@ int round_up(int v, int m) { return (v + m - 1) / m * m; }
 
 }  // namespace
 
+// How many clusters of `size` CTAs of these kernels (one CTA per SM) fit on the device at once.
+static int max_clusters(int size, int sms) {
+    static int cache[64][9] = {};  // per device and size; the GPU's partition into GPCs is fixed
+    if (size <= 1) return sms;
+    int dev = 0;
+    cudaGetDevice(&dev);
+    int n = dev < 64 ? cache[dev][size] : 0;
+    if (n == 0) {
+        using L = LinearLayout<16, kLinear, false>;
+        cudaFuncSetAttribute(linear_kernel<16, kLinear, false, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             L::kSmemBytes);
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(size * 64);
+        cfg.blockDim = dim3(L::kThreads);
+        cfg.dynamicSmemBytes = L::kSmemBytes;
+        cudaLaunchAttribute attr;
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = size;
+        attr.val.clusterDim.y = 1;
+        attr.val.clusterDim.z = 1;
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        if (cudaOccupancyMaxActiveClusters(&n, linear_kernel<16, kLinear, false, false>, &cfg) != cudaSuccess) {
+            cudaGetLastError();
+            n = 0;
+        }
+        if (n <= 0) n = -1;
+        if (dev < 64) cache[dev][size] = n;
+    }
+    return n > 0 ? n : 0;
+}
+
 // The cheapest cut by a model in SM cycles.  A k step of a tile costs the larger of its products
-// (nt / 2 cycles for each 16 of k and accumulator) and its bytes through L2 (48 per cycle and SM
-// measured with every SM loading); the whole product at least its weights from HBM (3390 bytes a
-// cycle).  On top: launch, ramp and the last tile's epilogue, and for ranged tiles the partials'
-// way through L2.
+// (nt / 2 cycles, at least 32 for reading 128 rows, for each 16 of k and accumulator) and its bytes
+// through L2 (48 per cycle and SM with every SM loading); the whole product at least its weights from
+// HBM (3390 bytes a cycle).  On top: launch, ramp and the last tile's epilogue, and what joins split
+// tiles.
 LinearPlan linear_plan(int rows, int k, int n, int mats, int sms) {
     const int nkb = (k + kLK - 1) / kLK;
     const double hbm = 2.0 * mats * n * (double)k / 3390.0;
     LinearPlan best;
     double best_cost = 1e300;
-    auto consider = [&](bool pair, int tiles_m, int f, bool ranged) {
+    auto consider = [&](bool pair, int tiles_m, int f, int cs, bool ranged) {
         LinearPlan p;
         const int unit = pair ? 32 : 16, ctas = pair ? 2 : 1;
         p.pair = pair;
+        p.cs = cs;
         p.tiles_m = tiles_m;
         p.nt = round_up((rows + tiles_m - 1) / tiles_m, unit);
         if (p.nt > 256) return;
         p.nt_kernel = p.nt <= 16 ? 16 : p.nt <= 32 ? 32 : p.nt <= 64 ? 64 : p.nt <= 128 ? 128 : 256;
         if (pair && p.nt_kernel < 128) p.nt_kernel = 128;
         p.f_rows = f;
+        const int accs = pair ? 1 : mats;
+        if (cs > 1 && (uint32_t)(accs * p.nt * kLF * 4) > kRing) return;
         const long long ftiles = (n + (long long)f * ctas - 1) / (f * ctas);
         p.tiles = ftiles * tiles_m;
-        const long long slots = std::max(1, sms / ctas);
+        const long long slots = std::max(1, cs > 1 ? max_clusters(ctas * cs, sms) : sms / ctas);
+        if (cs > 1 && p.tiles > slots) return;
         const int lanes = pair ? kLF : f * mats;  // weight rows of a k step and CTA
-        const double step = std::max((pair ? 1 : mats) * 4.0 * std::max(p.nt / 2, 32), (lanes + p.nt / ctas) * 128 / 48.0);
+        const double step = std::max(accs * 4.0 * std::max(p.nt / 2, 32), (lanes + p.nt / ctas) * 128 / 48.0);
         const double epilogue = 800.0 + p.nt * 24.0;
         double cost;
         if (ranged) {
-            const double join = 6000.0 + p.nt * 60.0;
+            const double join = 6000.0 + p.nt * 90.0;
             cost = (double)p.tiles * nkb / slots * step + join + epilogue;
+        } else if (cs > 1) {
+            cost = (double)((nkb + cs - 1) / cs) * step + 3000.0 + accs * p.nt * 12.0 + epilogue / cs;
         } else {
             cost = (double)((p.tiles + slots - 1) / slots) * nkb * step + epilogue;
         }
@@ -862,23 +974,27 @@ LinearPlan linear_plan(int rows, int k, int n, int mats, int sms) {
             best = p;
         }
     };
-    const int tm0 = (rows + 255) / 256;
+    const int tm0 = (rows + 255) / 256, pair_f = mats == 2 ? kLF / 2 : kLF;
     for (int tm = tm0; tm <= tm0 + 2; ++tm) {
         if (tm > tm0 && tm > rows) break;
-        // One CTA per tile: the feature count that makes the tiles fill one, two, ... waves.
-        for (int w = 1; w <= 4; ++w) {
-            const long long ft = (long long)sms * w / tm;
-            if (ft < 1) continue;
-            const int f = round_up((int)((n + ft - 1) / ft), 8);
-            if (f <= kLF) {
-                consider(false, tm, f, false);
-                break;
+        // One CTA (cluster) per tile: the feature count that makes the tiles fill one, two, ... waves.
+        for (int cs = 1; cs <= 8; ++cs) {
+            if (cs > nkb) break;
+            const int slots = cs > 1 ? max_clusters(cs, sms) : sms;
+            for (int w = 1; w <= (cs > 1 ? 1 : 4); ++w) {
+                const long long ft = (long long)slots * w / tm;
+                if (ft < 1) continue;
+                const int f = round_up((int)((n + ft - 1) / ft), 8);
+                if (f <= kLF) {
+                    consider(false, tm, f, cs, false);
+                    break;
+                }
             }
         }
-        consider(false, tm, kLF, true);
+        consider(false, tm, kLF, 1, true);
         if (rows > 32) {
-            consider(true, tm, mats == 2 ? kLF / 2 : kLF, false);
-            consider(true, tm, mats == 2 ? kLF / 2 : kLF, true);
+            for (int cs = 1; cs <= 4 && cs <= nkb; ++cs) consider(true, tm, pair_f, cs, false);
+            consider(true, tm, pair_f, 1, true);
         }
     }
     LinearPlan &p = best;
@@ -890,13 +1006,13 @@ LinearPlan linear_plan(int rows, int k, int n, int mats, int sms) {
     const bool by_step = k % kLK == 0 && !p.pair;
     const int step_rows = (p.pair ? kLF : p.f_rows * mats) + p.x_rows;
     p.kb = 1;
-    while (by_step && p.kb < 8 && 2 * p.kb * step_rows * 128 <= 40 * 1024 && nkb >= 4 * p.kb) p.kb *= 2;
+    while (by_step && p.kb < 8 && 2 * p.kb * step_rows * 128 <= 40 * 1024 && nkb >= 4 * p.kb * p.cs) p.kb *= 2;
     p.flat = p.kb == 1;
     p.stages = std::min<int>(kMaxStages, kRing / (p.kb * step_rows * 128));
     p.nk = (nkb + p.kb - 1) / p.kb;
     p.drain_steps = kDrainK / p.kb;
-    // Workers: a CTA (pair) per SM (two), no more than there is work for.
-    long long workers = std::max(1, sms / ctas);
+    // Workers: a CTA (pair, cluster) per SM (two, ...), no more than there is work for.
+    long long workers = p.cs > 1 ? p.tiles : std::max(1, sms / ctas);
     workers = std::min<long long>(workers, p.ranged ? p.tiles * p.nk : p.tiles);
     // Ranged: whole waves of tiles, but for the last one to two waves' (unless they divide).
     p.tiles_whole = p.tiles;
@@ -904,7 +1020,7 @@ LinearPlan linear_plan(int rows, int k, int n, int mats, int sms) {
         const long long waves = p.tiles / workers;
         p.tiles_whole = waves > 0 ? (waves - 1) * workers : 0;
     }
-    p.ctas = (int)workers * ctas;
+    p.ctas = (int)workers * ctas * p.cs;
     const long long units = (p.tiles - p.tiles_whole) * p.nk;
     p.range_units = (int)(units / workers), p.range_extra = (int)(units % workers);
     p.counters = (size_t)(p.tiles - p.tiles_whole) * ctas;
