@@ -1425,24 +1425,6 @@ size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
 bool aligned16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
-// Splits of the prefix's key tiles over CTAs (one CTA per SM).  A CTA's fixed cost (q staging, ring
-// ramp, join, partial) is worth about four tiles, and every split adds a partial to the merge.
-int prefix_splits(const brk_ctx *ctx, int units, int ntiles) {
-    const int most = std::min(32, std::max(1, ntiles / 2));
-    double best = 1e30;
-    int best_n = 1;
-    for (int n = 1; n <= most; ++n) {
-        const int tps = (ntiles + n - 1) / n;
-        const long long waves = ((long long)units * n + ctx->num_sms - 1) / ctx->num_sms;
-        const double cost = (double)waves * (tps + 4) + 0.25 * n;
-        if (cost < best - 1e-9) {
-            best = cost;
-            best_n = n;
-        }
-    }
-    return best_n;
-}
-
 int check_prefix_call(const brk_ctx *ctx, const brk_kv *prefix, int prefix_seq, int prefix_len, const brk_kv *kv,
                       int layer, const brk_attn_params *p, int batch, int n_tokens, const int32_t *past_len,
                       const void *q, int q_type, const void *out, int out_type) {
@@ -1501,14 +1483,12 @@ int run_decode_prefix(brk_ctx *ctx, const brk_kv *prefix, int prefix_seq, int pr
         if (prefix_len > 0 && prefix->q8()) k_begin = k_begin / 4 * 4;
     }
     const int keys = prefix_len - k_begin;
-    int splits = 0, tps = 0;
-    if (keys > 0) {
-        const int rb = brk::prefix_block_rows(D, batch * n_tokens * G);
-        const int ntiles = (keys + brk::prefix_tile_keys() - 1) / brk::prefix_tile_keys();
-        splits = prefix_splits(ctx, Hkv * ((batch * n_tokens * G + rb - 1) / rb), ntiles);
-        tps = (ntiles + splits - 1) / splits;
-        splits = (ntiles + tps - 1) / tps;  // no empty split
-    }
+    brk::PrefixPlan plan;
+    plan.parts = 0;
+    if (keys > 0)
+        plan = brk::prefix_plan(D, batch * n_tokens, G, Hkv, (keys + brk::prefix_tile_keys() - 1) / brk::prefix_tile_keys(),
+                                ctx->num_sms);
+    const int parts = plan.parts;
     int nsplit = 1, kps = 0;
     int rc = decode_split_plan(ctx, kv, p, batch, n_tokens, past_len, false, &nsplit, &kps);
     if (rc) return rc;
@@ -1524,66 +1504,96 @@ int run_decode_prefix(brk_ctx *ctx, const brk_kv *prefix, int prefix_seq, int pr
 
     const size_t n_ml = rows * 2 * sizeof(float), n_o = rows * D * sizeof(float);
     const size_t staged = keys > 0 && prefix->q8() ? (size_t)Hkv * keys * D * sizeof(__half) : 0;
-    const size_t off_o = align256(splits * n_ml), off_sml = off_o + align256(splits * n_o);
-    const size_t off_so = off_sml + (nsplit > 1 ? align256(nsplit * n_ml) : 0);
-    const size_t off_k = off_so + (nsplit > 1 ? align256(nsplit * n_o) : 0), off_v = off_k + align256(staged);
+    size_t bytes = 0;
+    auto take = [&](size_t n) {
+        const size_t at = bytes;
+        bytes += align256(n);
+        return at;
+    };
+    const size_t off_ml = take(parts * n_ml), off_o = take(parts * n_o);
+    const size_t off_sml = take(nsplit > 1 ? nsplit * n_ml : 0), off_so = take(nsplit > 1 ? nsplit * n_o : 0);
+    const size_t off_q = take(q_type == BRK_T_F32 ? rows * D * sizeof(__half) : 0);
+    const size_t off_k = take(staged), off_v = take(staged);
     brk_scratch *sc = nullptr;
-    rc = get_scratch(ctx, st, off_v + align256(staged), (size_t)units, &sc);
+    rc = get_scratch(ctx, st, bytes, (size_t)units, &sc);
     if (rc) return rc;
     char *ws = static_cast<char *>(sc->ws);
 
+    const __half *q16 = static_cast<const __half *>(q);
+    if (q_type == BRK_T_F32) {
+        __half *qh = reinterpret_cast<__half *>(ws + off_q);
+        cudaError_t e = brk::launch_half_rows(static_cast<const float *>(q), qh, rows * D, st, pdl);
+        if (e != cudaSuccess) return cuda_fail(e, "q cast launch");
+        ++ctx->launches;
+        q16 = qh;
+        pdl = true;
+    }
     if (keys > 0) {
         brk::PrefixArgs x;
         memset(&x, 0, sizeof(x));
-        x.q = q_type == BRK_T_F32 ? static_cast<const float *>(q) : nullptr;
-        x.q16 = q_type == BRK_T_F16 ? static_cast<const __half *>(q) : nullptr;
-        x.part_ml = reinterpret_cast<float *>(ws);
+        x.part_ml = reinterpret_cast<float *>(ws + off_ml);
         x.part_o = reinterpret_cast<float *>(ws + off_o);
         x.err = ctx->d_err;
         x.B = batch, x.T = n_tokens, x.Hq = p->n_heads, x.Hkv = Hkv, x.G = G;
-        x.rows = batch * n_tokens * G;
         x.k_begin = k_begin, x.k_end = prefix_len;
-        x.tiles_per_split = tps;
+        x.tiles_per_split = plan.tiles_per_split;
+        x.cluster = plan.cluster;
         x.window = window;
         x.scale_log2 = scale * (float)log2e;
         x.softcap = softcap, x.cap_k1 = cap_k1, x.cap_k2 = cap_k2;
         for (int b = 0; b < batch; ++b) x.past_len[b] = past_len[b];
         const size_t seg0 = ((size_t)layer * prefix->desc.batch + prefix_seq) * Hkv;
-        CUtensorMap mk, mv;
-        const CUtensorMap *tk = &prefix->tm_pre_k, *tv = &prefix->tm_pre_v;
+        CUtensorMap mk, mv, mq, ms;
+        const CUtensorMap *tk = &prefix->tm_pre_k, *tv = &prefix->tm_pre_v, *ts = &prefix->tm_pre_k;
+        x.scale_row = -1;
         if (staged) {
             __half *sk = reinterpret_cast<__half *>(ws + off_k), *sv = reinterpret_cast<__half *>(ws + off_v);
             const size_t off = seg0 * prefix->cap * D;
             cudaError_t e = brk::launch_codes_to_half(prefix->k8 + off, prefix->v8 + off, sk, sv, Hkv, D, prefix->cap,
-                                                      k_begin, keys, st);
+                                                      k_begin, keys, st, pdl);
             if (e != cudaSuccess) return cuda_fail(e, "prefix code staging launch");
             ++ctx->launches;
-            pdl = false;  // the staging kernel, an ordinary launch, is between the append and the prefix kernel
+            pdl = true;
             if ((rc = make_cache_map(&mk, sk, (uint64_t)Hkv * keys, D, brk::prefix_tile_keys()))) return rc;
             if ((rc = make_cache_map(&mv, sv, (uint64_t)Hkv * keys, D, brk::prefix_tile_keys()))) return rc;
-            tk = &mk, tv = &mv;
-            x.scales = prefix->scales + seg0 * 2 * prefix->scale_pitch;
-            x.scale_pitch = prefix->scale_pitch;
+            if ((rc = make_map(&ms, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, sizeof(float), prefix->scales,
+                               kv_segments(prefix->desc) * 2, (uint64_t)prefix->scale_pitch,
+                               (uint32_t)brk::prefix_tile_keys(), 2u, CU_TENSOR_MAP_SWIZZLE_NONE)))
+                return rc;
+            tk = &mk, tv = &mv, ts = &ms;
+            x.scale_row = (int)(seg0 * 2);
             x.row0 = -k_begin;
             x.head_rows = keys;
         } else {
             x.row0 = (int)(seg0 * prefix->cap);
             x.head_rows = prefix->cap;
         }
-        cudaError_t e = brk::launch_prefix(D, *tk, *tv, x, splits, st, pdl);
+        {
+            auto enc = tensor_map_encoder();
+            if (!enc) return fail(BRK_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+            cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)p->n_heads, (cuuint64_t)batch * n_tokens};
+            cuuint64_t strides[2] = {(cuuint64_t)D * 2, (cuuint64_t)p->n_heads * D * 2};
+            cuuint32_t box[3] = {64u, (cuuint32_t)G, (cuuint32_t)plan.tokens_box};
+            cuuint32_t estr[3] = {1u, 1u, 1u};
+            CUresult r = enc(&mq, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<__half *>(q16), dims, strides, box, estr,
+                             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+            if (r != CUDA_SUCCESS) return fail(BRK_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+        }
+        cudaError_t e = brk::launch_prefix(D, *tk, *tv, mq, *ts, x, plan, st, pdl);
         if (e != cudaSuccess) return cuda_fail(e, "prefix kernel launch");
         ++ctx->launches;
+        pdl = true;
     }
 
     brk::DecodeArgs a;
     memset(&a, 0, sizeof(a));
     a.with_prefix = 1;
     a.late_wait = keys > 0;
-    a.pre_parts = splits;
-    a.pre_ml = reinterpret_cast<const float *>(ws);
+    a.pre_parts = parts;
+    a.pre_ml = reinterpret_cast<const float *>(ws + off_ml);
     a.pre_o = reinterpret_cast<const float *>(ws + off_o);
-    a.q = q_type == BRK_T_F32 ? static_cast<const float *>(q) : nullptr;
-    a.q16 = q_type == BRK_T_F16 ? static_cast<const __half *>(q) : nullptr;
+    a.q16 = q16;
     a.out = out_type == BRK_T_F32 ? static_cast<float *>(out) : nullptr;
     a.out16 = out_type == BRK_T_F16 ? static_cast<__half *>(out) : nullptr;
     a.err = ctx->d_err;
@@ -1603,7 +1613,7 @@ int run_decode_prefix(brk_ctx *ctx, const brk_kv *prefix, int prefix_seq, int pr
     a.counters = sc->counters;
     for (int b = 0; b < batch; ++b) a.past_len[b] = past_len[b];
     cudaError_t e = brk::launch_decode(kv->q8(), D, kv->tm_dec_k, kv->tm_dec_v, kv->q8() ? kv->tm_dec_s : kv->tm_dec_k,
-                                       a, nsplit, Hkv * mtiles, batch, st, keys > 0 || pdl);
+                                       a, nsplit, Hkv * mtiles, batch, st, pdl);
     if (e != cudaSuccess) return cuda_fail(e, "decode kernel launch");
     ++ctx->launches;
     return BRK_OK;

@@ -260,7 +260,7 @@ __device__ __forceinline__ void patch_new_row(uint8_t *st, int rpos, const uint8
 
 // F: the fused-append form (brk_attn_step with one token); a separate instantiation, so that the
 // plain kernel's code and registers stay as they are.  H: the own rows of sequences that share a
-// prefix (brk_attn_decode_prefix): q f32 or fp16, and the final merge takes the prefix kernel's
+// prefix (brk_attn_decode_prefix): q in fp16, and the final merge takes the prefix kernel's
 // partials in; the cache streams while the prefix kernel still runs (a.late_wait: everything but
 // its partials was complete before this grid could start).
 template <bool Q8, int D, bool F, bool H = false>
@@ -493,7 +493,7 @@ __global__ void __launch_bounds__(decode_threads<Q8, D, F>(), DecodeCfg<Q8, D>::
     // Q^T fragments (B operand, column qr = query row row0 + qr), fp32 -> fp16: from global
     // memory, or (fused) from the staged rows.
     uint32_t qf[KS][2];
-    if (H && a.q16) {
+    if constexpr (H) {
         // fp16 q: the fragments' pairs as they are.
         const int rq = row0 + qr;
         const __half *qrow =

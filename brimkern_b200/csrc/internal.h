@@ -166,13 +166,13 @@ struct DecodeArgs {
     double eps;
     int one_plus;
     // Own rows of sequences that share a prefix (brk_attn_decode_prefix, decode_kernel's H form):
-    // q in fp16 (or a.q in f32), the prefix kernel's pre_parts partials [part][rows][2] and
+    // q in fp16, the prefix kernel's pre_parts partials [part][rows][2] and
     // [part][rows][D], the fp16 output (or a.out), and whether the preceding kernel of this call
     // is the prefix kernel, whose partials alone have to be waited for.
     int with_prefix;
     int late_wait;
     int pre_parts;
-    const __half *q16;
+    const __half *q16;      // replaces q
     const float *pre_ml, *pre_o;
     __half *out16;
     int past_len[BRK_MAX_BATCH];
@@ -180,22 +180,25 @@ struct DecodeArgs {
 
 // Attention of every sequence's query rows over one shared prefix (prefix.cu): partials only.
 struct PrefixArgs {
-    const float *q;       // [B][T][Hq][D] f32, or
-    const __half *q16;    //   fp16
-    float *part_ml;       // [split][B*T*Hq][2] (m natural-log units, l)
-    float *part_o;        // [split][B*T*Hq][D] unnormalised
-    const float *scales;  // int8 cache: this (layer, sequence)'s [kv head][2][scale_pitch], or nullptr
-    int scale_pitch;
+    float *part_ml;       // [part][B*T*Hq][2] (m natural-log units, l)
+    float *part_o;        // [part][B*T*Hq][D] unnormalised
+    int scale_row;        // int8 cache: the scale map's row of kv head 0 ([kv head][K, V]); -1: fp16
     int *err;
     int B, T, Hq, Hkv, G;
-    int rows;             // query rows per kv head: B * T * G
     int row0;             // map row of key 0 of kv head 0
     int head_rows;        // map rows from one kv head to the next
     int k_begin, k_end;   // keys some row attends
-    int tiles_per_split;
+    int tiles_per_split, cluster;
     int window;
     float scale_log2, softcap, cap_k1, cap_k2;
     int past_len[BRK_MAX_BATCH];
+};
+
+// How the prefix's work is cut: copies of the query rows in the MMA's rows, tokens per q box, row
+// blocks, key splits (`cluster` of them joined in a cluster), partials.
+struct PrefixPlan {
+    int copies = 1, tokens_box = 1, blocks = 1;
+    int splits = 1, cluster = 1, parts = 1, tiles_per_split = 1;
 };
 
 struct PrefillArgs {
@@ -345,15 +348,17 @@ int linear_rows_max();
 cudaError_t launch_linear_rows(int mats, const LinearArgs &a, cudaStream_t s);
 
 // Shared-prefix attention partials (prefix.cu): maps with prefix_tile_keys()-row boxes over fp16
-// rows (for an int8 cache: its codes as fp16, staged by launch_codes_to_half).  Query rows per CTA
-// for a head dim and row count: prefix_block_rows().
+// rows (for an int8 cache: its codes as fp16, staged by launch_codes_to_half, and its scales with
+// [2][64] boxes), tmq with boxes [tokens_box][group][64] over the fp16 q [tokens][heads][D].
 int prefix_tile_keys();
-int prefix_block_rows(int head_dim, int rows);
-cudaError_t launch_prefix(int head_dim, const CUtensorMap &tmk, const CUtensorMap &tmv, const PrefixArgs &a, int splits,
-                          cudaStream_t s, bool pdl);
+PrefixPlan prefix_plan(int head_dim, int tokens, int group, int kv_heads, int ntiles, int sms);
+cudaError_t launch_prefix(int head_dim, const CUtensorMap &tmk, const CUtensorMap &tmv, const CUtensorMap &tmq,
+                          const CUtensorMap &tms, const PrefixArgs &a, const PrefixPlan &p, cudaStream_t s, bool pdl);
+// n (a multiple of 8) fp16 values from f32 ones.
+cudaError_t launch_half_rows(const float *src, __half *dst, size_t n, cudaStream_t s, bool pdl);
 // Codes of rows [row0, row0 + rows) of every kv head of one (layer, sequence) as fp16 [Hkv][rows][D].
 cudaError_t launch_codes_to_half(const uint8_t *kc, const uint8_t *vc, __half *k, __half *v, int n_kv_heads,
-                                 int head_dim, int cap, int row0, int rows, cudaStream_t s);
+                                 int head_dim, int cap, int row0, int rows, cudaStream_t s, bool pdl);
 
 // Non-causal attention staging (full.cu): token-major f32 [B][L][H][D] K/V -> head-major fp16
 // [B][H][L][Dp] (zero-padded head dim), and f32 rows [rows][D] -> [rows][Dp] zero-padded.

@@ -9,9 +9,15 @@
 //   S = Q K^T (M 128, N 64) in TMEM, each row's softmax by one thread (running maximum and sum in
 //   f32), P as fp16 pairs in TMEM, O += P V in TMEM.
 // Two streams of 128 rows run a tile apart so that one's exponentials overlap the other's products:
-// with more than 128 rows in the block the streams are two row tiles that share every K/V tile; with
-// fewer they take alternate key tiles of the same rows, and their (m, l, O) are joined in shared
-// memory at the end.  head_dim 256 leaves TMEM for one stream.
+// with more rows than one stream holds the streams are two row tiles that share every K/V tile; with
+// fewer they take alternate key tiles of the same rows.  head_dim 256 leaves TMEM for one stream.
+// Few rows (COPIES 2 or 4): the MMA's 128 rows hold the same query rows 2 or 4 times, and each copy
+// takes its own 32 or 16 keys of a tile and leaves P = 0 for the others, so that all threads share the
+// exponentials instead of one warp doing them: what bounds the loop is then the K/V stream.
+//
+// The end: streams and copies are joined in shared memory, the splits of a cluster through distributed
+// shared memory, and one partial per cluster leaves in coalesced rows -- the partials are f32 and
+// would otherwise be as many bytes as the prefix itself.
 //
 // int8 prefix: the codes, as exact fp16 integers, are the operands; the K scale multiplies the
 // scores and the V scale the probabilities, so nothing is rounded that the fp16 form does not round.
@@ -43,14 +49,17 @@ struct PrefixLayout {
     static constexpr uint32_t kQBytes = kBlocks * kQBlock;
     static constexpr uint32_t kTileBytes = kBlocks * kKVBlock;
     static constexpr uint32_t kOffKV = kStreams * kQBytes;
-    static constexpr uint32_t kOffBar = kOffKV + kStages * 2 * kTileBytes;
+    static constexpr uint32_t kOffScale = kOffKV + kStages * 2 * kTileBytes;  // int8: [stage][K, V][64] f32
+    static constexpr uint32_t kOffState = kOffScale + kStages * 2 * kXK * 4;  // [m, l][stream][128], [m, l][256] f32
+    static constexpr uint32_t kOffBar = kOffState + 2 * kStreams * kXQ * 4 + 2 * 256 * 4;
     static constexpr uint32_t kSmemBytes = 1024 + kOffBar + 28 * 8 + 16;
     // TMEM columns: S, then P (fp16 pairs), then O from column 256 (one stream of D 256) or 192.
     static constexpr uint32_t kColS = 0, kColP = kStreams * kXK, kColO = kStreams == 1 ? 256 : 192;
     static_assert(kColP + kStreams * kXK / 2 <= kColO && kColO + kStreams * D <= kXTmemCols, "TMEM columns");
     static_assert(kSmemBytes <= 232448, "more than 227 KB of shared memory per CTA");
-    // The streams' join: stream 1's O [D][128] f32, then m and l, in the K/V ring.
-    static_assert(kStreams == 1 || (D * 128 + 256) * 4 <= kStages * 2 * kTileBytes, "join buffer");
+    // The join: every stream's O [128][kJoin] f32 over q and the ring; the padding spreads the banks.
+    static constexpr uint32_t kJoin = D + 4;
+    static_assert(kStreams * kXQ * kJoin * 4 <= kOffScale, "join buffer");
 };
 
 enum : int {
@@ -60,17 +69,76 @@ enum : int {
     kXSFree = 14,    // [2] softmax (S read) -> MMA
     kXPFull = 16,    // [2] softmax (P written, O rescaled) -> MMA
     kXODone = 18,    // [2] MMA commit (PV done) -> softmax
-    kXQFull = 20,    // q staged -> MMA
+    kXQFull = 20,    // TMA (q) -> MMA
     kXMmaDone = 21,  // [2] everything an issuer issued has completed -> teardown
     kXStagger = 23,  // stream 0's first P written -> stream 1's issuer starts
 };
 
-template <int D, bool CAP, bool Q8>
+// 3-D tiled TMA load (CTA-local).
+__device__ __forceinline__ void tma_load_q(void *dst, const CUtensorMap *map, int x, int y, int z, uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::
+            "r"(smem_addr(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_addr(bar))
+        : "memory");
+}
+__device__ __forceinline__ float4 ld_cluster_v4(const float *p, uint32_t rank) {
+    uint32_t at;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_addr(p)), "r"(rank));
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(at)
+                 : "memory");
+    return v;
+}
+
+// KC consecutive S columns of this thread's lane (no wait), and KC / 2 P columns.
+template <int KC>
+__device__ __forceinline__ void ld_scores(uint32_t taddr, uint32_t (&v)[KC]) {
+    if constexpr (KC == 16) {
+        asm volatile(
+            "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+            "%15}, [%16];"
+            : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+              "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+            : "r"(taddr));
+    } else {
+        uint32_t(&lo)[32] = reinterpret_cast<uint32_t(&)[32]>(v[0]);
+        tc_ld32_nowait(taddr, lo);
+        if constexpr (KC == 64) {
+            uint32_t(&hi)[32] = reinterpret_cast<uint32_t(&)[32]>(v[32]);
+            tc_ld32_nowait(taddr + 32, hi);
+        }
+    }
+}
+template <int N>
+__device__ __forceinline__ void st_probs(uint32_t taddr, const uint32_t (&r)[N]) {
+    if constexpr (N == 32) {
+        tc_st32(taddr, r);
+    } else if constexpr (N == 16) {
+        asm volatile(
+            "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
+            "%14, %15, %16};" ::"r"(taddr),
+            "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+            "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+            : "memory");
+    } else {
+        asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr),
+                     "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                     : "memory");
+    }
+}
+
+template <int D, int COPIES, bool Q8>
 __global__ void __launch_bounds__(PrefixLayout<D>::kThreads, 1)
     prefix_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
+                  const __grid_constant__ CUtensorMap tmq, const __grid_constant__ CUtensorMap tms,
                   const __grid_constant__ PrefixArgs a) {
     using L = PrefixLayout<D>;
     constexpr int NS = L::kStreams;
+    constexpr int RC = kXQ / COPIES;  // MMA rows of a copy
+    constexpr int KC = kXK / COPIES;  // keys of a tile that a copy takes
     // Raise the running max (and rescale O) only when a tile's max exceeds it by more than this
     // many powers of two: P stays below 2^8, or, times an int8 row's V scale, below 4 scales.
     constexpr float kRaise = Q8 ? 2.f : 8.f;
@@ -81,10 +149,11 @@ __global__ void __launch_bounds__(PrefixLayout<D>::kThreads, 1)
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int split = blockIdx.x, kvh = blockIdx.y;
-    constexpr int RB = NS * kXQ;
-    const int blk0 = blockIdx.z * RB;                 // first row of the block
-    const int nblk = min(RB, a.rows - blk0);          // rows of the block
-    const bool pair = nblk > kXQ;                     // streams: two row tiles, or alternate key tiles
+    // Tokens (of any sequence) in the block: G query rows each, nbt to a stream's copy.
+    const int nbt = RC / a.G, bt_total = a.B * a.T;
+    const int bt0 = blockIdx.z * (NS == 2 && COPIES == 1 ? 2 : 1) * nbt;
+    const int n_bt = min((NS == 2 && COPIES == 1 ? 2 : 1) * nbt, bt_total - bt0);
+    const bool pair = NS == 2 && COPIES == 1 && n_bt > nbt;  // streams: two row tiles, or alternate key tiles
     const int kb = a.k_begin + split * a.tiles_per_split * kXK;
     const int ke = min(a.k_end, kb + a.tiles_per_split * kXK);
     const int nk = kb < ke ? (ke - kb + kXK - 1) / kXK : 0;
@@ -106,7 +175,7 @@ __global__ void __launch_bounds__(PrefixLayout<D>::kThreads, 1)
             mbar_init(&bars[kXODone + s], 1);
             mbar_init(&bars[kXMmaDone + s], 1);
         }
-        mbar_init(&bars[kXQFull], NS * 128);
+        mbar_init(&bars[kXQFull], 1);
         mbar_init(&bars[kXStagger], 128);
         fence_barrier_init();
     }
@@ -115,6 +184,11 @@ __global__ void __launch_bounds__(PrefixLayout<D>::kThreads, 1)
                      "r"(kXTmemCols)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    } else if (warp == L::kProducer && lane == 0) {
+        tma_prefetch_desc(&tmk);
+        tma_prefetch_desc(&tmv);
+        tma_prefetch_desc(&tmq);
+        if constexpr (Q8) tma_prefetch_desc(&tms);
     }
     tc_fence_before();
     __syncthreads();
@@ -124,29 +198,39 @@ __global__ void __launch_bounds__(PrefixLayout<D>::kThreads, 1)
     auto sQ = [&](int s) { return smem + (pair ? s : 0) * L::kQBytes; };
     auto sK = [&](int st) { return smem + L::kOffKV + st * 2 * L::kTileBytes; };
     auto sV = [&](int st) { return smem + L::kOffKV + st * 2 * L::kTileBytes + L::kTileBytes; };
+    float *sScale = reinterpret_cast<float *>(smem + L::kOffScale);
 
     if (warp == L::kProducer) {
         if (lane == 0) {
-            tma_prefetch_desc(&tmk);
-            tma_prefetch_desc(&tmv);
-            griddep_wait();  // the rows, or the staged codes, may come from the kernel before
+            griddep_wait();  // q, the cache rows, or the staged codes may come from the kernel before
             // Everything before this grid is complete: the own rows' kernel may start streaming.
             griddep_launch_dependents();
+            // q: boxes [nbt tokens][G heads][64] -- rows of 128 bytes in the MMA's K-major layout.  Rows
+            // of a copy past nbt * G, and past the last token, hold anything: no output takes them.
+            const int tiles = pair ? 2 : COPIES;
+            mbar_arrive_expect_tx(&bars[kXQFull], (uint32_t)(tiles * L::kBlocks * nbt * a.G * 128));
+            for (int t = 0; t < tiles; ++t)
+#pragma unroll
+                for (int blk = 0; blk < L::kBlocks; ++blk)
+                    tma_load_q(smem + (pair ? t * L::kQBytes : t * RC * 128) + blk * L::kQBlock, &tmq, blk * 64, kvh * a.G,
+                               bt0 + (pair ? t * nbt : 0), &bars[kXQFull]);
             int issued = 0;
             for (int j = 0; j < nk; ++j) {
                 const int st = j % L::kStages;
                 if (j >= L::kStages && !mbar_wait(&bars[kXKvEmpty + st], ((j / L::kStages) - 1) & 1, a.err, kErrSlotTimeout))
                     break;
-                const int y = seg_row + kb + j * kXK;
-                mbar_arrive_expect_tx(&bars[kXKvFull + st], 2 * L::kTileBytes);
+                const int key = kb + j * kXK, y = seg_row + key;
+                mbar_arrive_expect_tx(&bars[kXKvFull + st], 2 * L::kTileBytes + (Q8 ? 2 * kXK * 4 : 0));
 #pragma unroll
                 for (int blk = 0; blk < L::kBlocks; ++blk)
                     tma_load_2d(sK(st) + blk * L::kKVBlock, &tmk, blk * 64, y, &bars[kXKvFull + st]);
 #pragma unroll
                 for (int blk = 0; blk < L::kBlocks; ++blk)
                     tma_load_2d(sV(st) + blk * L::kKVBlock, &tmv, blk * 64, y, &bars[kXKvFull + st]);
+                if constexpr (Q8) tma_load_2d(sScale + st * 2 * kXK, &tms, key, a.scale_row + kvh * 2, &bars[kXKvFull + st]);
                 issued = j + 1;
             }
+            mbar_wait(&bars[kXQFull], 0, a.err, kErrTmaTimeout);
             for (int j = issued > L::kStages ? issued - L::kStages : 0; j < issued; ++j)
                 mbar_wait(&bars[kXKvFull + j % L::kStages], (j / L::kStages) & 1, a.err, kErrTmaTimeout);
         }
@@ -202,169 +286,137 @@ __global__ void __launch_bounds__(PrefixLayout<D>::kThreads, 1)
         }
         __syncwarp();
     } else {
-        // ---- softmax warps: stream s = warp / 4, thread r <-> row r of the stream (TMEM lane r).
+        // ---- softmax warps: stream s = warp / 4, thread r <-> MMA row r of the stream (TMEM lane r).
         const int s = warp >> 2, r = threadIdx.x & 127;
         const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
-        const int TG = a.T * a.G;
-        griddep_wait();  // q may come from the kernel before
-        // Stage q as fp16 rows in the MMA's swizzled K-major layout: a warp per row, lane l holding
-        // PE consecutive elements, eight rows' loads in flight.
-        {
-            constexpr int PE = D / 32, kB = 8;
-            const int tiles = pair ? 2 : 1;
-#pragma unroll 1
-            for (int base = 0; base < tiles * kXQ; base += L::kSoftWarps * kB) {
-                uint32_t h[kB][PE / 2];
-#pragma unroll
-                for (int u = 0; u < kB; ++u) {
-                    const int rr = base + u * L::kSoftWarps + warp;
-                    const bool okr = rr < nblk;
-                    const int row = blk0 + (okr ? rr : 0);
-                    const int b = row / TG, tg = row % TG;
-                    const size_t R = ((size_t)b * a.T + tg / a.G) * a.Hq + kvh * a.G + tg % a.G;
-                    if (a.q16) {
-                        const uint32_t *src = reinterpret_cast<const uint32_t *>(a.q16 + R * D) + lane * (PE / 2);
-#pragma unroll
-                        for (int e = 0; e < PE / 2; ++e) h[u][e] = okr ? src[e] : 0u;
-                    } else {
-                        const float2 *src = reinterpret_cast<const float2 *>(a.q + R * D) + lane * (PE / 2);
-#pragma unroll
-                        for (int e = 0; e < PE / 2; ++e) {
-                            const float2 x = okr ? src[e] : make_float2(0.f, 0.f);
-                            h[u][e] = pack_half2(x.x, x.y);
-                        }
-                    }
-                }
-#pragma unroll
-                for (int u = 0; u < kB; ++u) {
-                    const int rr = base + u * L::kSoftWarps + warp;
-                    const int i = PE * lane;
-                    uint8_t *d = smem + (rr >> 7) * L::kQBytes + (i >> 6) * L::kQBlock + sw128(rr & 127, (i & 63) >> 3) +
-                                 (i & 7) * 2;
-#pragma unroll
-                    for (int e = 0; e < PE / 2; ++e) reinterpret_cast<uint32_t *>(d)[e] = h[u][e];
-                }
-            }
-            fence_proxy_async_smem();
-            mbar_arrive(&bars[kXQFull]);
-        }
+        const int copy = r / RC, rc = r % RC;      // the copy is the same for the whole warp
+        const int bt_of = rc / a.G;                // token within the stream's tile
+        const int bt = bt0 + (pair ? s * nbt : 0) + bt_of;
+        const bool row_ok = bt_of < nbt && bt < bt_total;
         const int cnt = tile_count(s), j0 = first_tile(s);
-        const int rr = (pair ? s * kXQ : 0) + r;
-        const bool row_ok = rr < nblk;
-        const int row = blk0 + (row_ok ? rr : 0);
-        const int b = row / TG, tg = row % TG;
-        const size_t R = ((size_t)b * a.T + tg / a.G) * a.Hq + kvh * a.G + tg % a.G;
-        const int lo = a.window > 0 && row_ok ? a.past_len[b] + tg / a.G - a.window + 1 : INT_MIN;
-        const uint32_t tS = tmem + L::kColS + s * kXK + lane_base;
+        const int lo = a.window > 0 && row_ok ? a.past_len[bt / a.T] + bt % a.T - a.window + 1 : INT_MIN;
+        const uint32_t tS = tmem + L::kColS + s * kXK + lane_base + copy * KC;
         const uint32_t tO = tmem + L::kColO + s * D + lane_base;
         const uint32_t tP = tmem + L::kColP + s * (kXK / 2) + lane_base;
-        const float *ksc = Q8 ? a.scales + (size_t)kvh * 2 * a.scale_pitch : nullptr;
-        const float *vsc = Q8 ? ksc + a.scale_pitch : nullptr;
+        // A warp without rows only keeps the barriers going.
+        const bool idle = !__any_sync(0xffffffffu, row_ok);
+        if (COPIES > 1 || idle) {
+            // The keys of the other copies: P = 0 for good.
+            uint32_t zero[32];
+#pragma unroll
+            for (int e = 0; e < 32; ++e) zero[e] = 0u;
+            tc_st32(tP, zero);
+            tc_wait_st();
+        }
         float m_used = -CUDART_INF_F;  // the maximum that the probabilities are relative to (log2 units)
         float l_run = 0.f;
         bool ok = true;
+        const bool cap = a.softcap > 0.f;
         for (int i = 0; i < cnt; ++i) {
-            const int j = j0 + i * step, kbase = kb + j * kXK;
-            const bool inside = kbase + kXK <= ke;
+            const int j = j0 + i * step, st = j % L::kStages;
+            const int kbase = kb + j * kXK + copy * KC;  // this thread's first key
+            const bool tail = kb + (j + 1) * kXK > ke;
             if (!__all_sync(0xffffffffu, mbar_wait(&bars[kXSFull + s], i & 1, a.err, kErrMmaTimeout))) {
                 ok = false;
                 break;
             }
             tc_fence_after();
-            uint32_t raw[2][32];
-            tc_ld32_nowait(tS, raw[0]);
-            tc_ld32_nowait(tS + 32, raw[1]);
-            tc_wait_ld();
-            tc_fence_before();
-            mbar_arrive(&bars[kXSFree + s]);
-            float v[64];
+            bool waited = false;
+            uint32_t pk[KC / 2];
+            float rsum = 0.f;
+            if (idle) {
+                mbar_arrive(&bars[kXSFree + s]);
+            } else {
+                float v[KC];
+                {
+                    uint32_t raw[KC];
+                    ld_scores<KC>(tS, raw);
+                    tc_wait_ld();
+                    tc_fence_before();
+                    mbar_arrive(&bars[kXSFree + s]);
 #pragma unroll
-            for (int e = 0; e < 64; ++e) v[e] = __uint_as_float(raw[e >> 5][e & 31]);
-            if constexpr (Q8) {
-                if (inside) {
+                    for (int e = 0; e < KC; ++e) v[e] = __uint_as_float(raw[e]);
+                }
+                const float *ksc = sScale + st * 2 * kXK + copy * KC, *vsc = ksc + kXK;
+                if constexpr (Q8) {
 #pragma unroll
-                    for (int e = 0; e < 64; e += 4) {
-                        const float4 k4 = *reinterpret_cast<const float4 *>(ksc + kbase + e);
+                    for (int e = 0; e < KC; e += 4) {
+                        const float4 k4 = *reinterpret_cast<const float4 *>(ksc + e);
                         v[e] *= k4.x, v[e + 1] *= k4.y, v[e + 2] *= k4.z, v[e + 3] *= k4.w;
                     }
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 64; ++e) v[e] *= kbase + e < ke ? ksc[kbase + e] : 0.f;
                 }
-            }
-            const bool edge = !inside || kbase < lo;
-            if (__any_sync(0xffffffffu, edge)) {
+                const bool edge = __any_sync(0xffffffffu, tail || kbase < lo);
+                if (edge) {
 #pragma unroll
-                for (int e = 0; e < 64; ++e) v[e] = kbase + e >= lo && kbase + e < ke ? v[e] : -CUDART_INF_F;
-            }
-            auto score = [&](float dot) {
-                if constexpr (CAP)
-                    return softcap_log2(dot, a.cap_k1, a.cap_k2);
-                else
-                    return dot * a.scale_log2;
-            };
-            const float mraw = max_tree(v);
-            const float mt = mraw == -CUDART_INF_F ? -CUDART_INF_F : score(mraw);
-            // Rows raise their maximum separately; the rescale pass is warp-collective.
-            const bool raise = mt > m_used + kRaise || (m_used == -CUDART_INF_F && mt != -CUDART_INF_F);
-            const bool rescale = raise && m_used != -CUDART_INF_F && i >= 1;
-            bool waited = false;
-            if (__any_sync(0xffffffffu, rescale)) {
-                const bool got = mbar_wait(&bars[kXODone + s], (i - 1) & 1, a.err, kErrMmaTimeout);
-                if (!__all_sync(0xffffffffu, got)) {
-                    ok = false;
-                    break;
+                    for (int e = 0; e < KC; ++e) v[e] = kbase + e >= lo && kbase + e < ke ? v[e] : -CUDART_INF_F;
                 }
-                waited = true;
-                tc_fence_after();
-                const float alpha = rescale ? ex2_fast(m_used - mt) : 1.f;
+                const float mraw = max_tree(v);
+                const float mt = mraw == -CUDART_INF_F ? -CUDART_INF_F
+                                 : cap                 ? softcap_log2(mraw, a.cap_k1, a.cap_k2)
+                                                       : mraw * a.scale_log2;
+                // Rows raise their maximum separately; the rescale pass is warp-collective.
+                const bool raise = mt > m_used + kRaise || (m_used == -CUDART_INF_F && mt != -CUDART_INF_F);
+                const bool rescale = raise && m_used != -CUDART_INF_F && i >= 1;
+                if (__any_sync(0xffffffffu, rescale)) {
+                    const bool got = mbar_wait(&bars[kXODone + s], (i - 1) & 1, a.err, kErrMmaTimeout);
+                    if (!__all_sync(0xffffffffu, got)) {
+                        ok = false;
+                        break;
+                    }
+                    waited = true;
+                    tc_fence_after();
+                    const float alpha = rescale ? ex2_fast(m_used - mt) : 1.f;
 #pragma unroll 1
-                for (int c = 0; c < D / 32; ++c) {
-                    uint32_t o[32];
-                    tc_ld32_nowait(tO + c * 32, o);
-                    tc_wait_ld();
+                    for (int c = 0; c < D / 32; ++c) {
+                        uint32_t o[32];
+                        tc_ld32_nowait(tO + c * 32, o);
+                        tc_wait_ld();
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-                    tc_st32(tO + c * 32, o);
+                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+                        tc_st32(tO + c * 32, o);
+                    }
+                    tc_wait_st();
+                    l_run *= alpha;
                 }
-                tc_wait_st();
-                l_run *= alpha;
-            }
-            if (raise) m_used = mt;
-            const float m_eff = m_used == -CUDART_INF_F ? 0.f : m_used;
-            float2 acc[4];
+                if (raise) m_used = mt;
+                const float m_eff = m_used == -CUDART_INF_F ? 0.f : m_used;
+                if (cap) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) acc[k] = make_float2(0.f, 0.f);
-            uint32_t pk[32];
-#pragma unroll
-            for (int u = 0; u < 32; ++u) {
-                float p0, p1;
-                if constexpr (CAP) {
-                    p0 = v[2 * u] == -CUDART_INF_F ? 0.f : ex2_fast(score(v[2 * u]) - m_eff);
-                    p1 = v[2 * u + 1] == -CUDART_INF_F ? 0.f : ex2_fast(score(v[2 * u + 1]) - m_eff);
+                    for (int e = 0; e < KC; ++e) {
+                        const float p = ex2_fast(softcap_log2(v[e], a.cap_k1, a.cap_k2) - m_eff);
+                        v[e] = v[e] == -CUDART_INF_F ? 0.f : p;
+                    }
                 } else {
-                    const float2 x = ffma2(make_float2(v[2 * u], v[2 * u + 1]), make_float2(a.scale_log2, a.scale_log2),
-                                           make_float2(-m_eff, -m_eff));
-                    p0 = ex2_fast(x.x);
-                    p1 = ex2_fast(x.y);
-                }
-                acc[u & 3] = fadd2(acc[u & 3], make_float2(p0, p1));
-                if constexpr (Q8) {
-                    // The V scale goes into the probability (a masked key's is not looked at).
-                    const int key = kbase + 2 * u;
-                    if (inside) {
-                        const float2 s2 = *reinterpret_cast<const float2 *>(vsc + key);
-                        p0 = v[2 * u] == -CUDART_INF_F ? 0.f : p0 * s2.x;
-                        p1 = v[2 * u + 1] == -CUDART_INF_F ? 0.f : p1 * s2.y;
-                    } else {
-                        p0 = v[2 * u] == -CUDART_INF_F ? 0.f : p0 * vsc[key];
-                        p1 = v[2 * u + 1] == -CUDART_INF_F ? 0.f : p1 * vsc[key + 1];
+                    const float2 sc2 = make_float2(a.scale_log2, a.scale_log2), nm2 = make_float2(-m_eff, -m_eff);
+#pragma unroll
+                    for (int u = 0; u < KC / 2; ++u) {
+                        const float2 x = ffma2(make_float2(v[2 * u], v[2 * u + 1]), sc2, nm2);
+                        v[2 * u] = ex2_fast(x.x);
+                        v[2 * u + 1] = ex2_fast(x.y);
                     }
                 }
-                pk[u] = pack_half2(p0, p1);
+                float2 acc[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) acc[k] = make_float2(0.f, 0.f);
+#pragma unroll
+                for (int u = 0; u < KC / 2; ++u) acc[u & 3] = fadd2(acc[u & 3], make_float2(v[2 * u], v[2 * u + 1]));
+                const float2 acc01 = fadd2(acc[0], acc[1]), acc23 = fadd2(acc[2], acc[3]);
+                rsum = (acc01.x + acc01.y) + (acc23.x + acc23.y);
+                if constexpr (Q8) {
+                    // The V scale goes into the probability; a masked key's (P 0) is not taken, as it
+                    // may be anything.
+#pragma unroll
+                    for (int e = 0; e < KC; e += 4) {
+                        const float4 s4 = *reinterpret_cast<const float4 *>(vsc + e);
+                        const float sv[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+                        for (int h = 0; h < 4; ++h)
+                            v[e + h] = edge && (kbase + e + h < lo || kbase + e + h >= ke) ? 0.f : v[e + h] * sv[h];
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < KC / 2; ++u) pk[u] = pack_half2(v[2 * u], v[2 * u + 1]);
             }
-            const float2 acc01 = fadd2(acc[0], acc[1]), acc23 = fadd2(acc[2], acc[3]);
-            const float rsum = (acc01.x + acc01.y) + (acc23.x + acc23.y);
             if (i >= 1 && !waited) {
                 const bool got = mbar_wait(&bars[kXODone + s], (i - 1) & 1, a.err, kErrMmaTimeout);
                 if (!__all_sync(0xffffffffu, got)) {
@@ -372,28 +424,28 @@ __global__ void __launch_bounds__(PrefixLayout<D>::kThreads, 1)
                     break;
                 }
             }
-            tc_st32(tP, pk);
+            if (!idle) st_probs<KC / 2>(tP + copy * (KC / 2), pk);
             // Keys past the range end: zero V rows, so that 0 * (whatever the tile holds) stays 0.
-            if ((s == 0 || !pair) && !inside) {
-                bool zok = true;
-                if (r < kXK && kbase + r >= ke) {
-                    zok = mbar_wait(&bars[kXKvFull + j % L::kStages], (j / L::kStages) & 1, a.err, kErrTmaTimeout);
-                    if (zok) {
-#pragma unroll
-                        for (int blk = 0; blk < L::kBlocks; ++blk)
-#pragma unroll
-                            for (int c = 0; c < 8; ++c)
-                                *reinterpret_cast<uint4 *>(sV(j % L::kStages) + blk * L::kKVBlock + sw128(r, c)) =
-                                    make_uint4(0u, 0u, 0u, 0u);
-                    }
-                }
-                if (!__all_sync(0xffffffffu, zok)) {
+            if ((s == 0 || !pair) && tail) {
+                const int key = kb + j * kXK + r;
+                if (!__all_sync(0xffffffffu, mbar_wait(&bars[kXKvFull + st], (j / L::kStages) & 1, a.err, kErrTmaTimeout))) {
                     ok = false;
                     break;
                 }
+                if (r < kXK && key >= ke) {
+#pragma unroll
+                    for (int blk = 0; blk < L::kBlocks; ++blk)
+#pragma unroll
+                        for (int c = 0; c < 8; ++c)
+                            *reinterpret_cast<uint4 *>(sV(st) + blk * L::kKVBlock + sw128(r, c)) = make_uint4(0u, 0u, 0u, 0u);
+                }
+                __syncwarp();
                 fence_proxy_async_smem();
             }
             tc_wait_st();
+            // The scales of this stage were read with ordinary loads; the stage's next copies are
+            // asynchronous and ordered behind this fence through the product's commit.
+            if constexpr (Q8) fence_proxy_async_smem();
             tc_fence_before();
             mbar_arrive(&bars[kXPFull + s]);
             if (s == 0 && i == 0) mbar_arrive(&bars[kXStagger]);
@@ -402,68 +454,112 @@ __global__ void __launch_bounds__(PrefixLayout<D>::kThreads, 1)
         // Every product of this stream has landed.
         if (ok && cnt > 0) ok = __all_sync(0xffffffffu, mbar_wait(&bars[kXODone + s], (cnt - 1) & 1, a.err, kErrMmaTimeout));
         tc_fence_after();
-        const int rows_total = a.B * a.T * a.Hq;
-        float *dst = a.part_o + ((size_t)split * rows_total + R) * D;
-        float f0 = 1.f, f1 = 0.f, m_fin = m_used, l_fin = l_run;
-        float *jo = reinterpret_cast<float *>(smem + L::kOffKV);  // [D][128]
-        float *jm = jo + D * 128, *jl = jm + 128;
-        if (NS == 2 && !pair) {
-            // Join the streams: stream 1 leaves its rows in the K/V ring (free: both streams'
-            // products, which read it, are complete at the barrier), stream 0 adds them to its own.
-            named_barrier_sync(1, 256);
-            if (s == 1) {
-                jm[r] = m_used;
-                jl[r] = l_run;
-#pragma unroll 1
-                for (int c = 0; cnt > 0 && c < D / 32; ++c) {
-                    uint32_t o[32];
-                    tc_ld32_nowait(tO + c * 32, o);
-                    tc_wait_ld();
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) jo[(c * 32 + e) * 128 + r] = __uint_as_float(o[e]);
-                }
-            }
-            named_barrier_sync(1, 256);
-            if (s == 0) {
-                const float m1 = jm[r];
-                m_fin = fmaxf(m_used, m1);
-                const float m_eff = m_fin == -CUDART_INF_F ? 0.f : m_fin;
-                f0 = ex2_fast(m_used - m_eff);
-                f1 = ex2_fast(m1 - m_eff);
-                l_fin = l_run * f0 + jl[r] * f1;
-            }
-        }
-        if (s == 0 || pair) {
-            const bool other = NS == 2 && !pair && tile_count(1) > 0;
+        // ---- join.  Every stream's (m, l, O) to shared memory, over q and the ring: all products that
+        // read them are complete behind the barrier.
+        constexpr int NT = L::kSoftWarps * 32;
+        float *jo = reinterpret_cast<float *>(smem);                 // [stream][128][kJoin]
+        float *jm = reinterpret_cast<float *>(smem + L::kOffState);  // [stream][128] m, then l
+        float *jl = jm + NS * kXQ;
+        float *rm = jl + NS * kXQ, *rl = rm + 256;                   // the CTA's rows: m, l
+        named_barrier_sync(1, NT);
+        jm[s * kXQ + r] = m_used;
+        jl[s * kXQ + r] = l_run;
+        if (!idle && cnt > 0) {
 #pragma unroll 1
             for (int c = 0; c < D / 32; ++c) {
                 uint32_t o[32];
+                tc_ld32_nowait(tO + c * 32, o);
+                tc_wait_ld();
+                uint4 *dst = reinterpret_cast<uint4 *>(jo + (size_t)(s * kXQ + r) * L::kJoin + c * 32);
 #pragma unroll
-                for (int e = 0; e < 32; ++e) o[e] = 0u;
-                if (cnt > 0) {
-                    tc_ld32_nowait(tO + c * 32, o);
-                    tc_wait_ld();
-                }
-                float y[32];
+                for (int e = 0; e < 8; ++e) dst[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+            }
+        }
+        named_barrier_sync(1, NT);
+        // The CTA's rows: x over (token, head), a thread per four elements.  Sources: the copies of
+        // every stream that took tiles (pair: the row's own stream).
+        const int n_rows = n_bt * a.G, rt = nbt * a.G;
+        constexpr int D4 = D / 4;
+        const size_t rows_total = (size_t)bt_total * a.Hq;
+        const bool in_cluster = a.cluster > 1;
+        const int part = split / a.cluster;
+        float *out_o = a.part_o + (size_t)part * rows_total * D, *out_ml = a.part_ml + (size_t)part * rows_total * 2;
+        for (int e = threadIdx.x; e < n_rows * D4; e += NT) {
+            const int x = e / D4, d4 = e % D4;
+            const int sx = pair ? x / rt : 0, rx = pair ? x % rt : x;
+            constexpr int MOST = NS * COPIES;
+            float m[MOST], M = -CUDART_INF_F;
 #pragma unroll
-                for (int e = 0; e < 32; ++e) {
-                    y[e] = __uint_as_float(o[e]) * f0;
-                    if (other) y[e] = fmaf(jo[(c * 32 + e) * 128 + r], f1, y[e]);
-                }
-                if (row_ok) {
+            for (int q = 0; q < MOST; ++q) {
+                const int sq = COPIES == 1 ? (pair ? sx : q) : q / COPIES;
+                const bool there = !(pair && q > 0) && tile_count(sq) > 0;
+                m[q] = there ? jm[sq * kXQ + (q % COPIES) * RC + rx] : -CUDART_INF_F;
+                M = fmaxf(M, m[q]);
+            }
+            float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+            float l = 0.f;
 #pragma unroll
-                    for (int e = 0; e < 32; e += 4)
-                        *reinterpret_cast<float4 *>(dst + c * 32 + e) = make_float4(y[e], y[e + 1], y[e + 2], y[e + 3]);
+            for (int q = 0; q < MOST; ++q) {
+                if (m[q] != -CUDART_INF_F) {
+                    const int sq = COPIES == 1 ? (pair ? sx : q) : q / COPIES;
+                    const int at = sq * kXQ + (q % COPIES) * RC + rx;
+                    const float f = ex2_fast(m[q] - M);
+                    const float4 y = *reinterpret_cast<const float4 *>(jo + (size_t)at * L::kJoin + 4 * d4);
+                    O.x = fmaf(f, y.x, O.x), O.y = fmaf(f, y.y, O.y), O.z = fmaf(f, y.z, O.z), O.w = fmaf(f, y.w, O.w);
+                    l = fmaf(f, jl[at], l);
                 }
             }
-            if (row_ok) {
-                float *ml = a.part_ml + ((size_t)split * rows_total + R) * 2;
-                *reinterpret_cast<float2 *>(ml) =
-                    make_float2(m_fin == -CUDART_INF_F ? -CUDART_INF_F : m_fin * kXLn2, l_fin);
+            if (in_cluster) {
+                // In place of the row's first source: only this thread reads these four elements.
+                *reinterpret_cast<float4 *>(jo + (size_t)(sx * kXQ + rx) * L::kJoin + 4 * d4) = O;
+                if (d4 == 0) rm[x] = M, rl[x] = l;
+            } else {
+                const size_t R = (size_t)(bt0 + x / a.G) * a.Hq + kvh * a.G + x % a.G;
+                *reinterpret_cast<float4 *>(out_o + R * D + 4 * d4) = O;
+                if (d4 == 0)
+                    *reinterpret_cast<float2 *>(out_ml + R * 2) = make_float2(M == -CUDART_INF_F ? M : M * kXLn2, l);
+            }
+        }
+        if (in_cluster) {
+            cluster_sync_all();  // every split's rows are in its CTA's shared memory
+            const int cs = a.cluster, me = split % cs;
+            const int total = n_rows * D4, share = (total + cs - 1) / cs;
+            for (int e = me * share + threadIdx.x; e < min(total, (me + 1) * share); e += NT) {
+                const int x = e / D4, d4 = e % D4;
+                const int sx = pair ? x / rt : 0, rx = pair ? x % rt : x;
+                const float *src = jo + (size_t)(sx * kXQ + rx) * L::kJoin + 4 * d4;
+                float m[8], lq[8], M = -CUDART_INF_F;
+                float4 y[8];
+#pragma unroll
+                for (int q = 0; q < 8; ++q) {
+                    const bool there = q < cs;
+                    m[q] = there ? ld_cluster_f32(rm + x, q) : -CUDART_INF_F;
+                    lq[q] = there ? ld_cluster_f32(rl + x, q) : 0.f;
+                    y[q] = there ? ld_cluster_v4(src, q) : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+#pragma unroll
+                for (int q = 0; q < 8; ++q) M = fmaxf(M, m[q]);
+                float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+                float l = 0.f;
+#pragma unroll
+                for (int q = 0; q < 8; ++q) {
+                    const float f = m[q] == -CUDART_INF_F ? 0.f : ex2_fast(m[q] - M);
+                    O.x = fmaf(f, y[q].x, O.x), O.y = fmaf(f, y[q].y, O.y), O.z = fmaf(f, y[q].z, O.z),
+                    O.w = fmaf(f, y[q].w, O.w);
+                    l = fmaf(f, lq[q], l);
+                }
+                const size_t R = (size_t)(bt0 + x / a.G) * a.Hq + kvh * a.G + x % a.G;
+                *reinterpret_cast<float4 *>(out_o + R * D + 4 * d4) = O;
+                if (d4 == 0)
+                    *reinterpret_cast<float2 *>(out_ml + R * 2) = make_float2(M == -CUDART_INF_F ? M : M * kXLn2, l);
             }
         }
     }
     // Teardown: every TMEM access and MMA is complete; the allocating warp releases TMEM.
+    if (a.cluster > 1) {
+        if (warp >= L::kProducer) cluster_sync_all();  // the softmax warps' first barrier counts every thread
+        cluster_sync_all();                            // no CTA leaves while another may still read its rows
+    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -471,47 +567,111 @@ __global__ void __launch_bounds__(PrefixLayout<D>::kThreads, 1)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kXTmemCols) : "memory");
 }
 
-template <int D, bool CAP, bool Q8>
-cudaError_t launch_prefix_t(const CUtensorMap &tmk, const CUtensorMap &tmv, const PrefixArgs &a, int splits,
-                            cudaStream_t s, bool pdl) {
-    using L = PrefixLayout<D>;
+template <int D, int COPIES, bool Q8>
+cudaError_t configure_prefix() {
     static unsigned long long configured = 0;  // one bit per device: the opt-in is per device
     int dev = 0;
     cudaGetDevice(&dev);
-    if (dev >= 64 || !(configured & (1ull << dev))) {
-        cudaError_t e = cudaFuncSetAttribute(prefix_kernel<D, CAP, Q8>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             L::kSmemBytes);
-        if (e != cudaSuccess) return e;
-        if (dev < 64) configured |= 1ull << dev;
-    }
-    const int rb = prefix_block_rows(D, a.rows);
+    if (dev < 64 && (configured & (1ull << dev))) return cudaSuccess;
+    cudaError_t e = cudaFuncSetAttribute(prefix_kernel<D, COPIES, Q8>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         PrefixLayout<D>::kSmemBytes);
+    if (e == cudaSuccess && dev < 64) configured |= 1ull << dev;
+    return e;
+}
+
+template <int D, int COPIES, bool Q8>
+cudaError_t launch_prefix_t(const CUtensorMap &tmk, const CUtensorMap &tmv, const CUtensorMap &tmq, const CUtensorMap &tms,
+                            const PrefixArgs &a, int splits, int blocks, cudaStream_t s, bool pdl) {
+    using L = PrefixLayout<D>;
+    cudaError_t e = configure_prefix<D, COPIES, Q8>();
+    if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(splits, a.Hkv, (a.rows + rb - 1) / rb);
+    cfg.gridDim = dim3(splits, a.Hkv, blocks);
     cfg.blockDim = dim3(L::kThreads);
     cfg.dynamicSmemBytes = L::kSmemBytes;
     cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchAttribute attr[2];
+    int n = 0;
+    if (pdl) {
+        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[n++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (a.cluster > 1) {
+        attr[n].id = cudaLaunchAttributeClusterDimension;
+        attr[n].val.clusterDim.x = a.cluster;
+        attr[n].val.clusterDim.y = 1;
+        attr[n++].val.clusterDim.z = 1;
+    }
     cfg.attrs = attr;
-    cfg.numAttrs = pdl ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, prefix_kernel<D, CAP, Q8>, tmk, tmv, a);
+    cfg.numAttrs = n;
+    return cudaLaunchKernelEx(&cfg, prefix_kernel<D, COPIES, Q8>, tmk, tmv, tmq, tms, a);
 }
 
 template <int D>
-cudaError_t launch_prefix_d(const CUtensorMap &tmk, const CUtensorMap &tmv, const PrefixArgs &a, int splits,
-                            cudaStream_t s, bool pdl) {
-    if (a.softcap > 0.f)
-        return a.scales ? launch_prefix_t<D, true, true>(tmk, tmv, a, splits, s, pdl)
-                        : launch_prefix_t<D, true, false>(tmk, tmv, a, splits, s, pdl);
-    return a.scales ? launch_prefix_t<D, false, true>(tmk, tmv, a, splits, s, pdl)
-                    : launch_prefix_t<D, false, false>(tmk, tmv, a, splits, s, pdl);
+cudaError_t launch_prefix_d(const CUtensorMap &tmk, const CUtensorMap &tmv, const CUtensorMap &tmq, const CUtensorMap &tms,
+                            const PrefixArgs &a, const PrefixPlan &p, cudaStream_t s, bool pdl) {
+    const bool q8 = a.scale_row >= 0;
+    switch (p.copies) {
+        case 1:
+            return q8 ? launch_prefix_t<D, 1, true>(tmk, tmv, tmq, tms, a, p.splits, p.blocks, s, pdl)
+                      : launch_prefix_t<D, 1, false>(tmk, tmv, tmq, tms, a, p.splits, p.blocks, s, pdl);
+        case 2:
+            return q8 ? launch_prefix_t<D, 2, true>(tmk, tmv, tmq, tms, a, p.splits, p.blocks, s, pdl)
+                      : launch_prefix_t<D, 2, false>(tmk, tmv, tmq, tms, a, p.splits, p.blocks, s, pdl);
+        default:
+            return q8 ? launch_prefix_t<D, 4, true>(tmk, tmv, tmq, tms, a, p.splits, p.blocks, s, pdl)
+                      : launch_prefix_t<D, 4, false>(tmk, tmv, tmq, tms, a, p.splits, p.blocks, s, pdl);
+    }
+}
+
+// How many clusters of `size` prefix CTAs (one per SM) fit on the device at once.
+template <int D>
+int prefix_clusters(int size, int sms) {
+    static int cache[64][9] = {};  // per device and size; the GPU's partition into GPCs is fixed
+    if (size <= 1) return sms;
+    int dev = 0;
+    cudaGetDevice(&dev);
+    int n = dev < 64 ? cache[dev][size] : 0;
+    if (n == 0) {
+        configure_prefix<D, 1, false>();
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(size, 64, 1);
+        cfg.blockDim = dim3(PrefixLayout<D>::kThreads);
+        cfg.dynamicSmemBytes = PrefixLayout<D>::kSmemBytes;
+        cudaLaunchAttribute attr;
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = size;
+        attr.val.clusterDim.y = 1;
+        attr.val.clusterDim.z = 1;
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        if (cudaOccupancyMaxActiveClusters(&n, prefix_kernel<D, 1, false>, &cfg) != cudaSuccess) {
+            cudaGetLastError();
+            n = 0;
+        }
+        if (n <= 0) n = -1;
+        if (dev < 64) cache[dev][size] = n;
+    }
+    return n > 0 ? n : 0;
+}
+
+// fp16 rows from f32 ones (q), eight elements per thread.
+__global__ void half_rows_kernel(const float *src, __half *dst, long long n8) {
+    griddep_wait();
+    griddep_launch_dependents();
+    const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+    if (i >= n8) return;
+    const float4 x = reinterpret_cast<const float4 *>(src)[2 * i], y = reinterpret_cast<const float4 *>(src)[2 * i + 1];
+    reinterpret_cast<uint4 *>(dst)[i] =
+        make_uint4(pack_half2(x.x, x.y), pack_half2(x.z, x.w), pack_half2(y.x, y.y), pack_half2(y.z, y.w));
 }
 
 // Codes (biased by +128) of rows [row0, row0 + rows) of every kv head as exact fp16 integers
 // [Hkv][rows][D], 16 codes per thread and matrix.
 __global__ void codes_to_half_kernel(const uint8_t *kc, const uint8_t *vc, __half *k, __half *v, int Hkv, int D, int cap,
                                      int row0, int rows) {
+    griddep_wait();  // the codes may come from the kernel before
+    griddep_launch_dependents();
     const int cs = D / 16;
     const long long n = (long long)Hkv * rows * cs;
     for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (long long)gridDim.x * blockDim.x) {
@@ -542,29 +702,78 @@ __global__ void codes_to_half_kernel(const uint8_t *kc, const uint8_t *vc, __hal
 
 int prefix_tile_keys() { return kXK; }
 
-int prefix_block_rows(int head_dim, int rows) {
-    (void)rows;
-    return head_dim == 256 ? kXQ : 2 * kXQ;
+// Rows: as many copies of them as fit the MMA's 128 rows, or blocks of two row tiles.  Splits of the
+// key tiles: clusters of up to eight that are all resident at once.  A split's fixed cost (launch,
+// ramp, join) is worth about six tiles, and every partial costs the merge about one.
+PrefixPlan prefix_plan(int head_dim, int tokens, int group, int kv_heads, int ntiles, int sms) {
+    PrefixPlan p;
+    const int streams = head_dim == 256 ? 1 : 2;
+    p.copies = tokens * group <= (kXQ / 4 / group) * group ? 4 : tokens * group <= (kXQ / 2 / group) * group ? 2 : 1;
+    p.tokens_box = kXQ / p.copies / group;
+    const int per_block = p.tokens_box * (p.copies == 1 ? streams : 1);
+    p.blocks = (tokens + per_block - 1) / per_block;
+    const int units = kv_heads * p.blocks;
+    double best = 1e300;
+    for (int cs = 1; cs <= 8; cs *= 2) {
+        const int clusters = head_dim == 64    ? prefix_clusters<64>(cs, sms)
+                             : head_dim == 128 ? prefix_clusters<128>(cs, sms)
+                                               : prefix_clusters<256>(cs, sms);
+        if (clusters < 1) continue;
+        for (int parts = 1; parts <= 32; ++parts) {
+            const int splits = parts * cs;
+            if (splits > 1 && splits * 2 > ntiles) break;
+            const int tps = (ntiles + splits - 1) / splits;
+            // A cluster may have empty splits (they give -inf), but no part is empty.
+            if ((ntiles + tps - 1) / tps <= splits - cs) continue;
+            const long long waves = ((long long)units * parts + clusters - 1) / clusters;
+            const double cost = (double)waves * (tps + 6) + parts + (cs > 1 ? 1.0 : 0.0);
+            if (cost < best - 1e-9) {
+                best = cost;
+                p.cluster = cs, p.parts = parts, p.splits = splits, p.tiles_per_split = tps;
+            }
+        }
+    }
+    return p;
 }
 
-cudaError_t launch_prefix(int head_dim, const CUtensorMap &tmk, const CUtensorMap &tmv, const PrefixArgs &a, int splits,
-                          cudaStream_t s, bool pdl) {
+cudaError_t launch_prefix(int head_dim, const CUtensorMap &tmk, const CUtensorMap &tmv, const CUtensorMap &tmq,
+                          const CUtensorMap &tms, const PrefixArgs &a, const PrefixPlan &p, cudaStream_t s, bool pdl) {
     switch (head_dim) {
-        case 64: return launch_prefix_d<64>(tmk, tmv, a, splits, s, pdl);
-        case 128: return launch_prefix_d<128>(tmk, tmv, a, splits, s, pdl);
-        case 256: return launch_prefix_d<256>(tmk, tmv, a, splits, s, pdl);
+        case 64: return launch_prefix_d<64>(tmk, tmv, tmq, tms, a, p, s, pdl);
+        case 128: return launch_prefix_d<128>(tmk, tmv, tmq, tms, a, p, s, pdl);
+        case 256: return launch_prefix_d<256>(tmk, tmv, tmq, tms, a, p, s, pdl);
         default: return cudaErrorInvalidValue;
     }
 }
 
+cudaError_t launch_half_rows(const float *src, __half *dst, size_t n, cudaStream_t s, bool pdl) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((n / 8 + 127) / 128));
+    cfg.blockDim = dim3(128);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, half_rows_kernel, src, dst, (long long)(n / 8));
+}
+
 cudaError_t launch_codes_to_half(const uint8_t *kc, const uint8_t *vc, __half *k, __half *v, int n_kv_heads,
-                                 int head_dim, int cap, int row0, int rows, cudaStream_t s) {
+                                 int head_dim, int cap, int row0, int rows, cudaStream_t s, bool pdl) {
     const long long n = (long long)n_kv_heads * rows * (head_dim / 16);
     if (n == 0) return cudaSuccess;
     const long long g = (n + 255) / 256;
-    codes_to_half_kernel<<<(unsigned)(g < 8192 ? g : 8192), 256, 0, s>>>(kc, vc, k, v, n_kv_heads, head_dim, cap, row0,
-                                                                         rows);
-    return cudaGetLastError();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(g < 8192 ? g : 8192));
+    cfg.blockDim = dim3(256);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, codes_to_half_kernel, kc, vc, k, v, n_kv_heads, head_dim, cap, row0, rows);
 }
 
 }  // namespace brk
