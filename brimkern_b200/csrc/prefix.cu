@@ -50,9 +50,9 @@ struct PrefixLayout {
     static constexpr uint32_t kTileBytes = kBlocks * kKVBlock;
     static constexpr uint32_t kOffKV = kStreams * kQBytes;
     static constexpr uint32_t kOffScale = kOffKV + kStages * 2 * kTileBytes;  // int8: [stage][K, V][64] f32
-    static constexpr uint32_t kOffState = kOffScale + kStages * 2 * kXK * 4;  // [m, l][stream][128], [m, l][256] f32
-    static constexpr uint32_t kOffBar = kOffState + 2 * kStreams * kXQ * 4 + 2 * 256 * 4;
-    static constexpr uint32_t kSmemBytes = 1024 + kOffBar + 28 * 8 + 16;
+    static constexpr uint32_t kOffState = kOffScale + kStages * 2 * kXK * 4;  // [m, l][stream][128] f32
+    static constexpr uint32_t kOffBar = kOffState + 2 * kStreams * kXQ * 4;
+    static constexpr uint32_t kSmemBytes = 1024 + kOffBar + 36 * 8 + 16;
     // TMEM columns: S, then P (fp16 pairs), then O from column 256 (one stream of D 256) or 192.
     static constexpr uint32_t kColS = 0, kColP = kStreams * kXK, kColO = kStreams == 1 ? 256 : 192;
     static_assert(kColP + kStreams * kXK / 2 <= kColO && kColO + kStreams * D <= kXTmemCols, "TMEM columns");
@@ -63,15 +63,18 @@ struct PrefixLayout {
 };
 
 enum : int {
-    kXKvFull = 0,    // [6] TMA -> MMA
-    kXKvEmpty = 6,   // [6] MMA commit -> producer
-    kXSFull = 12,    // [2] MMA commit (S ready) -> softmax
-    kXSFree = 14,    // [2] softmax (S read) -> MMA
-    kXPFull = 16,    // [2] softmax (P written, O rescaled) -> MMA
-    kXODone = 18,    // [2] MMA commit (PV done) -> softmax
-    kXQFull = 20,    // TMA (q) -> MMA
-    kXMmaDone = 21,  // [2] everything an issuer issued has completed -> teardown
-    kXStagger = 23,  // stream 0's first P written -> stream 1's issuer starts
+    kXKFull = 0,     // [6] TMA (K) -> MMA
+    kXVFull = 6,     // [6] TMA (V, int8: and the scales) -> MMA, softmax
+    kXKEmpty = 12,   // [6] MMA commit (S done) -> producer
+    kXVEmpty = 18,   // [6] MMA commit (PV done) -> producer
+    kXSFull = 24,    // [2] MMA commit (S ready) -> softmax
+    kXSFree = 26,    // [2] softmax (S read) -> MMA
+    kXPFull = 28,    // [2] softmax (P written, O rescaled) -> MMA
+    kXODone = 30,    // [2] MMA commit (PV done) -> softmax
+    kXQFull = 32,    // TMA (q) -> MMA
+    kXMmaDone = 33,  // [2] everything an issuer issued has completed -> teardown
+    kXStagger = 35,  // stream 0's first P written -> stream 1's issuer starts
+    kXBars = 36,
 };
 
 // 3-D tiled TMA load (CTA-local).
@@ -145,7 +148,7 @@ __global__ void __launch_bounds__(PrefixLayout<D>::kThreads, 1)
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::kOffBar);
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 28);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + kXBars);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int split = blockIdx.x, kvh = blockIdx.y;
@@ -165,8 +168,10 @@ __global__ void __launch_bounds__(PrefixLayout<D>::kThreads, 1)
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < L::kStages; ++i) {
-            mbar_init(&bars[kXKvFull + i], 1);
-            mbar_init(&bars[kXKvEmpty + i], pair ? 2 : 1);  // one commit per stream that reads the tile
+            mbar_init(&bars[kXKFull + i], 1);
+            mbar_init(&bars[kXVFull + i], 1);
+            mbar_init(&bars[kXKEmpty + i], pair ? 2 : 1);  // one commit per stream that reads the tile
+            mbar_init(&bars[kXVEmpty + i], pair ? 2 : 1);
         }
         for (int s = 0; s < NS; ++s) {
             mbar_init(&bars[kXSFull + s], 1);
@@ -214,25 +219,31 @@ __global__ void __launch_bounds__(PrefixLayout<D>::kThreads, 1)
                 for (int blk = 0; blk < L::kBlocks; ++blk)
                     tma_load_q(smem + (pair ? t * L::kQBytes : t * RC * 128) + blk * L::kQBlock, &tmq, blk * 64, kvh * a.G,
                                bt0 + (pair ? t * nbt : 0), &bars[kXQFull]);
+            // A K slot is free again after the tile's scores, a V slot after its product: K runs ahead.
             int issued = 0;
-            for (int j = 0; j < nk; ++j) {
+            bool ok = true;
+            for (int j = 0; ok && j < nk; ++j) {
                 const int st = j % L::kStages;
-                if (j >= L::kStages && !mbar_wait(&bars[kXKvEmpty + st], ((j / L::kStages) - 1) & 1, a.err, kErrSlotTimeout))
-                    break;
                 const int key = kb + j * kXK, y = seg_row + key;
-                mbar_arrive_expect_tx(&bars[kXKvFull + st], 2 * L::kTileBytes + (Q8 ? 2 * kXK * 4 : 0));
+                const uint32_t phase = ((j / L::kStages) - 1) & 1;
+                if (j >= L::kStages && !mbar_wait(&bars[kXKEmpty + st], phase, a.err, kErrSlotTimeout)) break;
+                mbar_arrive_expect_tx(&bars[kXKFull + st], L::kTileBytes);
 #pragma unroll
                 for (int blk = 0; blk < L::kBlocks; ++blk)
-                    tma_load_2d(sK(st) + blk * L::kKVBlock, &tmk, blk * 64, y, &bars[kXKvFull + st]);
+                    tma_load_2d(sK(st) + blk * L::kKVBlock, &tmk, blk * 64, y, &bars[kXKFull + st]);
+                if (j >= L::kStages && !mbar_wait(&bars[kXVEmpty + st], phase, a.err, kErrSlotTimeout)) ok = false;
+                mbar_arrive_expect_tx(&bars[kXVFull + st], L::kTileBytes + (Q8 ? 2 * kXK * 4 : 0));
 #pragma unroll
                 for (int blk = 0; blk < L::kBlocks; ++blk)
-                    tma_load_2d(sV(st) + blk * L::kKVBlock, &tmv, blk * 64, y, &bars[kXKvFull + st]);
-                if constexpr (Q8) tma_load_2d(sScale + st * 2 * kXK, &tms, key, a.scale_row + kvh * 2, &bars[kXKvFull + st]);
+                    tma_load_2d(sV(st) + blk * L::kKVBlock, &tmv, blk * 64, y, &bars[kXVFull + st]);
+                if constexpr (Q8) tma_load_2d(sScale + st * 2 * kXK, &tms, key, a.scale_row + kvh * 2, &bars[kXVFull + st]);
                 issued = j + 1;
             }
             mbar_wait(&bars[kXQFull], 0, a.err, kErrTmaTimeout);
-            for (int j = issued > L::kStages ? issued - L::kStages : 0; j < issued; ++j)
-                mbar_wait(&bars[kXKvFull + j % L::kStages], (j / L::kStages) & 1, a.err, kErrTmaTimeout);
+            for (int j = issued > L::kStages ? issued - L::kStages : 0; j < issued; ++j) {
+                mbar_wait(&bars[kXKFull + j % L::kStages], (j / L::kStages) & 1, a.err, kErrTmaTimeout);
+                mbar_wait(&bars[kXVFull + j % L::kStages], (j / L::kStages) & 1, a.err, kErrTmaTimeout);
+            }
         }
         __syncwarp();
     } else if (warp >= L::kMma) {
@@ -247,7 +258,7 @@ __global__ void __launch_bounds__(PrefixLayout<D>::kThreads, 1)
             bool ok = mbar_wait(&bars[kXQFull], 0, a.err, kErrMmaTimeout);
             auto issue_s = [&](int i) -> bool {
                 const int j = j0 + i * step, st = j % L::kStages;
-                if (!mbar_wait(&bars[kXKvFull + st], (j / L::kStages) & 1, a.err, kErrTmaTimeout)) return false;
+                if (!mbar_wait(&bars[kXKFull + st], (j / L::kStages) & 1, a.err, kErrTmaTimeout)) return false;
                 if (i >= 1 && !mbar_wait(&bars[kXSFree + s], (i - 1) & 1, a.err, kErrMmaTimeout)) return false;
                 tc_fence_after();
                 const uint32_t q_base = smem_addr(sQ(s)), k_base = smem_addr(sK(st));
@@ -257,11 +268,13 @@ __global__ void __launch_bounds__(PrefixLayout<D>::kThreads, 1)
                            sw128_desc(q_base + (ks >> 2) * L::kQBlock + (ks & 3) * 32, 16, 1024),
                            sw128_desc(k_base + (ks >> 2) * L::kKVBlock + (ks & 3) * 32, 16, 1024), idesc_qk, ks > 0);
                 tc_commit(&bars[kXSFull + s]);
+                tc_commit(&bars[kXKEmpty + st]);
                 return true;
             };
             auto issue_pv = [&](int i) -> bool {
                 const int j = j0 + i * step, st = j % L::kStages;
                 if (!mbar_wait(&bars[kXPFull + s], i & 1, a.err, kErrMmaTimeout)) return false;
+                if (!mbar_wait(&bars[kXVFull + st], (j / L::kStages) & 1, a.err, kErrTmaTimeout)) return false;
                 if (pair && s == 1 && tail && j == nk - 1 && !mbar_wait(&bars[kXPFull], i & 1, a.err, kErrMmaTimeout))
                     return false;
                 tc_fence_after();
@@ -271,6 +284,7 @@ __global__ void __launch_bounds__(PrefixLayout<D>::kThreads, 1)
                     tc_mma_ts(tmem + L::kColO + s * D, tmem + L::kColP + s * (kXK / 2) + kk * 8,
                               sw128_desc(v_base + kk * 16 * 128, L::kKVBlock, 1024), idesc_pv, i > 0 || kk > 0);
                 tc_commit(&bars[kXODone + s]);
+                tc_commit(&bars[kXVEmpty + st]);
                 return true;
             };
             if (ok && s == 1) ok = mbar_wait(&bars[kXStagger], 0, a.err, kErrMmaTimeout);
@@ -279,7 +293,6 @@ __global__ void __launch_bounds__(PrefixLayout<D>::kThreads, 1)
                 // S of the next tile needs only that this one's was read: it runs under the softmax.
                 if (i + 1 < cnt && !issue_s(i + 1)) break;
                 if (!issue_pv(i)) break;
-                tc_commit(&bars[kXKvEmpty + (j0 + i * step) % L::kStages]);
             }
             tc_commit(&bars[kXMmaDone + s]);
             mbar_wait(&bars[kXMmaDone + s], 0, a.err, kErrMmaTimeout);
@@ -339,6 +352,11 @@ __global__ void __launch_bounds__(PrefixLayout<D>::kThreads, 1)
                 }
                 const float *ksc = sScale + st * 2 * kXK + copy * KC, *vsc = ksc + kXK;
                 if constexpr (Q8) {
+                    const bool there = mbar_wait(&bars[kXVFull + st], (j / L::kStages) & 1, a.err, kErrTmaTimeout);
+                    if (!__all_sync(0xffffffffu, there)) {
+                        ok = false;
+                        break;
+                    }
 #pragma unroll
                     for (int e = 0; e < KC; e += 4) {
                         const float4 k4 = *reinterpret_cast<const float4 *>(ksc + e);
@@ -408,10 +426,11 @@ __global__ void __launch_bounds__(PrefixLayout<D>::kThreads, 1)
 #pragma unroll
                     for (int e = 0; e < KC; e += 4) {
                         const float4 s4 = *reinterpret_cast<const float4 *>(vsc + e);
-                        const float sv[4] = {s4.x, s4.y, s4.z, s4.w};
+                        v[e] *= s4.x, v[e + 1] *= s4.y, v[e + 2] *= s4.z, v[e + 3] *= s4.w;
+                    }
+                    if (edge) {
 #pragma unroll
-                        for (int h = 0; h < 4; ++h)
-                            v[e + h] = edge && (kbase + e + h < lo || kbase + e + h >= ke) ? 0.f : v[e + h] * sv[h];
+                        for (int e = 0; e < KC; ++e) v[e] = kbase + e >= lo && kbase + e < ke ? v[e] : 0.f;
                     }
                 }
 #pragma unroll
@@ -428,7 +447,7 @@ __global__ void __launch_bounds__(PrefixLayout<D>::kThreads, 1)
             // Keys past the range end: zero V rows, so that 0 * (whatever the tile holds) stays 0.
             if ((s == 0 || !pair) && tail) {
                 const int key = kb + j * kXK + r;
-                if (!__all_sync(0xffffffffu, mbar_wait(&bars[kXKvFull + st], (j / L::kStages) & 1, a.err, kErrTmaTimeout))) {
+                if (!__all_sync(0xffffffffu, mbar_wait(&bars[kXVFull + st], (j / L::kStages) & 1, a.err, kErrTmaTimeout))) {
                     ok = false;
                     break;
                 }
@@ -460,7 +479,6 @@ __global__ void __launch_bounds__(PrefixLayout<D>::kThreads, 1)
         float *jo = reinterpret_cast<float *>(smem);                 // [stream][128][kJoin]
         float *jm = reinterpret_cast<float *>(smem + L::kOffState);  // [stream][128] m, then l
         float *jl = jm + NS * kXQ;
-        float *rm = jl + NS * kXQ, *rl = rm + 256;                   // the CTA's rows: m, l
         named_barrier_sync(1, NT);
         jm[s * kXQ + r] = m_used;
         jl[s * kXQ + r] = l_run;
@@ -476,81 +494,104 @@ __global__ void __launch_bounds__(PrefixLayout<D>::kThreads, 1)
             }
         }
         named_barrier_sync(1, NT);
-        // The CTA's rows: x over (token, head), a thread per four elements.  Sources: the copies of
-        // every stream that took tiles (pair: the row's own stream).
+        // Rows by (half-)warps, lanes over the row's float4s.  Row x of the block: stream sx (pair), MMA
+        // row rx of its first copy.
+        constexpr int D4 = D / 4, LPR = D4 < 32 ? D4 : 32, RPW = 32 / LPR, VPL = D4 / LPR;
         const int n_rows = n_bt * a.G, rt = nbt * a.G;
-        constexpr int D4 = D / 4;
+        const int sub = lane / LPR, l4 = lane % LPR;
         const size_t rows_total = (size_t)bt_total * a.Hq;
-        const bool in_cluster = a.cluster > 1;
-        const int part = split / a.cluster;
+        const int cs = a.cluster, me = split % cs;
+        const int part = split / cs;
         float *out_o = a.part_o + (size_t)part * rows_total * D, *out_ml = a.part_ml + (size_t)part * rows_total * 2;
-        for (int e = threadIdx.x; e < n_rows * D4; e += NT) {
-            const int x = e / D4, d4 = e % D4;
-            const int sx = pair ? x / rt : 0, rx = pair ? x % rt : x;
-            constexpr int MOST = NS * COPIES;
-            float m[MOST], M = -CUDART_INF_F;
+        auto global_row = [&](int x) { return (size_t)(bt0 + x / a.G) * a.Hq + kvh * a.G + x % a.G; };
+        if (!pair) {
+            // The copies of every stream that took tiles, joined in place of the first (only this warp
+            // looks at the row), or straight to the output.
+            for (int x = warp * RPW + sub; __any_sync(0xffffffffu, x < n_rows); x += L::kSoftWarps * RPW) {
+                const bool valid = x < n_rows;
+                constexpr int MOST = NS * COPIES;
+                float m[MOST], f[MOST], M = -CUDART_INF_F, l = 0.f;
 #pragma unroll
-            for (int q = 0; q < MOST; ++q) {
-                const int sq = COPIES == 1 ? (pair ? sx : q) : q / COPIES;
-                const bool there = !(pair && q > 0) && tile_count(sq) > 0;
-                m[q] = there ? jm[sq * kXQ + (q % COPIES) * RC + rx] : -CUDART_INF_F;
-                M = fmaxf(M, m[q]);
-            }
-            float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-            float l = 0.f;
+                for (int q = 0; q < MOST; ++q) {
+                    m[q] = valid && tile_count(q / COPIES) > 0 ? jm[(q / COPIES) * kXQ + (q % COPIES) * RC + x] : -CUDART_INF_F;
+                    M = fmaxf(M, m[q]);
+                }
 #pragma unroll
-            for (int q = 0; q < MOST; ++q) {
-                if (m[q] != -CUDART_INF_F) {
-                    const int sq = COPIES == 1 ? (pair ? sx : q) : q / COPIES;
-                    const int at = sq * kXQ + (q % COPIES) * RC + rx;
-                    const float f = ex2_fast(m[q] - M);
-                    const float4 y = *reinterpret_cast<const float4 *>(jo + (size_t)at * L::kJoin + 4 * d4);
-                    O.x = fmaf(f, y.x, O.x), O.y = fmaf(f, y.y, O.y), O.z = fmaf(f, y.z, O.z), O.w = fmaf(f, y.w, O.w);
-                    l = fmaf(f, jl[at], l);
+                for (int q = 0; q < MOST; ++q) {
+                    f[q] = m[q] == -CUDART_INF_F ? 0.f : ex2_fast(m[q] - M);
+                    if (f[q] != 0.f) l = fmaf(f[q], jl[(q / COPIES) * kXQ + (q % COPIES) * RC + x], l);
+                }
+                float4 O[VPL];
+#pragma unroll
+                for (int v = 0; v < VPL; ++v) {
+                    O[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                    for (int q = 0; q < MOST; ++q)
+                        if (m[q] != -CUDART_INF_F) {
+                            const float4 y = *reinterpret_cast<const float4 *>(
+                                jo + (size_t)((q / COPIES) * kXQ + (q % COPIES) * RC + x) * L::kJoin + 4 * (l4 + v * LPR));
+                            O[v].x = fmaf(f[q], y.x, O[v].x), O[v].y = fmaf(f[q], y.y, O[v].y);
+                            O[v].z = fmaf(f[q], y.z, O[v].z), O[v].w = fmaf(f[q], y.w, O[v].w);
+                        }
+                }
+                __syncwarp();
+                if (valid && cs > 1) {
+#pragma unroll
+                    for (int v = 0; v < VPL; ++v)
+                        *reinterpret_cast<float4 *>(jo + (size_t)x * L::kJoin + 4 * (l4 + v * LPR)) = O[v];
+                    if (l4 == 0) jm[x] = M, jl[x] = l;
+                } else if (valid) {
+                    const size_t R = global_row(x);
+#pragma unroll
+                    for (int v = 0; v < VPL; ++v)
+                        *reinterpret_cast<float4 *>(out_o + R * D + 4 * (l4 + v * LPR)) = O[v];
+                    if (l4 == 0)
+                        *reinterpret_cast<float2 *>(out_ml + R * 2) = make_float2(M == -CUDART_INF_F ? M : M * kXLn2, l);
                 }
             }
-            if (in_cluster) {
-                // In place of the row's first source: only this thread reads these four elements.
-                *reinterpret_cast<float4 *>(jo + (size_t)(sx * kXQ + rx) * L::kJoin + 4 * d4) = O;
-                if (d4 == 0) rm[x] = M, rl[x] = l;
-            } else {
-                const size_t R = (size_t)(bt0 + x / a.G) * a.Hq + kvh * a.G + x % a.G;
-                *reinterpret_cast<float4 *>(out_o + R * D + 4 * d4) = O;
-                if (d4 == 0)
-                    *reinterpret_cast<float2 *>(out_ml + R * 2) = make_float2(M == -CUDART_INF_F ? M : M * kXLn2, l);
-            }
         }
-        if (in_cluster) {
-            cluster_sync_all();  // every split's rows are in its CTA's shared memory
-            const int cs = a.cluster, me = split % cs;
-            const int total = n_rows * D4, share = (total + cs - 1) / cs;
-            for (int e = me * share + threadIdx.x; e < min(total, (me + 1) * share); e += NT) {
-                const int x = e / D4, d4 = e % D4;
-                const int sx = pair ? x / rt : 0, rx = pair ? x % rt : x;
-                const float *src = jo + (size_t)(sx * kXQ + rx) * L::kJoin + 4 * d4;
+        if (cs > 1) cluster_sync_all();  // every split's rows are in its CTA's shared memory
+        if (cs > 1 || pair) {
+            // Rows dealt over the cluster's CTAs; a row's splits read at once.
+            for (int x = me + cs * (warp * RPW + sub); x < n_rows; x += cs * L::kSoftWarps * RPW) {
+                const int at = pair && x >= rt ? kXQ + x - rt : x;
                 float m[8], lq[8], M = -CUDART_INF_F;
-                float4 y[8];
+                float4 y[VPL][8];
 #pragma unroll
                 for (int q = 0; q < 8; ++q) {
                     const bool there = q < cs;
-                    m[q] = there ? ld_cluster_f32(rm + x, q) : -CUDART_INF_F;
-                    lq[q] = there ? ld_cluster_f32(rl + x, q) : 0.f;
-                    y[q] = there ? ld_cluster_v4(src, q) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    m[q] = there ? (cs > 1 ? ld_cluster_f32(jm + at, q) : jm[at]) : -CUDART_INF_F;
+                    lq[q] = there ? (cs > 1 ? ld_cluster_f32(jl + at, q) : jl[at]) : 0.f;
+#pragma unroll
+                    for (int v = 0; v < VPL; ++v) {
+                        const float *src = jo + (size_t)at * L::kJoin + 4 * (l4 + v * LPR);
+                        y[v][q] = !there   ? make_float4(0.f, 0.f, 0.f, 0.f)
+                                  : cs > 1 ? ld_cluster_v4(src, q)
+                                           : *reinterpret_cast<const float4 *>(src);
+                    }
                 }
 #pragma unroll
                 for (int q = 0; q < 8; ++q) M = fmaxf(M, m[q]);
-                float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+                float4 O[VPL];
+#pragma unroll
+                for (int v = 0; v < VPL; ++v) O[v] = make_float4(0.f, 0.f, 0.f, 0.f);
                 float l = 0.f;
 #pragma unroll
                 for (int q = 0; q < 8; ++q) {
-                    const float f = m[q] == -CUDART_INF_F ? 0.f : ex2_fast(m[q] - M);
-                    O.x = fmaf(f, y[q].x, O.x), O.y = fmaf(f, y[q].y, O.y), O.z = fmaf(f, y[q].z, O.z),
-                    O.w = fmaf(f, y[q].w, O.w);
-                    l = fmaf(f, lq[q], l);
+                    if (m[q] != -CUDART_INF_F) {
+                        const float f = ex2_fast(m[q] - M);
+                        l = fmaf(f, lq[q], l);
+#pragma unroll
+                        for (int v = 0; v < VPL; ++v) {
+                            O[v].x = fmaf(f, y[v][q].x, O[v].x), O[v].y = fmaf(f, y[v][q].y, O[v].y);
+                            O[v].z = fmaf(f, y[v][q].z, O[v].z), O[v].w = fmaf(f, y[v][q].w, O[v].w);
+                        }
+                    }
                 }
-                const size_t R = (size_t)(bt0 + x / a.G) * a.Hq + kvh * a.G + x % a.G;
-                *reinterpret_cast<float4 *>(out_o + R * D + 4 * d4) = O;
-                if (d4 == 0)
+                const size_t R = global_row(x);
+#pragma unroll
+                for (int v = 0; v < VPL; ++v) *reinterpret_cast<float4 *>(out_o + R * D + 4 * (l4 + v * LPR)) = O[v];
+                if (l4 == 0)
                     *reinterpret_cast<float2 *>(out_ml + R * 2) = make_float2(M == -CUDART_INF_F ? M : M * kXLn2, l);
             }
         }
