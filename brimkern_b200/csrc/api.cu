@@ -1484,23 +1484,29 @@ int run_decode_prefix(brk_ctx *ctx, const brk_kv *prefix, int prefix_seq, int pr
     }
     const int keys = prefix_len - k_begin;
     brk::PrefixPlan plan;
-    plan.parts = 0;
+    plan.splits = 0;
     if (keys > 0)
         plan = brk::prefix_plan(D, batch * n_tokens, G, Hkv, (keys + brk::prefix_tile_keys() - 1) / brk::prefix_tile_keys(),
                                 ctx->num_sms);
-    const int parts = plan.parts;
+    const int parts = plan.splits;
     int nsplit = 1, kps = 0;
     int rc = decode_split_plan(ctx, kv, p, batch, n_tokens, past_len, false, &nsplit, &kps);
     if (rc) return rc;
-    if (nsplit > 32) {  // the merge takes in at most 32 of these and 32 of the prefix's partials
-        const int tk = brk::decode_stage_keys(D);
-        const int span = nsplit * kps;
-        kps = ((span + 31) / 32 + tk - 1) / tk * tk;
-        nsplit = (span + kps - 1) / kps;
-    }
     const int rt = brk::decode_rows_per_tile();
     const int mtiles = (n_tokens * G + rt - 1) / rt;
     const int units = batch * Hkv * mtiles;
+    // The own rows' merge takes in at most 32 of their splits (and 32 of the prefix's), and splits
+    // them no further than one CTA per SM: the split ranges' join through memory costs more than it
+    // gives here (16 sequences x 2 tokens of up to 777 int8 rows behind 4099: 40.7 us with 3 splits,
+    // 29.2 with 1; 8 sequences of 5000 rows and 8 kv heads still split).
+    if (!getenv("BRK_DECODE_SPLITS") || nsplit > 32) {
+        const int most = getenv("BRK_DECODE_SPLITS") ? 32 : std::max(1, std::min(32, ctx->num_sms / units));
+        if (nsplit > most) {
+            const int tk = brk::decode_stage_keys(D), span = nsplit * kps;
+            kps = ((span + most - 1) / most + tk - 1) / tk * tk;
+            nsplit = (span + kps - 1) / kps;
+        }
+    }
 
     const size_t n_ml = rows * 2 * sizeof(float), n_o = rows * D * sizeof(float);
     const size_t staged = keys > 0 && prefix->q8() ? (size_t)Hkv * keys * D * sizeof(__half) : 0;
@@ -1537,7 +1543,6 @@ int run_decode_prefix(brk_ctx *ctx, const brk_kv *prefix, int prefix_seq, int pr
         x.B = batch, x.T = n_tokens, x.Hq = p->n_heads, x.Hkv = Hkv, x.G = G;
         x.k_begin = k_begin, x.k_end = prefix_len;
         x.tiles_per_split = plan.tiles_per_split;
-        x.cluster = plan.cluster;
         x.window = window;
         x.scale_log2 = scale * (float)log2e;
         x.softcap = softcap, x.cap_k1 = cap_k1, x.cap_k2 = cap_k2;

@@ -180,25 +180,25 @@ struct DecodeArgs {
 
 // Attention of every sequence's query rows over one shared prefix (prefix.cu): partials only.
 struct PrefixArgs {
-    float *part_ml;       // [part][B*T*Hq][2] (m natural-log units, l)
-    float *part_o;        // [part][B*T*Hq][D] unnormalised
+    float *part_ml;       // [split][B*T*Hq][2] (m natural-log units, l)
+    float *part_o;        // [split][B*T*Hq][D] unnormalised
     int scale_row;        // int8 cache: the scale map's row of kv head 0 ([kv head][K, V]); -1: fp16
     int *err;
     int B, T, Hq, Hkv, G;
     int row0;             // map row of key 0 of kv head 0
     int head_rows;        // map rows from one kv head to the next
     int k_begin, k_end;   // keys some row attends
-    int tiles_per_split, cluster;
+    int tiles_per_split;
     int window;
     float scale_log2, softcap, cap_k1, cap_k2;
     int past_len[BRK_MAX_BATCH];
 };
 
 // How the prefix's work is cut: copies of the query rows in the MMA's rows, tokens per q box, row
-// blocks, key splits (`cluster` of them joined in a cluster), partials.
+// blocks, key splits.
 struct PrefixPlan {
     int copies = 1, tokens_box = 1, blocks = 1;
-    int splits = 1, cluster = 1, parts = 1, tiles_per_split = 1;
+    int splits = 1, tiles_per_split = 1;
 };
 
 struct PrefillArgs {

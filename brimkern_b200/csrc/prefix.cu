@@ -15,9 +15,10 @@
 // takes its own 32 or 16 keys of a tile and leaves P = 0 for the others, so that all threads share the
 // exponentials instead of one warp doing them: what bounds the loop is then the K/V stream.
 //
-// The end: streams and copies are joined in shared memory, the splits of a cluster through distributed
-// shared memory, and one partial per cluster leaves in coalesced rows -- the partials are f32 and
-// would otherwise be as many bytes as the prefix itself.
+// The end: streams and copies are joined in shared memory and the split's partial leaves in coalesced
+// rows; the merge of the own rows' kernel takes in the splits.  (Joining the splits of a cluster
+// through distributed shared memory first, for an eighth of the partials: 131 KB a CTA took 5 us
+// there, and the merge was no faster with 2 partials than with 16.)
 //
 // int8 prefix: the codes, as exact fp16 integers, are the operands; the K scale multiplies the
 // scores and the V scale the probabilities, so nothing is rounded that the fp16 form does not round.
@@ -85,17 +86,6 @@ __device__ __forceinline__ void tma_load_q(void *dst, const CUtensorMap *map, in
         "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_addr(bar))
         : "memory");
 }
-__device__ __forceinline__ float4 ld_cluster_v4(const float *p, uint32_t rank) {
-    uint32_t at;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_addr(p)), "r"(rank));
-    float4 v;
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-                 : "r"(at)
-                 : "memory");
-    return v;
-}
-
 // KC consecutive S columns of this thread's lane (no wait), and KC / 2 P columns.
 template <int KC>
 __device__ __forceinline__ void ld_scores(uint32_t taddr, uint32_t (&v)[KC]) {
@@ -494,54 +484,45 @@ __global__ void __launch_bounds__(PrefixLayout<D>::kThreads, 1)
             }
         }
         named_barrier_sync(1, NT);
-        // Rows by (half-)warps, lanes over the row's float4s.  Row x of the block: stream sx (pair), MMA
-        // row rx of its first copy.
+        // Rows by (half-)warps, lanes over the row's float4s, UR rows at a time.  The sources of a row:
+        // the copies of every stream that took tiles, or (pair) its own stream.
         constexpr int D4 = D / 4, LPR = D4 < 32 ? D4 : 32, RPW = 32 / LPR, VPL = D4 / LPR;
+        constexpr int UR = COPIES == 1 ? 4 : COPIES == 2 ? 2 : 1, MOST = NS * COPIES;
         const int n_rows = n_bt * a.G, rt = nbt * a.G;
         const int sub = lane / LPR, l4 = lane % LPR;
         const size_t rows_total = (size_t)bt_total * a.Hq;
-        const int cs = a.cluster, me = split % cs;
-        const int part = split / cs;
-        float *out_o = a.part_o + (size_t)part * rows_total * D, *out_ml = a.part_ml + (size_t)part * rows_total * 2;
-        auto global_row = [&](int x) { return (size_t)(bt0 + x / a.G) * a.Hq + kvh * a.G + x % a.G; };
-        if (!pair) {
-            // The copies of every stream that took tiles, joined in place of the first (only this warp
-            // looks at the row), or straight to the output.
-            for (int x = warp * RPW + sub; __any_sync(0xffffffffu, x < n_rows); x += L::kSoftWarps * RPW) {
-                const bool valid = x < n_rows;
-                constexpr int MOST = NS * COPIES;
-                float m[MOST], f[MOST], M = -CUDART_INF_F, l = 0.f;
+        float *out_o = a.part_o + (size_t)split * rows_total * D, *out_ml = a.part_ml + (size_t)split * rows_total * 2;
+        for (int x0 = (warp * RPW + sub) * UR; x0 < n_rows; x0 += L::kSoftWarps * RPW * UR) {
+#pragma unroll
+            for (int u = 0; u < UR; ++u) {
+                const int x = min(x0 + u, n_rows - 1);
+                // The row's first MMA row in shared memory, and how many sources it has.
+                const int at = pair && x >= rt ? kXQ + x - rt : x;
+                float m[MOST], M = -CUDART_INF_F, l = 0.f;
 #pragma unroll
                 for (int q = 0; q < MOST; ++q) {
-                    m[q] = valid && tile_count(q / COPIES) > 0 ? jm[(q / COPIES) * kXQ + (q % COPIES) * RC + x] : -CUDART_INF_F;
+                    const bool there = pair ? q == 0 : tile_count(q / COPIES) > 0;
+                    m[q] = there ? jm[at + (q / COPIES) * kXQ + (q % COPIES) * RC] : -CUDART_INF_F;
                     M = fmaxf(M, m[q]);
-                }
-#pragma unroll
-                for (int q = 0; q < MOST; ++q) {
-                    f[q] = m[q] == -CUDART_INF_F ? 0.f : ex2_fast(m[q] - M);
-                    if (f[q] != 0.f) l = fmaf(f[q], jl[(q / COPIES) * kXQ + (q % COPIES) * RC + x], l);
                 }
                 float4 O[VPL];
 #pragma unroll
-                for (int v = 0; v < VPL; ++v) {
-                    O[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+                for (int v = 0; v < VPL; ++v) O[v] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-                    for (int q = 0; q < MOST; ++q)
-                        if (m[q] != -CUDART_INF_F) {
-                            const float4 y = *reinterpret_cast<const float4 *>(
-                                jo + (size_t)((q / COPIES) * kXQ + (q % COPIES) * RC + x) * L::kJoin + 4 * (l4 + v * LPR));
-                            O[v].x = fmaf(f[q], y.x, O[v].x), O[v].y = fmaf(f[q], y.y, O[v].y);
-                            O[v].z = fmaf(f[q], y.z, O[v].z), O[v].w = fmaf(f[q], y.w, O[v].w);
+                for (int q = 0; q < MOST; ++q)
+                    if (m[q] != -CUDART_INF_F) {
+                        const int src = at + (q / COPIES) * kXQ + (q % COPIES) * RC;
+                        const float f = ex2_fast(m[q] - M);
+                        l = fmaf(f, jl[src], l);
+#pragma unroll
+                        for (int v = 0; v < VPL; ++v) {
+                            const float4 y = *reinterpret_cast<const float4 *>(jo + (size_t)src * L::kJoin + 4 * (l4 + v * LPR));
+                            O[v].x = fmaf(f, y.x, O[v].x), O[v].y = fmaf(f, y.y, O[v].y);
+                            O[v].z = fmaf(f, y.z, O[v].z), O[v].w = fmaf(f, y.w, O[v].w);
                         }
-                }
-                __syncwarp();
-                if (valid && cs > 1) {
-#pragma unroll
-                    for (int v = 0; v < VPL; ++v)
-                        *reinterpret_cast<float4 *>(jo + (size_t)x * L::kJoin + 4 * (l4 + v * LPR)) = O[v];
-                    if (l4 == 0) jm[x] = M, jl[x] = l;
-                } else if (valid) {
-                    const size_t R = global_row(x);
+                    }
+                if (x0 + u < n_rows) {
+                    const size_t R = (size_t)(bt0 + x / a.G) * a.Hq + kvh * a.G + x % a.G;
 #pragma unroll
                     for (int v = 0; v < VPL; ++v)
                         *reinterpret_cast<float4 *>(out_o + R * D + 4 * (l4 + v * LPR)) = O[v];
@@ -550,57 +531,8 @@ __global__ void __launch_bounds__(PrefixLayout<D>::kThreads, 1)
                 }
             }
         }
-        if (cs > 1) cluster_sync_all();  // every split's rows are in its CTA's shared memory
-        if (cs > 1 || pair) {
-            // Rows dealt over the cluster's CTAs; a row's splits read at once.
-            for (int x = me + cs * (warp * RPW + sub); x < n_rows; x += cs * L::kSoftWarps * RPW) {
-                const int at = pair && x >= rt ? kXQ + x - rt : x;
-                float m[8], lq[8], M = -CUDART_INF_F;
-                float4 y[VPL][8];
-#pragma unroll
-                for (int q = 0; q < 8; ++q) {
-                    const bool there = q < cs;
-                    m[q] = there ? (cs > 1 ? ld_cluster_f32(jm + at, q) : jm[at]) : -CUDART_INF_F;
-                    lq[q] = there ? (cs > 1 ? ld_cluster_f32(jl + at, q) : jl[at]) : 0.f;
-#pragma unroll
-                    for (int v = 0; v < VPL; ++v) {
-                        const float *src = jo + (size_t)at * L::kJoin + 4 * (l4 + v * LPR);
-                        y[v][q] = !there   ? make_float4(0.f, 0.f, 0.f, 0.f)
-                                  : cs > 1 ? ld_cluster_v4(src, q)
-                                           : *reinterpret_cast<const float4 *>(src);
-                    }
-                }
-#pragma unroll
-                for (int q = 0; q < 8; ++q) M = fmaxf(M, m[q]);
-                float4 O[VPL];
-#pragma unroll
-                for (int v = 0; v < VPL; ++v) O[v] = make_float4(0.f, 0.f, 0.f, 0.f);
-                float l = 0.f;
-#pragma unroll
-                for (int q = 0; q < 8; ++q) {
-                    if (m[q] != -CUDART_INF_F) {
-                        const float f = ex2_fast(m[q] - M);
-                        l = fmaf(f, lq[q], l);
-#pragma unroll
-                        for (int v = 0; v < VPL; ++v) {
-                            O[v].x = fmaf(f, y[v][q].x, O[v].x), O[v].y = fmaf(f, y[v][q].y, O[v].y);
-                            O[v].z = fmaf(f, y[v][q].z, O[v].z), O[v].w = fmaf(f, y[v][q].w, O[v].w);
-                        }
-                    }
-                }
-                const size_t R = global_row(x);
-#pragma unroll
-                for (int v = 0; v < VPL; ++v) *reinterpret_cast<float4 *>(out_o + R * D + 4 * (l4 + v * LPR)) = O[v];
-                if (l4 == 0)
-                    *reinterpret_cast<float2 *>(out_ml + R * 2) = make_float2(M == -CUDART_INF_F ? M : M * kXLn2, l);
-            }
-        }
     }
     // Teardown: every TMEM access and MMA is complete; the allocating warp releases TMEM.
-    if (a.cluster > 1) {
-        if (warp >= L::kProducer) cluster_sync_all();  // the softmax warps' first barrier counts every thread
-        cluster_sync_all();                            // no CTA leaves while another may still read its rows
-    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -609,42 +541,28 @@ __global__ void __launch_bounds__(PrefixLayout<D>::kThreads, 1)
 }
 
 template <int D, int COPIES, bool Q8>
-cudaError_t configure_prefix() {
-    static unsigned long long configured = 0;  // one bit per device: the opt-in is per device
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (dev < 64 && (configured & (1ull << dev))) return cudaSuccess;
-    cudaError_t e = cudaFuncSetAttribute(prefix_kernel<D, COPIES, Q8>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         PrefixLayout<D>::kSmemBytes);
-    if (e == cudaSuccess && dev < 64) configured |= 1ull << dev;
-    return e;
-}
-
-template <int D, int COPIES, bool Q8>
 cudaError_t launch_prefix_t(const CUtensorMap &tmk, const CUtensorMap &tmv, const CUtensorMap &tmq, const CUtensorMap &tms,
                             const PrefixArgs &a, int splits, int blocks, cudaStream_t s, bool pdl) {
     using L = PrefixLayout<D>;
-    cudaError_t e = configure_prefix<D, COPIES, Q8>();
-    if (e != cudaSuccess) return e;
+    static unsigned long long configured = 0;  // one bit per device: the opt-in is per device
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev >= 64 || !(configured & (1ull << dev))) {
+        cudaError_t e = cudaFuncSetAttribute(prefix_kernel<D, COPIES, Q8>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             L::kSmemBytes);
+        if (e != cudaSuccess) return e;
+        if (dev < 64) configured |= 1ull << dev;
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(splits, a.Hkv, blocks);
     cfg.blockDim = dim3(L::kThreads);
     cfg.dynamicSmemBytes = L::kSmemBytes;
     cfg.stream = s;
-    cudaLaunchAttribute attr[2];
-    int n = 0;
-    if (pdl) {
-        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[n++].val.programmaticStreamSerializationAllowed = 1;
-    }
-    if (a.cluster > 1) {
-        attr[n].id = cudaLaunchAttributeClusterDimension;
-        attr[n].val.clusterDim.x = a.cluster;
-        attr[n].val.clusterDim.y = 1;
-        attr[n++].val.clusterDim.z = 1;
-    }
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = n;
+    cfg.numAttrs = pdl ? 1 : 0;
     return cudaLaunchKernelEx(&cfg, prefix_kernel<D, COPIES, Q8>, tmk, tmv, tmq, tms, a);
 }
 
@@ -663,37 +581,6 @@ cudaError_t launch_prefix_d(const CUtensorMap &tmk, const CUtensorMap &tmv, cons
             return q8 ? launch_prefix_t<D, 4, true>(tmk, tmv, tmq, tms, a, p.splits, p.blocks, s, pdl)
                       : launch_prefix_t<D, 4, false>(tmk, tmv, tmq, tms, a, p.splits, p.blocks, s, pdl);
     }
-}
-
-// How many clusters of `size` prefix CTAs (one per SM) fit on the device at once.
-template <int D>
-int prefix_clusters(int size, int sms) {
-    static int cache[64][9] = {};  // per device and size; the GPU's partition into GPCs is fixed
-    if (size <= 1) return sms;
-    int dev = 0;
-    cudaGetDevice(&dev);
-    int n = dev < 64 ? cache[dev][size] : 0;
-    if (n == 0) {
-        configure_prefix<D, 1, false>();
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3(size, 64, 1);
-        cfg.blockDim = dim3(PrefixLayout<D>::kThreads);
-        cfg.dynamicSmemBytes = PrefixLayout<D>::kSmemBytes;
-        cudaLaunchAttribute attr;
-        attr.id = cudaLaunchAttributeClusterDimension;
-        attr.val.clusterDim.x = size;
-        attr.val.clusterDim.y = 1;
-        attr.val.clusterDim.z = 1;
-        cfg.attrs = &attr;
-        cfg.numAttrs = 1;
-        if (cudaOccupancyMaxActiveClusters(&n, prefix_kernel<D, 1, false>, &cfg) != cudaSuccess) {
-            cudaGetLastError();
-            n = 0;
-        }
-        if (n <= 0) n = -1;
-        if (dev < 64) cache[dev][size] = n;
-    }
-    return n > 0 ? n : 0;
 }
 
 // fp16 rows from f32 ones (q), eight elements per thread.
@@ -744,8 +631,8 @@ __global__ void codes_to_half_kernel(const uint8_t *kc, const uint8_t *vc, __hal
 int prefix_tile_keys() { return kXK; }
 
 // Rows: as many copies of them as fit the MMA's 128 rows, or blocks of two row tiles.  Splits of the
-// key tiles: clusters of up to eight that are all resident at once.  A split's fixed cost (launch,
-// ramp, join) is worth about six tiles, and every partial costs the merge about one.
+// key tiles over one CTA per SM: a split's fixed cost (ramp, join) is worth about six tiles, and every
+// partial costs the merge a quarter of one.
 PrefixPlan prefix_plan(int head_dim, int tokens, int group, int kv_heads, int ntiles, int sms) {
     PrefixPlan p;
     const int streams = head_dim == 256 ? 1 : 2;
@@ -753,25 +640,15 @@ PrefixPlan prefix_plan(int head_dim, int tokens, int group, int kv_heads, int nt
     p.tokens_box = kXQ / p.copies / group;
     const int per_block = p.tokens_box * (p.copies == 1 ? streams : 1);
     p.blocks = (tokens + per_block - 1) / per_block;
-    const int units = kv_heads * p.blocks;
+    const long long units = (long long)kv_heads * p.blocks;
     double best = 1e300;
-    for (int cs = 1; cs <= 8; cs *= 2) {
-        const int clusters = head_dim == 64    ? prefix_clusters<64>(cs, sms)
-                             : head_dim == 128 ? prefix_clusters<128>(cs, sms)
-                                               : prefix_clusters<256>(cs, sms);
-        if (clusters < 1) continue;
-        for (int parts = 1; parts <= 32; ++parts) {
-            const int splits = parts * cs;
-            if (splits > 1 && splits * 2 > ntiles) break;
-            const int tps = (ntiles + splits - 1) / splits;
-            // A cluster may have empty splits (they give -inf), but no part is empty.
-            if ((ntiles + tps - 1) / tps <= splits - cs) continue;
-            const long long waves = ((long long)units * parts + clusters - 1) / clusters;
-            const double cost = (double)waves * (tps + 6) + parts + (cs > 1 ? 1.0 : 0.0);
-            if (cost < best - 1e-9) {
-                best = cost;
-                p.cluster = cs, p.parts = parts, p.splits = splits, p.tiles_per_split = tps;
-            }
+    for (int n = 1; n <= 32 && (n == 1 || 2 * n <= ntiles); ++n) {
+        const int tps = (ntiles + n - 1) / n;
+        if ((ntiles + tps - 1) / tps != n) continue;  // no empty split
+        const double cost = (double)((units * n + sms - 1) / sms) * (tps + 6) + 0.25 * n;
+        if (cost < best - 1e-9) {
+            best = cost;
+            p.splits = n, p.tiles_per_split = tps;
         }
     }
     return p;
