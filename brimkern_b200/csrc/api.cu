@@ -1466,7 +1466,7 @@ int run_decode_prefix(brk_ctx *ctx, const brk_kv *prefix, int prefix_seq, int pr
                       const brk_attn_params *p, int batch, int n_tokens, const int32_t *past_len, const void *q,
                       int q_type, void *out, int out_type, cudaStream_t st, bool pdl) {
     const int D = p->head_dim, G = p->n_heads / p->n_kv_heads, Hkv = p->n_kv_heads;
-    const int window = p->window > 0 ? p->window : 0;
+    const int window = p->window > 0 ? std::min(p->window, 1 << 30) : 0;
     const size_t rows = (size_t)batch * n_tokens * p->n_heads;
     const float scale = effective_scale(p);
     const float softcap = p->softcap > 0.f ? p->softcap : 0.f;
@@ -1483,22 +1483,15 @@ int run_decode_prefix(brk_ctx *ctx, const brk_kv *prefix, int prefix_seq, int pr
         if (prefix_len > 0 && prefix->q8()) k_begin = k_begin / 4 * 4;
     }
     const int keys = prefix_len - k_begin;
-    brk::PrefixPlan plan;
-    plan.splits = 0;
-    if (keys > 0)
-        plan = brk::prefix_plan(D, batch * n_tokens, G, Hkv, (keys + brk::prefix_tile_keys() - 1) / brk::prefix_tile_keys(),
-                                ctx->num_sms);
-    const int parts = plan.splits;
     int nsplit = 1, kps = 0;
     int rc = decode_split_plan(ctx, kv, p, batch, n_tokens, past_len, false, &nsplit, &kps);
     if (rc) return rc;
     const int rt = brk::decode_rows_per_tile();
     const int mtiles = (n_tokens * G + rt - 1) / rt;
     const int units = batch * Hkv * mtiles;
-    // The own rows' merge takes in at most 32 of their splits (and 32 of the prefix's), and splits
-    // them no further than one CTA per SM: the split ranges' join through memory costs more than it
-    // gives here (16 sequences x 2 tokens of up to 777 int8 rows behind 4099: 40.7 us with 3 splits,
-    // 29.2 with 1; 8 sequences of 5000 rows and 8 kv heads still split).
+    // The merge takes in at most 32 splits of the own rows (and 32 of the prefix's); they are split no
+    // further than one CTA per SM, as the partials' way through memory costs more than it gives (16
+    // sequences x 2 tokens of up to 777 int8 rows: 16.7 us with 3 splits, 13.2 with 1).
     if (!getenv("BRK_DECODE_SPLITS") || nsplit > 32) {
         const int most = getenv("BRK_DECODE_SPLITS") ? 32 : std::max(1, std::min(32, ctx->num_sms / units));
         if (nsplit > most) {
@@ -1507,6 +1500,23 @@ int run_decode_prefix(brk_ctx *ctx, const brk_kv *prefix, int prefix_seq, int pr
             nsplit = (span + kps - 1) / kps;
         }
     }
+
+    // Own rows that are all resident at once (or alone) merge the prefix in; else a kernel of its own does.
+    const bool merge_here = keys <= 0 || (long long)units * nsplit <= ctx->num_sms;
+
+    brk::PrefixPlan plan;
+    plan.splits = 0;
+    if (keys > 0) {
+        double own_tiles = 0.0;
+        for (int b = 0; b < batch; ++b) {
+            const int own = past_len[b] + n_tokens - p->kv_offset;
+            own_tiles += ((window > 0 ? std::min(own, window) : own) + 63) / 64 * (D / 128.0);
+        }
+        own_tiles *= (double)Hkv * mtiles * (kv->q8() ? 2.0 : 1.0);
+        const int tk = brk::prefix_tile_keys();
+        plan = brk::prefix_plan(D, batch * n_tokens, G, Hkv, (keys + tk - 1) / tk, own_tiles, ctx->num_sms);
+    }
+    const int parts = plan.splits;
 
     const size_t n_ml = rows * 2 * sizeof(float), n_o = rows * D * sizeof(float);
     const size_t staged = keys > 0 && prefix->q8() ? (size_t)Hkv * keys * D * sizeof(__half) : 0;
@@ -1517,7 +1527,7 @@ int run_decode_prefix(brk_ctx *ctx, const brk_kv *prefix, int prefix_seq, int pr
         return at;
     };
     const size_t off_ml = take(parts * n_ml), off_o = take(parts * n_o);
-    const size_t off_sml = take(nsplit > 1 ? nsplit * n_ml : 0), off_so = take(nsplit > 1 ? nsplit * n_o : 0);
+    const size_t off_sml = take(nsplit * n_ml), off_so = take(nsplit * n_o);
     const size_t off_q = take(q_type == BRK_T_F32 ? rows * D * sizeof(__half) : 0);
     const size_t off_k = take(staged), off_v = take(staged);
     brk_scratch *sc = nullptr;
@@ -1543,6 +1553,7 @@ int run_decode_prefix(brk_ctx *ctx, const brk_kv *prefix, int prefix_seq, int pr
         x.B = batch, x.T = n_tokens, x.Hq = p->n_heads, x.Hkv = Hkv, x.G = G;
         x.k_begin = k_begin, x.k_end = prefix_len;
         x.tiles_per_split = plan.tiles_per_split;
+        x.g_magic = (65536 + G - 1) / G;
         x.window = window;
         x.scale_log2 = scale * (float)log2e;
         x.softcap = softcap, x.cap_k1 = cap_k1, x.cap_k2 = cap_k2;
@@ -1595,12 +1606,14 @@ int run_decode_prefix(brk_ctx *ctx, const brk_kv *prefix, int prefix_seq, int pr
     memset(&a, 0, sizeof(a));
     a.with_prefix = 1;
     a.late_wait = keys > 0;
+    a.merge_here = merge_here;
     a.pre_parts = parts;
     a.pre_ml = reinterpret_cast<const float *>(ws + off_ml);
     a.pre_o = reinterpret_cast<const float *>(ws + off_o);
     a.q16 = q16;
     a.out = out_type == BRK_T_F32 ? static_cast<float *>(out) : nullptr;
     a.out16 = out_type == BRK_T_F16 ? static_cast<__half *>(out) : nullptr;
+    a.counters = sc->counters;
     a.err = ctx->d_err;
     a.B = batch, a.T = n_tokens, a.Hq = p->n_heads, a.Hkv = Hkv, a.G = G;
     a.layer = layer;
@@ -1615,11 +1628,21 @@ int run_decode_prefix(brk_ctx *ctx, const brk_kv *prefix, int prefix_seq, int pr
     a.softcap = softcap, a.cap_k1 = cap_k1, a.cap_k2 = cap_k2;
     a.part_ml = reinterpret_cast<float *>(ws + off_sml);
     a.part_o = reinterpret_cast<float *>(ws + off_so);
-    a.counters = sc->counters;
     for (int b = 0; b < batch; ++b) a.past_len[b] = past_len[b];
     cudaError_t e = brk::launch_decode(kv->q8(), D, kv->tm_dec_k, kv->tm_dec_v, kv->q8() ? kv->tm_dec_s : kv->tm_dec_k,
                                        a, nsplit, Hkv * mtiles, batch, st, pdl);
     if (e != cudaSuccess) return cuda_fail(e, "decode kernel launch");
+    ++ctx->launches;
+    if (merge_here) return BRK_OK;
+    brk::PrefixMergeArgs g;
+    g.ml[0] = reinterpret_cast<const float *>(ws + off_ml), g.o[0] = reinterpret_cast<const float *>(ws + off_o);
+    g.ml[1] = a.part_ml, g.o[1] = a.part_o;
+    g.parts[0] = parts, g.parts[1] = nsplit;
+    g.rows = (int)rows, g.D = D;
+    g.out = out_type == BRK_T_F32 ? static_cast<float *>(out) : nullptr;
+    g.out16 = out_type == BRK_T_F16 ? static_cast<__half *>(out) : nullptr;
+    e = brk::launch_prefix_merge(g, st);
+    if (e != cudaSuccess) return cuda_fail(e, "prefix merge launch");
     ++ctx->launches;
     return BRK_OK;
 }

@@ -311,6 +311,8 @@ __global__ void __launch_bounds__(decode_threads<Q8, D, F>(), DecodeCfg<Q8, D>::
     const int new_row = past - a.kv_offset;
     const bool writes_row = F && new_row >= k_begin && new_row < k_end;
 
+    if constexpr (H)
+        if (!a.merge_here) griddep_launch_dependents();  // (the merge waits for this grid before it reads)
     if (threadIdx.x == 0) {
         for (int s = 0; s < S; ++s) {
             mbar_init(&full[s], 1);
@@ -404,6 +406,9 @@ __global__ void __launch_bounds__(decode_threads<Q8, D, F>(), DecodeCfg<Q8, D>::
             __syncwarp();
             decode_cluster_idle();  // the cluster merge's two barriers count every thread
         }
+        if constexpr (H)
+            if (a.late_wait && !a.merge_here && blockIdx.x + 1 == gridDim.x && blockIdx.y + 1 == gridDim.y && blockIdx.z + 1 == gridDim.z)
+                griddep_wait();
         return;
     }
     if constexpr (DecodeRowWarp<Q8, F>::value) {
@@ -822,9 +827,12 @@ __global__ void __launch_bounds__(decode_threads<Q8, D, F>(), DecodeCfg<Q8, D>::
     }
     named_barrier_sync(1, NC * 32);
 
-    if constexpr (H)
-        decode_epilogue_prefix<D, KG, NC, kRT>(a, ring, row0, nrows, kvh, mtile, b, split);
-    else if (a.cluster)
+    if constexpr (H) {
+        if (a.merge_here)
+            decode_epilogue_merge<D, KG, NC, kRT>(a, ring, row0, nrows, kvh, mtile, b, split);
+        else
+            decode_epilogue_prefix<D, KG, NC, kRT>(a, ring, row0, nrows, kvh, b, split);
+    } else if (a.cluster)
         decode_epilogue_cluster<D, KG, NC, kRT>(a, ring, row0, nrows, kvh, b, split);
     else
         decode_epilogue<D, KG, NC, kRT>(a, ring, row0, nrows, kvh, mtile, b, split);

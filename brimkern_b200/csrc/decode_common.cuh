@@ -199,12 +199,12 @@ __device__ __forceinline__ void decode_epilogue(const DecodeArgs &a, uint8_t *ri
     if (a.push_world) push_finish<NC>(a);
 }
 
-// The epilogue of the own rows of sequences that share a prefix (brk_attn_decode_prefix).  As in
-// decode_epilogue, but what merges a row -- the tile's only CTA, or with split-KV its last -- also
-// takes in the prefix kernel's pre_parts partials of that row and writes the final output, f32 or
-// fp16.  The partials are ordered, so the sums are the same whichever CTA is last.
+// The epilogues of the own rows of sequences that share a prefix (brk_attn_decode_prefix).  First: what
+// merges a row -- the tile's only CTA, or with split-KV its last -- also takes in the prefix kernel's
+// pre_parts partials of that row and writes the final output, f32 or fp16; a CTA waits for that kernel
+// only here.  For grids that are resident all at once.
 template <int D, int KG, int NC, int RT>
-__device__ __forceinline__ void decode_epilogue_prefix(const DecodeArgs &a, uint8_t *ring, int row0, int nrows, int kvh,
+__device__ __forceinline__ void decode_epilogue_merge(const DecodeArgs &a, uint8_t *ring, int row0, int nrows, int kvh,
                                                        int mt, int b, int split) {
     float *cm = reinterpret_cast<float *>(ring);
     float *cl = cm + KG * RT;
@@ -329,6 +329,42 @@ __device__ __forceinline__ void decode_epilogue_prefix(const DecodeArgs &a, uint
             *reinterpret_cast<uint2 *>(a.out16 + R * D + 4 * d4) = make_uint2(pack_half2(O.x, O.y), pack_half2(O.z, O.w));
         else
             *reinterpret_cast<float4 *>(a.out + R * D + 4 * d4) = O;
+    }
+}
+
+// Second, for grids of several waves, whose CTAs must not wait for the prefix kernel in their slots:
+// the CTA's partial goes out as it is, and prefix_merge_kernel joins it with the other splits' and the
+// prefix's.
+template <int D, int KG, int NC, int RT>
+__device__ __forceinline__ void decode_epilogue_prefix(const DecodeArgs &a, uint8_t *ring, int row0, int nrows, int kvh,
+                                                       int b, int split) {
+    const float *cm = reinterpret_cast<const float *>(ring);
+    const float *cl = cm + KG * RT;
+    const float *co = cl + KG * RT;
+    const int nvalid = min(RT, nrows - row0);
+    constexpr int D4 = D / 4;
+    for (int idx = threadIdx.x; idx < nvalid * D4; idx += NC * 32) {
+        const int r = idx / D4, d4 = idx % D4;
+        float m[KG], M = -CUDART_INF_F;
+#pragma unroll
+        for (int w = 0; w < KG; ++w) {
+            m[w] = cm[w * RT + r];
+            M = fmaxf(M, m[w]);
+        }
+        float l = 0.f;
+        float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < KG; ++w) {
+            const float f = m[w] == -CUDART_INF_F ? 0.f : ex2_fast(m[w] - M);
+            const float4 x = *reinterpret_cast<const float4 *>(co + (w * RT + r) * D + 4 * d4);
+            l = fmaf(f, cl[w * RT + r], l);
+            O.x = fmaf(f, x.x, O.x), O.y = fmaf(f, x.y, O.y), O.z = fmaf(f, x.z, O.z), O.w = fmaf(f, x.w, O.w);
+        }
+        const int rr = row0 + r, t = rr / a.G;
+        const size_t PR = ((size_t)split * a.B * a.T + (size_t)b * a.T + t) * a.Hq + kvh * a.G + (rr - t * a.G);
+        *reinterpret_cast<float4 *>(a.part_o + PR * D + 4 * d4) = O;
+        if (d4 == 0)
+            *reinterpret_cast<float2 *>(a.part_ml + PR * 2) = make_float2(M == -CUDART_INF_F ? M : M * kLn2, l);
     }
 }
 

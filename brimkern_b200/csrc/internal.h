@@ -166,13 +166,15 @@ struct DecodeArgs {
     double eps;
     int one_plus;
     // Own rows of sequences that share a prefix (brk_attn_decode_prefix, decode_kernel's H form):
-    // q in fp16, the prefix kernel's pre_parts partials [part][rows][2] and
-    // [part][rows][D], the fp16 output (or a.out), and whether the preceding kernel of this call
-    // is the prefix kernel, whose partials alone have to be waited for.
+    // q in fp16 (replaces q); whether the preceding kernel is the prefix kernel, which has to be
+    // waited for only before its partials are read; merge_here: the prefix kernel's pre_parts
+    // partials [part][rows][2], [part][rows][D] are merged in and the output (fp16 out16, or out)
+    // written here, else the partials [split][rows] at part_ml / part_o.
     int with_prefix;
     int late_wait;
+    int merge_here;
     int pre_parts;
-    const __half *q16;      // replaces q
+    const __half *q16;
     const float *pre_ml, *pre_o;
     __half *out16;
     int past_len[BRK_MAX_BATCH];
@@ -189,9 +191,20 @@ struct PrefixArgs {
     int head_rows;        // map rows from one kv head to the next
     int k_begin, k_end;   // keys some row attends
     int tiles_per_split;
+    int g_magic;          // x / G = x * g_magic >> 16 for x < 256
     int window;
     float scale_log2, softcap, cap_k1, cap_k2;
     int past_len[BRK_MAX_BATCH];
+};
+
+// The merge of a shared-prefix call: the prefix's and the own rows' partials to the output.
+constexpr int kPrefixMostParts = 64;  // of both together; at most 32 of the prefix's
+struct PrefixMergeArgs {
+    const float *ml[2], *o[2];  // prefix, own rows: [part][rows][2] (m natural-log units, l), [part][rows][D]
+    int parts[2];
+    int rows, D;
+    float *out;                 // [rows][D] f32, or
+    __half *out16;              //   fp16
 };
 
 // How the prefix's work is cut: copies of the query rows in the MMA's rows, tokens per q box, row
@@ -351,9 +364,11 @@ cudaError_t launch_linear_rows(int mats, const LinearArgs &a, cudaStream_t s);
 // rows (for an int8 cache: its codes as fp16, staged by launch_codes_to_half, and its scales with
 // [2][64] boxes), tmq with boxes [tokens_box][group][64] over the fp16 q [tokens][heads][D].
 int prefix_tile_keys();
-PrefixPlan prefix_plan(int head_dim, int tokens, int group, int kv_heads, int ntiles, int sms);
+// own_tiles: 64-key tiles of own rows that another kernel reads at the same time.
+PrefixPlan prefix_plan(int head_dim, int tokens, int group, int kv_heads, int ntiles, double own_tiles, int sms);
 cudaError_t launch_prefix(int head_dim, const CUtensorMap &tmk, const CUtensorMap &tmv, const CUtensorMap &tmq,
                           const CUtensorMap &tms, const PrefixArgs &a, const PrefixPlan &p, cudaStream_t s, bool pdl);
+cudaError_t launch_prefix_merge(const PrefixMergeArgs &a, cudaStream_t s);  // a programmatic dependent
 // n (a multiple of 8) fp16 values from f32 ones.
 cudaError_t launch_half_rows(const float *src, __half *dst, size_t n, cudaStream_t s, bool pdl);
 // Codes of rows [row0, row0 + rows) of every kv head of one (layer, sequence) as fp16 [Hkv][rows][D].

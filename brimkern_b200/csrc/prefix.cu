@@ -16,13 +16,15 @@
 // exponentials instead of one warp doing them: what bounds the loop is then the K/V stream.
 //
 // The end: streams and copies are joined in shared memory and the split's partial leaves in coalesced
-// rows; the merge of the own rows' kernel takes in the splits.  (Joining the splits of a cluster
-// through distributed shared memory first, for an eighth of the partials: 131 KB a CTA took 5 us
-// there, and the merge was no faster with 2 partials than with 16.)
+// rows; the own rows' kernel or prefix_merge_kernel joins the splits with the own rows.  (Joining the splits of a
+// cluster through distributed shared memory first, for an eighth of the partials: 131 KB a CTA took
+// 5 us there.)
 //
 // int8 prefix: the codes, as exact fp16 integers, are the operands; the K scale multiplies the
 // scores and the V scale the probabilities, so nothing is rounded that the fp16 form does not round.
 #include <math_constants.h>
+
+#include <algorithm>
 
 #include "common.cuh"
 #include "internal.h"
@@ -522,7 +524,8 @@ __global__ void __launch_bounds__(PrefixLayout<D>::kThreads, 1)
                         }
                     }
                 if (x0 + u < n_rows) {
-                    const size_t R = (size_t)(bt0 + x / a.G) * a.Hq + kvh * a.G + x % a.G;
+                    const int xt = x * a.g_magic >> 16;  // x / G
+                    const size_t R = (size_t)(bt0 + xt) * a.Hq + kvh * a.G + (x - xt * a.G);
 #pragma unroll
                     for (int v = 0; v < VPL; ++v)
                         *reinterpret_cast<float4 *>(out_o + R * D + 4 * (l4 + v * LPR)) = O[v];
@@ -583,6 +586,70 @@ cudaError_t launch_prefix_d(const CUtensorMap &tmk, const CUtensorMap &tmv, cons
     }
 }
 
+static_assert(kPrefixMostParts == 64, "the merge's two weights per lane");
+
+// A warp per row: the partials' weights by lanes, then the row's float4s by lanes with eight partials'
+// loads in flight.  M = max m, o = sum e^{m - M} o / sum e^{m - M} l.
+__global__ void __launch_bounds__(128) prefix_merge_kernel(const __grid_constant__ PrefixMergeArgs a) {
+    griddep_wait();
+    const int row = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (row >= a.rows) return;
+    const size_t R = row, n = a.rows;
+    const int n0 = a.parts[0], parts = n0 + a.parts[1];
+    constexpr int NU = kPrefixMostParts / 32;
+    float2 ml[NU];
+    float M = -CUDART_INF_F;
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+        const int p = lane + 32 * u;
+        ml[u] = make_float2(-CUDART_INF_F, 0.f);
+        if (p < parts)
+            ml[u] = *reinterpret_cast<const float2 *>(p < n0 ? a.ml[0] + ((size_t)p * n + R) * 2
+                                                             : a.ml[1] + ((size_t)(p - n0) * n + R) * 2);
+        M = fmaxf(M, ml[u].x);
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
+    float w[NU], l = 0.f;
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+        w[u] = ml[u].x == -CUDART_INF_F ? 0.f : expf(ml[u].x - M);
+        l = fmaf(w[u], ml[u].y, l);
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+    const float inv = 1.f / l;
+    for (int d0 = 0; d0 < a.D / 4; d0 += 32) {
+        const int d4 = d0 + lane;
+        const bool in = d4 < a.D / 4;  // (head_dim 64: half of the warp has none, but has weights)
+        float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int p0 = 0; p0 < parts; p0 += 8) {
+            float4 v[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int p = p0 + u;
+                const float *src = p < n0 ? a.o[0] + ((size_t)p * n + R) * a.D : a.o[1] + ((size_t)(p - n0) * n + R) * a.D;
+                v[u] = in && p < parts ? __ldcs(reinterpret_cast<const float4 *>(src) + d4) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                // Partials that hold nothing (weight 0) are not multiplied: an idle split's row may be anything.
+                const int p = p0 + u;
+                const float f = __shfl_sync(0xffffffffu, p < 32 ? w[0] : w[1], p & 31);
+                if (p < parts && f != 0.f)
+                    O.x = fmaf(f, v[u].x, O.x), O.y = fmaf(f, v[u].y, O.y), O.z = fmaf(f, v[u].z, O.z),
+                    O.w = fmaf(f, v[u].w, O.w);
+            }
+        }
+        O.x *= inv, O.y *= inv, O.z *= inv, O.w *= inv;
+        if (!in) continue;
+        if (a.out16)
+            reinterpret_cast<uint2 *>(a.out16 + R * a.D)[d4] = make_uint2(pack_half2(O.x, O.y), pack_half2(O.z, O.w));
+        else
+            reinterpret_cast<float4 *>(a.out + R * a.D)[d4] = O;
+    }
+}
+
 // fp16 rows from f32 ones (q), eight elements per thread.
 __global__ void half_rows_kernel(const float *src, __half *dst, long long n8) {
     griddep_wait();
@@ -632,8 +699,11 @@ int prefix_tile_keys() { return kXK; }
 
 // Rows: as many copies of them as fit the MMA's 128 rows, or blocks of two row tiles.  Splits of the
 // key tiles over one CTA per SM: a split's fixed cost (ramp, join) is worth about six tiles, and every
-// partial costs the merge a quarter of one.
-PrefixPlan prefix_plan(int head_dim, int tokens, int group, int kv_heads, int ntiles, int sms) {
+// partial costs the merge a quarter of one.  The own rows' kernel runs beside this one on the SMs that
+// it leaves (an SM has room for one or the other), so the SMs are shared out by the work of both, at
+// most half of them to the own rows: 64 sequences of 256 own rows behind 4096 take 39.6 us with 16
+// splits for 8 kv heads (one after the other), 30.5 with 8, 45.6 with 3.
+PrefixPlan prefix_plan(int head_dim, int tokens, int group, int kv_heads, int ntiles, double own_tiles, int sms) {
     PrefixPlan p;
     const int streams = head_dim == 256 ? 1 : 2;
     p.copies = tokens * group <= (kXQ / 4 / group) * group ? 4 : tokens * group <= (kXQ / 2 / group) * group ? 2 : 1;
@@ -641,11 +711,15 @@ PrefixPlan prefix_plan(int head_dim, int tokens, int group, int kv_heads, int nt
     const int per_block = p.tokens_box * (p.copies == 1 ? streams : 1);
     p.blocks = (tokens + per_block - 1) / per_block;
     const long long units = (long long)kv_heads * p.blocks;
+    // Thousands of cycles of an SM: a tile here, a tile of own rows there (half: two of its CTAs run).
+    const double tile = streams == 1 || (p.copies == 1 && tokens > p.tokens_box) ? 2.0 : p.copies == 1 ? 1.0 : 0.75;
+    const double mine = (double)units * ntiles * tile, theirs = 0.5 * own_tiles;
+    const int share = std::max(1, (int)(sms * (1.0 - std::min(0.5, theirs / (mine + theirs)))));
     double best = 1e300;
     for (int n = 1; n <= 32 && (n == 1 || 2 * n <= ntiles); ++n) {
         const int tps = (ntiles + n - 1) / n;
         if ((ntiles + tps - 1) / tps != n) continue;  // no empty split
-        const double cost = (double)((units * n + sms - 1) / sms) * (tps + 6) + 0.25 * n;
+        const double cost = (double)((units * n + share - 1) / share) * (tps + 6) + 0.25 * n;
         if (cost < best - 1e-9) {
             best = cost;
             p.splits = n, p.tiles_per_split = tps;
@@ -662,6 +736,19 @@ cudaError_t launch_prefix(int head_dim, const CUtensorMap &tmk, const CUtensorMa
         case 256: return launch_prefix_d<256>(tmk, tmv, tmq, tms, a, p, s, pdl);
         default: return cudaErrorInvalidValue;
     }
+}
+
+cudaError_t launch_prefix_merge(const PrefixMergeArgs &a, cudaStream_t s) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((a.rows + 3) / 4));
+    cfg.blockDim = dim3(128);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, prefix_merge_kernel, a);
 }
 
 cudaError_t launch_half_rows(const float *src, __half *dst, size_t n, cudaStream_t s, bool pdl) {
