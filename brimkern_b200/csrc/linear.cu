@@ -17,8 +17,8 @@
 //     SMs stream without a way through global memory;
 //   - products whose tiles do not fill whole waves: the last one to two waves' tiles are dealt as
 //     (tile, k step) units in equal contiguous ranges.  A range's first and last piece may cover part
-//     of a tile's k; such pieces leave f32 partials in the workspace, and the last CTA of a tile
-//     to finish adds them in k order (the same order whoever is last: results do not change from run
+//     of a tile's k; such pieces leave f32 partials in the workspace (the last to finish keeps its own
+//     in TMEM), and the last CTA of a tile to finish adds them in k order (the same order whoever is last: results do not change from run
 //     to run; so does the cluster's join).  The ranges come first, so that the joins run under the whole tiles.
 // Gate-up (MODE): a CTA holds the gate and the up tile of the same F features in two accumulators
 // (kTwoAcc); with PAIR they are interleaved, 64 gate rows and 64 up rows in one accumulator
@@ -202,6 +202,11 @@ __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
                  : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
                  : "r"(addr)
                  : "memory");
+    return v;
+}
+__device__ __forceinline__ int ld_acquire_gpu(const int *p) {
+    int v;
+    asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
     return v;
 }
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
@@ -552,7 +557,20 @@ __global__ void __launch_bounds__(LinearLayout<NT, MODE, PAIR>::kThreads, 1)
             ok = __all_sync(0xffffffffu, got);
             ++seg;
             tc_fence_after();
-            if (DRAIN && has_res && whole && cs == 1) load_res(0, res);
+            // A part of a tile: when all the others have arrived this one need not go through memory.
+            const int t0 = (p.tile - a.tiles_whole) * a.nk;
+            const int c_first = whole ? 0 : worker_of(a, t0), c_last = whole ? 0 : worker_of(a, t0 + a.nk - 1);
+            int *counter = a.counters + (p.tile - a.tiles_whole) * CTAS + rank;
+            bool joining = false;
+            if (!whole) {
+                if (threadIdx.x == 0) {
+                    s_last = ld_acquire_gpu(counter) == c_last - c_first;
+                    if (s_last) *counter = 0;  // ready for the next launch
+                }
+                named_barrier_sync(2, EPI);
+                joining = s_last;
+            }
+            if (has_res && cs == 1 && (joining || (DRAIN && whole))) load_res(0, res);
 #pragma unroll 1
             for (int c0 = 0; c0 < ntok; c0 += CH) {
                 uint32_t vr[CH], wr[CH];
@@ -571,8 +589,40 @@ __global__ void __launch_bounds__(LinearLayout<NT, MODE, PAIR>::kThreads, 1)
                             *reinterpret_cast<uint4 *>(dst + (size_t)nt * kLF + e * kLF) =
                                 make_uint4(wr[e], wr[e + 1], wr[e + 2], wr[e + 3]);
                     }
-                } else if (whole) {
+                } else if (whole || joining) {
                     float v[CH], w[CH];
+                    if (joining) {
+                        // The parts added in k order, this one from TMEM in its place.
+                        float sum[MATS][CH];
+#pragma unroll
+                        for (int m = 0; m < MATS; ++m)
+#pragma unroll
+                            for (int e = 0; e < CH; ++e) sum[m][e] = 0.f;
+#pragma unroll 1
+                        for (int q = c_first; q <= c_last; ++q) {
+                            const int slot = range_begin(a, q) >= t0 ? 0 : 1;
+                            const float *src = a.ws + ((size_t)(q * CTAS + rank) * 2 + slot) * slot_floats +
+                                               (size_t)(col0 + c0) * kLF + lrow * 4;
+#pragma unroll
+                            for (int m = 0; m < MATS; ++m)
+#pragma unroll
+                                for (int e = 0; e < CH; e += 4) {
+                                    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+                                    if (q != worker && c0 + e < ntok)
+                                        x = __ldcg(reinterpret_cast<const float4 *>(src + (size_t)(m * nt + e) * kLF));
+                                    const uint32_t(&own)[CH] = m ? wr : vr;
+                                    sum[m][e] += q == worker ? __uint_as_float(own[e]) : x.x;
+                                    sum[m][e + 1] += q == worker ? __uint_as_float(own[e + 1]) : x.y;
+                                    sum[m][e + 2] += q == worker ? __uint_as_float(own[e + 2]) : x.z;
+                                    sum[m][e + 3] += q == worker ? __uint_as_float(own[e + 3]) : x.w;
+                                }
+                        }
+#pragma unroll
+                        for (int e = 0; e < CH; ++e) {
+                            vr[e] = __float_as_uint(sum[0][e]);
+                            if constexpr (MATS == 2) wr[e] = __float_as_uint(sum[MATS - 1][e]);
+                        }
+                    }
                     if constexpr (MODE == kInterleaved) {
                         const bool up = quarter >= 2;
                         float *buf_g = swap + (swaps & 1) * 512, *buf_u = buf_g + 256;
@@ -616,17 +666,16 @@ __global__ void __launch_bounds__(LinearLayout<NT, MODE, PAIR>::kThreads, 1)
                 }
             }
             release(buf);
-            if (!whole) {
-                // The last CTA of the tile (and rank) to finish adds the pieces in k order.
+            if (joining) named_barrier_sync(2, EPI);  // s_last is read before the next piece writes it
+            if (!whole && !joining) {
+                // Others are still at it: the last of them to finish -- this one after all, maybe -- adds
+                // the pieces in k order.
                 named_barrier_sync(2, EPI);
-                const int t0 = (p.tile - a.tiles_whole) * a.nk;
-                const int c_first = worker_of(a, t0), c_last = worker_of(a, t0 + a.nk - 1);
                 if (threadIdx.x == 0) {
-                    int *counter = a.counters + (p.tile - a.tiles_whole) * CTAS + rank;
                     __threadfence();  // the CTA's partial (ordered before by the barrier) before the count
                     const int prev = atomicAdd(counter, 1);
                     s_last = prev == c_last - c_first;
-                    if (s_last) *counter = 0;  // ready for the next launch
+                    if (s_last) *counter = 0;
                     __threadfence();
                 }
                 named_barrier_sync(2, EPI);
@@ -957,10 +1006,10 @@ LinearPlan linear_plan(int rows, int k, int n, int mats, int sms) {
         if (cs > 1 && p.tiles > slots) return;
         const int lanes = pair ? kLF : f * mats;  // weight rows of a k step and CTA
         const double step = std::max(accs * 4.0 * std::max(p.nt / 2, 32), (lanes + p.nt / ctas) * 128 / 48.0);
-        const double epilogue = 800.0 + p.nt * 24.0;
+        const double epilogue = 800.0 + p.nt * (accs == 2 ? 60.0 : 24.0);
         double cost;
         if (ranged) {
-            const double join = 6000.0 + p.nt * 90.0;
+            const double join = 4000.0 + p.nt * 60.0;
             cost = (double)p.tiles * nkb / slots * step + join + epilogue;
         } else if (cs > 1) {
             cost = (double)((nkb + cs - 1) / cs) * step + 3000.0 + accs * p.nt * 12.0 + epilogue / cs;

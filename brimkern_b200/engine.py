@@ -42,9 +42,20 @@ def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
 
 
 _T_TYPES = {torch.float32: L.BRK_T_F32, torch.float16: L.BRK_T_F16}
+_F16, _F32 = (torch.float16,), (torch.float32,)
+
+# The current stream's handle without a Stream object around it (2 us of a small call), where this
+# torch has that.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _positions(past_len, batch: int):
+    if isinstance(past_len, (list, tuple)) and len(past_len) == batch:
+        try:
+            return (ctypes.c_int32 * batch)(*past_len)
+        except TypeError:
+            pass  # not all plain ints
     arr = (ctypes.c_int32 * batch)()
     vals = [int(past_len)] * batch if np.isscalar(past_len) else [int(x) for x in past_len]
     if len(vals) != batch:
@@ -641,11 +652,14 @@ class AttentionEngine:
     def _tensor(self, t: torch.Tensor, name: str, dtypes, shape) -> int:
         """The address of a tensor that the kernels read or write as it is: on this engine's device,
         of one of `dtypes`, contiguous, of `shape` (None: not checked)."""
+        if (t.dtype in dtypes and t.get_device() == self.device.index and (shape is None or t.shape == shape)
+                and t.is_contiguous()):
+            return t.data_ptr()
         if t.device != self.device:
             raise BrkError(L.BRK_ERR_INVALID, f"{name} is on {t.device}, the engine on {self.device}")
         if t.dtype not in dtypes:
             raise BrkError(L.BRK_ERR_INVALID, f"{name} is {t.dtype}, not {' or '.join(map(str, dtypes))}")
-        if shape is not None and tuple(t.shape) != shape:
+        if shape is not None and t.shape != shape:
             raise BrkError(L.BRK_ERR_INVALID, f"{name} has shape {tuple(t.shape)}, not {shape}")
         if not t.is_contiguous():
             raise BrkError(L.BRK_ERR_INVALID, f"{name} is not contiguous")
@@ -653,7 +667,7 @@ class AttentionEngine:
 
     def _stream(self, stream: Optional[torch.cuda.Stream]) -> int:
         """The given stream, or the current one of this engine's device."""
-        return (stream if stream is not None else torch.cuda.current_stream(self.device)).cuda_stream
+        return _raw_stream(self.device.index) if stream is None else stream.cuda_stream
 
     @staticmethod
     def _activation(act: str) -> int:
@@ -663,10 +677,10 @@ class AttentionEngine:
             raise BrkError(L.BRK_ERR_INVALID, f"activation {act!r} (one of {', '.join(L.ACTIVATIONS)})") from None
 
     def _prefix_tokens(self, kv: KvCache, cfg: AttnConfig, q: torch.Tensor, name: str) -> int:
-        per = kv.batch * cfg.n_heads * cfg.head_dim
-        if per < 1 or q.numel() % per or q.numel() == 0:
-            raise BrkError(L.BRK_ERR_INVALID, f"{name} has {q.numel()} elements, not a multiple of batch * heads * dim {per}")
-        return q.numel() // per
+        per, n = kv.batch * cfg.n_heads * cfg.head_dim, q.numel()
+        if per < 1 or n % per or n == 0:
+            raise BrkError(L.BRK_ERR_INVALID, f"{name} has {n} elements, not a multiple of batch * heads * dim {per}")
+        return n // per
 
     def decodePrefix(self, prefix: Optional[KvCache], prefix_len: int, kv: KvCache, layer: int, cfg: AttnConfig,
                      q: torch.Tensor, out: torch.Tensor, past_len, prefix_seq: int = 0, stream=None) -> torch.Tensor:
@@ -694,10 +708,10 @@ class AttentionEngine:
         RoPE as appendKv), then decodePrefix.  q_in [B, T, Hq, D], k_in / v_in [B, T, Hkv, D] f32
         projections; out f32 (default) or fp16."""
         T = self._prefix_tokens(kv, cfg, q_in, "q_in")
-        f32, n_kv = (torch.float32,), kv.batch * T * cfg.n_kv_heads * cfg.head_dim
+        n_kv = kv.batch * T * cfg.n_kv_heads * cfg.head_dim
         q_work = torch.empty_like(q_in) if q_work is None else q_work
         out = torch.empty_like(q_in) if out is None else out
-        ptrs = [self._tensor(t, n, f32, None) for t, n in ((q_in, "q_in"), (k_in, "k_in"), (v_in, "v_in"), (q_work, "q_work"))]
+        ptrs = [self._tensor(t, n, _F32, None) for t, n in ((q_in, "q_in"), (k_in, "k_in"), (v_in, "v_in"), (q_work, "q_work"))]
         op = self._tensor(out, "out", _T_TYPES, None)
         for t, n, want in ((k_in, "k_in", n_kv), (v_in, "v_in", n_kv), (q_work, "q_work", q_in.numel()),
                            (out, "out", q_in.numel())):
@@ -714,15 +728,14 @@ class AttentionEngine:
                act: str = "none", residual: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
         """out = act(x w^T + bias) + residual.  x [rows, k] fp16, w [n, k] fp16, bias [n] f32,
         residual [rows, n] f32, out [rows, n] f32 or fp16 (f32: may be the residual itself)."""
-        f16, f32 = (torch.float16,), (torch.float32,)
         if x.dim() != 2 or w.dim() != 2:
             raise BrkError(L.BRK_ERR_INVALID, f"x and w are matrices, not {tuple(x.shape)} and {tuple(w.shape)}")
         rows, k = x.shape
         n = w.shape[0]
-        check(L.lib().brk_linear(self.ctx.handle, rows, k, n, self._tensor(x, "x", f16, None),
-                                 self._tensor(w, "w", f16, (n, k)),
-                                 None if bias is None else self._tensor(bias, "bias", f32, (n,)), self._activation(act),
-                                 None if residual is None else self._tensor(residual, "residual", f32, (rows, n)),
+        check(L.lib().brk_linear(self.ctx.handle, rows, k, n, self._tensor(x, "x", _F16, None),
+                                 self._tensor(w, "w", _F16, (n, k)),
+                                 None if bias is None else self._tensor(bias, "bias", _F32, (n,)), self._activation(act),
+                                 None if residual is None else self._tensor(residual, "residual", _F32, (rows, n)),
                                  self._tensor(out, "out", _T_TYPES, (rows, n)), _T_TYPES[out.dtype],
                                  self._stream(stream)))
         return out
@@ -732,17 +745,16 @@ class AttentionEngine:
                   stream=None) -> torch.Tensor:
         """hidden = act(x w_gate^T + b_gate) * (x w_up^T + b_up).  x [rows, d] fp16, weights [ff, d]
         fp16, biases [ff] f32, hidden [rows, ff] fp16."""
-        f16, f32 = (torch.float16,), (torch.float32,)
         if x.dim() != 2 or w_gate.dim() != 2:
             raise BrkError(L.BRK_ERR_INVALID, f"x and w_gate are matrices, not {tuple(x.shape)} and {tuple(w_gate.shape)}")
         rows, d = x.shape
         ff = w_gate.shape[0]
-        check(L.lib().brk_ffn_gate_up(self.ctx.handle, rows, d, ff, self._tensor(x, "x", f16, None),
-                                      self._tensor(w_gate, "w_gate", f16, (ff, d)),
-                                      self._tensor(w_up, "w_up", f16, (ff, d)),
-                                      None if b_gate is None else self._tensor(b_gate, "b_gate", f32, (ff,)),
-                                      None if b_up is None else self._tensor(b_up, "b_up", f32, (ff,)),
-                                      self._activation(act), self._tensor(hidden, "hidden", f16, (rows, ff)),
+        check(L.lib().brk_ffn_gate_up(self.ctx.handle, rows, d, ff, self._tensor(x, "x", _F16, None),
+                                      self._tensor(w_gate, "w_gate", _F16, (ff, d)),
+                                      self._tensor(w_up, "w_up", _F16, (ff, d)),
+                                      None if b_gate is None else self._tensor(b_gate, "b_gate", _F32, (ff,)),
+                                      None if b_up is None else self._tensor(b_up, "b_up", _F32, (ff,)),
+                                      self._activation(act), self._tensor(hidden, "hidden", _F16, (rows, ff)),
                                       self._stream(stream)))
         return hidden
 
@@ -752,17 +764,16 @@ class AttentionEngine:
         """The feed-forward half of a layer: out = h + w_down (act(w_gate x) * (w_up x)) with
         x = rmsnorm(h, ffn_norm) (Gemma-2: the block's output normed by post_norm before the add).
         h / out [rows, d] f32, w_gate / w_up [ff, d] and w_down [d, ff] fp16."""
-        f16, f32 = (torch.float16,), (torch.float32,)
         if h.dim() != 2 or w_gate.dim() != 2:
             raise BrkError(L.BRK_ERR_INVALID, f"h and w_gate are matrices, not {tuple(h.shape)} and {tuple(w_gate.shape)}")
         rows, d = h.shape
         ff = w_gate.shape[0]
-        check(L.lib().brk_ffn(self.ctx.handle, rows, d, ff, self._tensor(h, "h", f32, None),
-                              None if ffn_norm is None else self._tensor(ffn_norm, "ffn_norm", f32, (d,)), float(eps),
-                              int(bool(one_plus)), self._tensor(w_gate, "w_gate", f16, (ff, d)),
-                              self._tensor(w_up, "w_up", f16, (ff, d)), self._tensor(w_down, "w_down", f16, (d, ff)),
-                              None if post_norm is None else self._tensor(post_norm, "post_norm", f32, (d,)),
-                              self._activation(act), self._tensor(out, "out", f32, (rows, d)), self._stream(stream)))
+        check(L.lib().brk_ffn(self.ctx.handle, rows, d, ff, self._tensor(h, "h", _F32, None),
+                              None if ffn_norm is None else self._tensor(ffn_norm, "ffn_norm", _F32, (d,)), float(eps),
+                              int(bool(one_plus)), self._tensor(w_gate, "w_gate", _F16, (ff, d)),
+                              self._tensor(w_up, "w_up", _F16, (ff, d)), self._tensor(w_down, "w_down", _F16, (d, ff)),
+                              None if post_norm is None else self._tensor(post_norm, "post_norm", _F32, (d,)),
+                              self._activation(act), self._tensor(out, "out", _F32, (rows, d)), self._stream(stream)))
         return out
 
     # ---- the projections either side of the operator (recordLayerKV, kernels.ts:1700-1736) -----
