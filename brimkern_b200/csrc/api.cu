@@ -1425,6 +1425,16 @@ size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
 bool aligned16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
+// The prefix's bytes, counted once per unit that would read them for itself, up to which a single launch
+// does (from L2: the units ask for the same rows).  Above, one kernel reads the prefix once for all
+// sequences and the own rows go beside it.  Both ways at 32 query / 8 KV heads of 128, 200 own rows,
+// one launch / prefix kernel, us: 4 sequences x 128 rows (2 MB) 6.6 / 9.0, 16 x 128 (8 MB) 7.1 / 10.7,
+// 4 x 2048 (34 MB) 10.0 / 10.4, 16 x 512 (34 MB) 11.1 / 11.0, 8 x 2048 (67 MB) 12.0 / 11.4,
+// 16 x 2048 (134 MB) 18.2 / 12.1; heads of 64 and 256 cross over between the same bytes; int8 rows
+// (which the prefix kernel would stage as fp16) 4 x 512 (4 MB) 9.2 / 11.6, 8 x 2048 (34 MB) 15.4 / 15.4,
+// 16 x 2048 (67 MB) 20.9 / 17.1.
+constexpr double kPrefixRereadBytes = 32.0 * 1024 * 1024;
+
 int check_prefix_call(const brk_ctx *ctx, const brk_kv *prefix, int prefix_seq, int prefix_len, const brk_kv *kv,
                       int layer, const brk_attn_params *p, int batch, int n_tokens, const int32_t *past_len,
                       const void *q, int q_type, const void *out, int out_type) {
@@ -1501,12 +1511,33 @@ int run_decode_prefix(brk_ctx *ctx, const brk_kv *prefix, int prefix_seq, int pr
         }
     }
 
+    // One launch in which each unit goes over the prefix's rows and then its own, or the prefix apart.
+    const double reread = (double)units * keys * D * (kv->q8() ? 2.0 : 4.0);
+    const bool together = keys > 0 && prefix->q8() == kv->q8() && reread <= kPrefixRereadBytes;
+    int pre_tiles = 0, tps_together = 0;
+    bool cluster = false;
+    if (together) {
+        const int tk = brk::decode_stage_keys(D);
+        pre_tiles = (keys + tk - 1) / tk;
+        int own = 0;  // the longest sequence's own stages (+ 1: a window's first key may be rounded down)
+        for (int b = 0; b < batch; ++b) {
+            const int hi = past_len[b] + n_tokens - p->kv_offset;
+            const int lo = window > 0 ? std::max(0, past_len[b] - window + 1 - p->kv_offset) : 0;
+            own = std::max(own, (hi - lo + 3 + tk - 1) / tk);
+        }
+        const int tiles = pre_tiles + own;
+        nsplit = std::min(32, choose_splits(ctx, D, kv->q8(), units, tiles * tk));
+        tps_together = (tiles + nsplit - 1) / nsplit;
+        nsplit = (tiles + tps_together - 1) / tps_together;
+        kps = 1 << 30;  // the own rows are one range
+        cluster = nsplit > 1 && nsplit <= brk::kMaxClusterSplits && units <= brk::decode_max_clusters(D, kv->q8(), nsplit);
+    }
     // Own rows that are all resident at once (or alone) merge the prefix in; else a kernel of its own does.
-    const bool merge_here = keys <= 0 || (long long)units * nsplit <= ctx->num_sms;
+    const bool merge_here = keys <= 0 || together || (long long)units * nsplit <= ctx->num_sms;
 
     brk::PrefixPlan plan;
     plan.splits = 0;
-    if (keys > 0) {
+    if (keys > 0 && !together) {
         double own_tiles = 0.0;
         for (int b = 0; b < batch; ++b) {
             const int own = past_len[b] + n_tokens - p->kv_offset;
@@ -1519,7 +1550,7 @@ int run_decode_prefix(brk_ctx *ctx, const brk_kv *prefix, int prefix_seq, int pr
     const int parts = plan.splits;
 
     const size_t n_ml = rows * 2 * sizeof(float), n_o = rows * D * sizeof(float);
-    const size_t staged = keys > 0 && prefix->q8() ? (size_t)Hkv * keys * D * sizeof(__half) : 0;
+    const size_t staged = parts > 0 && prefix->q8() ? (size_t)Hkv * keys * D * sizeof(__half) : 0;
     size_t bytes = 0;
     auto take = [&](size_t n) {
         const size_t at = bytes;
@@ -1544,7 +1575,7 @@ int run_decode_prefix(brk_ctx *ctx, const brk_kv *prefix, int prefix_seq, int pr
         q16 = qh;
         pdl = true;
     }
-    if (keys > 0) {
+    if (parts > 0) {
         brk::PrefixArgs x;
         memset(&x, 0, sizeof(x));
         x.part_ml = reinterpret_cast<float *>(ws + off_ml);
@@ -1602,10 +1633,19 @@ int run_decode_prefix(brk_ctx *ctx, const brk_kv *prefix, int prefix_seq, int pr
         pdl = true;
     }
 
-    brk::DecodeArgs a;
+    brk::OwnArgs a;
     memset(&a, 0, sizeof(a));
-    a.with_prefix = 1;
-    a.late_wait = keys > 0;
+    a.late_wait = parts > 0;
+    if (together) {
+        const size_t seg0 = ((size_t)layer * prefix->desc.batch + prefix_seq) * Hkv;
+        a.tm_pre_k = prefix->tm_dec_k, a.tm_pre_v = prefix->tm_dec_v, a.tm_pre_s = prefix->tm_dec_s;
+        a.pre_tiles = pre_tiles;
+        a.pre_k0 = k_begin;
+        a.pre_row0 = (int)(seg0 * prefix->cap), a.pre_head_rows = prefix->cap;
+        a.pre_scale_row = (int)(seg0 * 2);
+        a.tiles_per_split = tps_together;
+        a.cluster = cluster;
+    }
     a.merge_here = merge_here;
     a.pre_parts = parts;
     a.pre_ml = reinterpret_cast<const float *>(ws + off_ml);
@@ -1629,8 +1669,8 @@ int run_decode_prefix(brk_ctx *ctx, const brk_kv *prefix, int prefix_seq, int pr
     a.part_ml = reinterpret_cast<float *>(ws + off_sml);
     a.part_o = reinterpret_cast<float *>(ws + off_so);
     for (int b = 0; b < batch; ++b) a.past_len[b] = past_len[b];
-    cudaError_t e = brk::launch_decode(kv->q8(), D, kv->tm_dec_k, kv->tm_dec_v, kv->q8() ? kv->tm_dec_s : kv->tm_dec_k,
-                                       a, nsplit, Hkv * mtiles, batch, st, pdl);
+    cudaError_t e = brk::launch_own_rows(kv->q8(), D, kv->tm_dec_k, kv->tm_dec_v,
+                                         kv->q8() ? kv->tm_dec_s : kv->tm_dec_k, a, nsplit, Hkv * mtiles, batch, st, pdl);
     if (e != cudaSuccess) return cuda_fail(e, "decode kernel launch");
     ++ctx->launches;
     if (merge_here) return BRK_OK;

@@ -258,6 +258,25 @@ __device__ __forceinline__ void patch_new_row(uint8_t *st, int rpos, const uint8
     }
 }
 
+// Two int8 codes as an fp16 pair, biased by 1152 (the bias comes off the sums) or, EXACT, as they are.
+template <bool EXACT>
+__device__ __forceinline__ uint32_t codes_half2(uint32_t w, uint32_t sel) {
+    const uint32_t b = codes_biased_half2(w, sel);
+    if constexpr (!EXACT) return b;
+    const __half2 x = __hsub2(*reinterpret_cast<const __half2 *>(&b), __floats2half2_rn(kCodeBias, kCodeBias));
+    return *reinterpret_cast<const uint32_t *>(&x);
+}
+
+// The argument block of a kernel form.
+template <bool H>
+struct DecodeArgsOf {
+    using type = DecodeArgs;
+};
+template <>
+struct DecodeArgsOf<true> {
+    using type = OwnArgs;
+};
+
 // F: the fused-append form (brk_attn_step with one token); a separate instantiation, so that the
 // plain kernel's code and registers stay as they are.  H: the own rows of sequences that share a
 // prefix (brk_attn_decode_prefix): q in fp16, and the final merge takes the prefix kernel's
@@ -266,7 +285,7 @@ __device__ __forceinline__ void patch_new_row(uint8_t *st, int rpos, const uint8
 template <bool Q8, int D, bool F, bool H = false>
 __global__ void __launch_bounds__(decode_threads<Q8, D, F>(), DecodeCfg<Q8, D>::kMinBlocks)
     decode_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
-                   const __grid_constant__ CUtensorMap tms, const __grid_constant__ DecodeArgs a) {
+                   const __grid_constant__ CUtensorMap tms, const __grid_constant__ typename DecodeArgsOf<H>::type a) {
     using L = DecodeLayout<Q8, D>;
     constexpr int S = DecodeCfg<Q8, D>::kStages;
     constexpr int DS = L::kDS;
@@ -303,8 +322,34 @@ __global__ void __launch_bounds__(decode_threads<Q8, D, F>(), DecodeCfg<Q8, D>::
 
     // Key range; for int8 a window's first key is rounded down to a multiple of 4 (16-byte scale
     // boxes) -- the extra keys are below every row's window and masked.
-    const KeyRange kr = decode_key_range(a, past, row0, nrows, split, SK, Q8 ? 4 : 1, kRT);
-    const int k_begin = kr.k_begin, k_end = kr.k_end, ntiles = kr.ntiles;
+    int range = split;  // of the own rows
+    if constexpr (H)
+        if (a.pre_tiles) range = 0;
+    const KeyRange kr = decode_key_range(a, past, row0, nrows, range, SK, Q8 ? 4 : 1, kRT);
+    const int k_begin = kr.k_begin, k_end = kr.k_end;
+    int ntiles = kr.ntiles;
+    // H with the prefix read here too (a.pre_tiles): the splits share out the prefix's tiles followed by
+    // the own rows' (k_begin .. k_end, one range); keys count from the first own row, the prefix's below
+    // zero.  Tile i's first key and the end of its rows:
+    int t0 = 0, npt = 0;
+    if constexpr (H) {
+        if (a.pre_tiles) {
+            npt = a.pre_tiles;
+            t0 = split * a.tiles_per_split;
+            ntiles = max(0, min(npt + kr.ntiles, t0 + a.tiles_per_split) - t0);
+        }
+    }
+    auto tile_key = [&](int i) {
+        if constexpr (H) {
+            if (t0 + i < npt) return a.pre_k0 - a.kv_offset + (t0 + i) * SK;
+            return k_begin + (t0 + i - npt) * SK;
+        }
+        return k_begin + i * SK;
+    };
+    auto tile_end = [&](int i) {
+        if constexpr (H) return t0 + i < npt ? 0 : k_end;
+        return k_end;
+    };
     const int seg = (a.layer * a.B + b) * a.Hkv + kvh;
     // Fused append: this CTA writes the new token's K / V rows (cache row past - kv_offset) when
     // its key range holds them, before its ring loads that row.
@@ -339,7 +384,7 @@ __global__ void __launch_bounds__(decode_threads<Q8, D, F>(), DecodeCfg<Q8, D>::
         auto issue = [&](int i_end) {
             for (int i = issued; i < i_end && ok; ++i) {
                 const int s = i % S;
-                const int key = k_begin + i * SK;
+                const int key = tile_key(i);
                 if (i >= S && !mbar_wait(&empty[s], ((i / S) - 1) & 1, a.err, kErrSlotTimeout)) {
                     ok = false;
                     break;
@@ -347,6 +392,21 @@ __global__ void __launch_bounds__(decode_threads<Q8, D, F>(), DecodeCfg<Q8, D>::
                 uint64_t *bar = i == rt ? rowbar : &full[s];
                 mbar_arrive_expect_tx(bar, L::kLoadBytes);
                 uint8_t *st = ring + s * L::kStageBytes;
+                if constexpr (H) {
+                    if (t0 + i < npt) {
+                        const int pk = key + a.kv_offset, py = a.pre_row0 + kvh * a.pre_head_rows + pk;
+#pragma unroll
+                        for (int j = 0; j < L::kBoxes; ++j)
+                            tma_load_2d(st + j * L::kBoxBytes, &a.tm_pre_k, j * L::kBoxElems, py, bar);
+#pragma unroll
+                        for (int j = 0; j < L::kBoxes; ++j)
+                            tma_load_2d(st + L::kTileBytes + j * L::kBoxBytes, &a.tm_pre_v, j * L::kBoxElems, py, bar);
+                        if constexpr (Q8)
+                            tma_load_2d(st + 2 * L::kTileBytes, &a.tm_pre_s, pk, a.pre_scale_row + kvh * 2, bar);
+                        issued = i + 1;
+                        continue;
+                    }
+                }
                 const int y = seg * a.cap + key;
 #pragma unroll
                 for (int j = 0; j < L::kBoxes; ++j) tma_load_2d(st + j * L::kBoxBytes, &tmk, j * L::kBoxElems, y, bar);
@@ -377,7 +437,7 @@ __global__ void __launch_bounds__(decode_threads<Q8, D, F>(), DecodeCfg<Q8, D>::
             // finished; cache rows (and the fused append's inputs) may come from it or, as kernels
             // that trigger their dependents early wait for their own predecessors before they
             // finish, from anything the stream ran before.  The CTA's set-up has overlapped it.
-            if (!H || !a.late_wait) griddep_wait();
+            if (!waits_late(a)) griddep_wait();
             if constexpr (F && !kRowWarp) {
                 if (writes_row) {
                     // The first ring stages (the new row's among them, unpatched, if it is that
@@ -430,7 +490,7 @@ __global__ void __launch_bounds__(decode_threads<Q8, D, F>(), DecodeCfg<Q8, D>::
         }
     }
 
-    if (!H || !a.late_wait) griddep_wait();  // q (or, fused, q_in / k_in / v_in) may come from the preceding kernel
+    if (!waits_late(a)) griddep_wait();  // q (or, fused, q_in / k_in / v_in) may come from the preceding kernel
     const int kg = warp % KG;  // key group: keys [16 kg, 16 kg + 16) of every stage
     const int dh = warp / KG;  // head-dim slice [DH dh, DH dh + DH)
     const int qr = lane >> 2, qc = lane & 3;
@@ -536,7 +596,7 @@ __global__ void __launch_bounds__(decode_threads<Q8, D, F>(), DecodeCfg<Q8, D>::
     // int8: 1152 * (sum of the fp16 q over this slice) for rows 2qc, 2qc + 1 -- the bias of the
     // raw scores against biased codes.
     float qbias[2] = {0.f, 0.f};
-    if constexpr (Q8) {
+    if constexpr (Q8 && !H) {
         float part = 0.f;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
@@ -561,7 +621,7 @@ __global__ void __launch_bounds__(decode_threads<Q8, D, F>(), DecodeCfg<Q8, D>::
     const bool use_cap = a.softcap > 0.f;
     // Keys every valid row of the tile attends: [kin_lo, kin_hi).
     const int t_first = row0 / G, t_last = (min(row0 + kRT, nrows) - 1) / G;
-    const int kin_hi = min(k_end, past + t_first + 1 - a.kv_offset);
+    const int kin_all = past + t_first + 1 - a.kv_offset;
     const int kin_lo = a.window > 0 ? past + t_last - a.window + 1 - a.kv_offset : INT_MIN;
 
     float o[MT][4];
@@ -576,7 +636,7 @@ __global__ void __launch_bounds__(decode_threads<Q8, D, F>(), DecodeCfg<Q8, D>::
         if (!mbar_wait(&full[s], (i / S) & 1, a.err, kErrTmaTimeout)) break;
         uint8_t *kt = ring + s * L::kStageBytes;
         uint8_t *vt = kt + L::kTileBytes;
-        const int key0 = k_begin + i * SK + kg * 16;
+        const int key0 = tile_key(i) + kg * 16, end = tile_end(i), kin_hi = min(end, kin_all);
 
         // ---- S^T = K Q^T for the warp's 16 keys over its head-dim slice (two accumulators, even
         // and odd k-steps, to halve the dependent MMA chain).
@@ -603,11 +663,10 @@ __global__ void __launch_bounds__(decode_threads<Q8, D, F>(), DecodeCfg<Q8, D>::
             }
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks)
-                mma_16816(sacc2[ks & 1], codes_biased_half2(wa[ks], 0x4140u), codes_biased_half2(wb[ks], 0x4140u),
-                          codes_biased_half2(wa[ks], 0x4342u), codes_biased_half2(wb[ks], 0x4342u), qf[ks][0],
-                          qf[ks][1]);
+                mma_16816(sacc2[ks & 1], codes_half2<H>(wa[ks], 0x4140u), codes_half2<H>(wb[ks], 0x4140u),
+                          codes_half2<H>(wa[ks], 0x4342u), codes_half2<H>(wb[ks], 0x4342u), qf[ks][0], qf[ks][1]);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sacc[e] = (sacc2[0][e] + sacc2[1][e]) - qbias[e & 1];
+            for (int e = 0; e < 4; ++e) sacc[e] = (sacc2[0][e] + sacc2[1][e]) - (H ? 0.f : qbias[e & 1]);
         } else {
             const int krow = kg * 16 + (lane & 15);
 #pragma unroll
@@ -662,7 +721,7 @@ __global__ void __launch_bounds__(decode_threads<Q8, D, F>(), DecodeCfg<Q8, D>::
             for (int e = 0; e < 4; ++e) {
                 const int key = key0 + qr + (e >> 1) * 8;
                 const int j = e & 1;  // row 2qc + j
-                valid[e] = key >= lo[j] && key <= hi[j] && key < k_end;
+                valid[e] = key >= lo[j] && key <= hi[j] && key < end;
                 sacc[e] = valid[e] ? sacc[e] : -CUDART_INF_F;
             }
         }
@@ -705,7 +764,7 @@ __global__ void __launch_bounds__(decode_threads<Q8, D, F>(), DecodeCfg<Q8, D>::
             if constexpr (Q8) p[e] = valid[e] ? p[e] * vsc[e >> 1] : 0.f;
         }
         const uint32_t pt0 = pack_half2(p[0], p[1]), pt1 = pack_half2(p[2], p[3]);
-        if constexpr (Q8) {
+        if constexpr (Q8 && !H) {
             // The fp16 p' the tensor cores see, per row: the bias 1152 * sum(p') of the outputs.
             const float2 f0 = __half22float2(*reinterpret_cast<const __half2 *>(&pt0));
             const float2 f1 = __half22float2(*reinterpret_cast<const __half2 *>(&pt1));
@@ -738,17 +797,17 @@ __global__ void __launch_bounds__(decode_threads<Q8, D, F>(), DecodeCfg<Q8, D>::
                 // lo, t = 2, 3 in hi.  m-tile 2g+u takes bytes 4g+2u (its row qr) and 4g+2u+1 (row qr+8).
                 const uint32_t lo01 = prmt(vw[0][g], vw[1][g], 0x5140u), hi01 = prmt(vw[0][g], vw[1][g], 0x7362u);
                 const uint32_t lo23 = prmt(vw[2][g], vw[3][g], 0x5140u), hi23 = prmt(vw[2][g], vw[3][g], 0x7362u);
-                mma_16816(o[2 * g], codes_biased_half2(lo01, 0x4140u), codes_biased_half2(lo01, 0x4342u),
-                          codes_biased_half2(lo23, 0x4140u), codes_biased_half2(lo23, 0x4342u), pb0, pb1);
-                mma_16816(o[2 * g + 1], codes_biased_half2(hi01, 0x4140u), codes_biased_half2(hi01, 0x4342u),
-                          codes_biased_half2(hi23, 0x4140u), codes_biased_half2(hi23, 0x4342u), pb0, pb1);
+                mma_16816(o[2 * g], codes_half2<H>(lo01, 0x4140u), codes_half2<H>(lo01, 0x4342u),
+                          codes_half2<H>(lo23, 0x4140u), codes_half2<H>(lo23, 0x4342u), pb0, pb1);
+                mma_16816(o[2 * g + 1], codes_half2<H>(hi01, 0x4140u), codes_half2<H>(hi01, 0x4342u),
+                          codes_half2<H>(hi23, 0x4140u), codes_half2<H>(hi23, 0x4342u), pb0, pb1);
             }
         } else {
             // Keys past the range end get zero V (in this warp's slice), so that 0 * (whatever
             // the tile holds there) stays 0.
-            const bool tail = key0 + 16 > k_end;
+            const bool tail = key0 + 16 > end;
             if (tail) {
-                const int first = max(k_end - key0, 0);
+                const int first = max(end - key0, 0);
                 for (int idx = lane; idx < (16 - first) * (DH / 8); idx += 32) {
                     const int rl = first + idx / (DH / 8), ch = dh * (DH / 8) + idx % (DH / 8);
                     *reinterpret_cast<uint4 *>(vt + (ch >> 3) * L::kBoxBytes + sw128(kg * 16 + rl, ch & 7)) =
@@ -788,7 +847,7 @@ __global__ void __launch_bounds__(decode_threads<Q8, D, F>(), DecodeCfg<Q8, D>::
             psum[j] += __shfl_xor_sync(0xffffffffu, psum[j], 16);
         }
     }
-    if constexpr (Q8) {
+    if constexpr (Q8 && !H) {
         // Remove the code bias: O^T[d][row] -= 1152 * sum of the row's p'.
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
@@ -828,7 +887,9 @@ __global__ void __launch_bounds__(decode_threads<Q8, D, F>(), DecodeCfg<Q8, D>::
     named_barrier_sync(1, NC * 32);
 
     if constexpr (H) {
-        if (a.merge_here)
+        if (a.cluster)
+            decode_epilogue_cluster<D, KG, NC, kRT>(a, ring, row0, nrows, kvh, b, split);
+        else if (a.merge_here)
             decode_epilogue_merge<D, KG, NC, kRT>(a, ring, row0, nrows, kvh, mtile, b, split);
         else
             decode_epilogue_prefix<D, KG, NC, kRT>(a, ring, row0, nrows, kvh, b, split);
@@ -906,7 +967,8 @@ __global__ void combine_peers_kernel(const __grid_constant__ CombineArgs a, cons
 }
 
 template <bool Q8, int D, bool F, bool H = false>
-cudaError_t launch_t(const CUtensorMap &tmk, const CUtensorMap &tmv, const CUtensorMap &tms, const DecodeArgs &a,
+cudaError_t launch_t(const CUtensorMap &tmk, const CUtensorMap &tmv, const CUtensorMap &tms,
+                     const typename DecodeArgsOf<H>::type &a,
                       dim3 grid, cudaStream_t s, bool pdl) {
     static unsigned long long configured = 0;  // one bit per device: the opt-in is per device
     int dev = 0;
@@ -944,9 +1006,6 @@ cudaError_t launch_t(const CUtensorMap &tmk, const CUtensorMap &tmv, const CUten
 template <int D>
 cudaError_t launch_dt(bool q8, bool fused, const CUtensorMap &tmk, const CUtensorMap &tmv, const CUtensorMap &tms,
                       const DecodeArgs &a, dim3 grid, cudaStream_t s, bool pdl) {
-    if (a.with_prefix)
-        return q8 ? launch_t<true, D, false, true>(tmk, tmv, tms, a, grid, s, pdl)
-                  : launch_t<false, D, false, true>(tmk, tmv, tms, a, grid, s, pdl);
     if (q8) return fused ? launch_t<true, D, true>(tmk, tmv, tms, a, grid, s, pdl)
                          : launch_t<true, D, false>(tmk, tmv, tms, a, grid, s, pdl);
     return fused ? launch_t<false, D, true>(tmk, tmv, tms, a, grid, s, pdl)
@@ -1050,6 +1109,21 @@ cudaError_t launch_decode(bool q8, int head_dim, const CUtensorMap &tmk, const C
         case 64: return launch_dt<64>(q8, a.fuse != 0, tmk, tmv, tms, a, grid, s, pdl);
         case 128: return launch_dt<128>(q8, a.fuse != 0, tmk, tmv, tms, a, grid, s, pdl);
         case 256: return launch_dt<256>(q8, a.fuse != 0, tmk, tmv, tms, a, grid, s, pdl);
+        default: return cudaErrorInvalidValue;
+    }
+}
+
+cudaError_t launch_own_rows(bool q8, int head_dim, const CUtensorMap &tmk, const CUtensorMap &tmv,
+                            const CUtensorMap &tms, const OwnArgs &a, int grid_x, int grid_y, int grid_z, cudaStream_t s,
+                            bool pdl) {
+    const dim3 grid(grid_x, grid_y, grid_z);
+    switch (head_dim) {
+        case 64: return q8 ? launch_t<true, 64, false, true>(tmk, tmv, tms, a, grid, s, pdl)
+                           : launch_t<false, 64, false, true>(tmk, tmv, tms, a, grid, s, pdl);
+        case 128: return q8 ? launch_t<true, 128, false, true>(tmk, tmv, tms, a, grid, s, pdl)
+                            : launch_t<false, 128, false, true>(tmk, tmv, tms, a, grid, s, pdl);
+        case 256: return q8 ? launch_t<true, 256, false, true>(tmk, tmv, tms, a, grid, s, pdl)
+                            : launch_t<false, 256, false, true>(tmk, tmv, tms, a, grid, s, pdl);
         default: return cudaErrorInvalidValue;
     }
 }

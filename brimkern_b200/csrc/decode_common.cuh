@@ -12,6 +12,10 @@ namespace brk {
 
 constexpr float kLn2 = 0.6931471805599453f;
 
+// Whether the kernel waits for the preceding one only at its end (OwnArgs).
+__device__ __forceinline__ bool waits_late(const DecodeArgs &) { return false; }
+__device__ __forceinline__ bool waits_late(const OwnArgs &a) { return a.late_wait; }
+
 // Cache rows [k_begin, k_end) that one CTA attends, in stage-sized tiles.  Token t of the CTA's
 // rows attends [pos_t - W + 1, pos_t] (W <= 0: from 0).  `align` rounds the window's first key
 // down (the int8 kernel loads scales in 16-byte boxes); keys below a row's own limit are masked.
@@ -204,7 +208,7 @@ __device__ __forceinline__ void decode_epilogue(const DecodeArgs &a, uint8_t *ri
 // pre_parts partials of that row and writes the final output, f32 or fp16; a CTA waits for that kernel
 // only here.  For grids that are resident all at once.
 template <int D, int KG, int NC, int RT>
-__device__ __forceinline__ void decode_epilogue_merge(const DecodeArgs &a, uint8_t *ring, int row0, int nrows, int kvh,
+__device__ __forceinline__ void decode_epilogue_merge(const OwnArgs &a, uint8_t *ring, int row0, int nrows, int kvh,
                                                        int mt, int b, int split) {
     float *cm = reinterpret_cast<float *>(ring);
     float *cl = cm + KG * RT;
@@ -336,7 +340,7 @@ __device__ __forceinline__ void decode_epilogue_merge(const DecodeArgs &a, uint8
 // the CTA's partial goes out as it is, and prefix_merge_kernel joins it with the other splits' and the
 // prefix's.
 template <int D, int KG, int NC, int RT>
-__device__ __forceinline__ void decode_epilogue_prefix(const DecodeArgs &a, uint8_t *ring, int row0, int nrows, int kvh,
+__device__ __forceinline__ void decode_epilogue_prefix(const OwnArgs &a, uint8_t *ring, int row0, int nrows, int kvh,
                                                        int b, int split) {
     const float *cm = reinterpret_cast<const float *>(ring);
     const float *cl = cm + KG * RT;
@@ -376,8 +380,18 @@ __device__ __forceinline__ void decode_epilogue_prefix(const DecodeArgs &a, uint
 // until the last remote read.  No global partials, no fences or arrival counters, and the merge
 // is spread over the cluster instead of falling to one last CTA.  Called by the NC consumer
 // warps; the producer warp takes the two cluster barriers on its own (decode_cluster_idle).
-template <int D, int KG, int NC, int RT>
-__device__ __forceinline__ void decode_epilogue_cluster(const DecodeArgs &a, uint8_t *ring, int row0, int nrows,
+__device__ __forceinline__ bool has_out(const DecodeArgs &a) { return a.out != nullptr; }
+__device__ __forceinline__ void store_out(const DecodeArgs &a, size_t i, float v) { a.out[i] = v; }
+__device__ __forceinline__ bool has_out(const OwnArgs &a) { return true; }
+__device__ __forceinline__ void store_out(const OwnArgs &a, size_t i, float v) {
+    if (a.out16)
+        a.out16[i] = __float2half_rn(v);
+    else
+        a.out[i] = v;
+}
+
+template <int D, int KG, int NC, int RT, typename Args>
+__device__ __forceinline__ void decode_epilogue_cluster(const Args &a, uint8_t *ring, int row0, int nrows,
                                                         int kvh, int b, int split) {
     const float *cm = reinterpret_cast<const float *>(ring);
     const float *cl = cm + KG * RT;
@@ -442,8 +456,8 @@ __device__ __forceinline__ void decode_epilogue_cluster(const DecodeArgs &a, uin
         }
         const int rr = row0 + r;
         const size_t R = ((size_t)b * T + rr / G) * a.Hq + kvh * G + rr % G;
-        if (a.out) {
-            a.out[R * D + d] = O / Lsum;
+        if (has_out(a)) {
+            store_out(a, R * D + d, O / Lsum);
         } else {
             a.res_o[R * D + d] = O;
             if (d == 0) {

@@ -165,19 +165,25 @@ struct DecodeArgs {
     const float *q_norm, *k_norm;
     double eps;
     int one_plus;
-    // Own rows of sequences that share a prefix (brk_attn_decode_prefix, decode_kernel's H form):
-    // q in fp16 (replaces q); whether the preceding kernel is the prefix kernel, which has to be
-    // waited for only before its partials are read; merge_here: the prefix kernel's pre_parts
-    // partials [part][rows][2], [part][rows][D] are merged in and the output (fp16 out16, or out)
-    // written here, else the partials [split][rows] at part_ml / part_o.
-    int with_prefix;
+    int past_len[BRK_MAX_BATCH];
+};
+
+// Own rows of sequences that share a prefix (brk_attn_decode_prefix, decode_kernel's H form): q in fp16
+// (replaces q); whether the preceding kernel is the prefix kernel, which has to be waited for only
+// before its partials are read; merge_here: the prefix kernel's pre_parts partials [part][rows][2],
+// [part][rows][D] are merged in and the output (fp16 out16, or out) written here, else the partials
+// [split][rows] at part_ml / part_o.  pre_tiles: the prefix is read here too, as that many stages of
+// keys from pre_k0 on (kv head 0's key 0 at map row pre_row0, a kv head pre_head_rows rows) before the
+// own rows' stages, tiles_per_split of both together to a split.
+struct OwnArgs : DecodeArgs {
+    CUtensorMap tm_pre_k, tm_pre_v, tm_pre_s;
     int late_wait;
     int merge_here;
     int pre_parts;
+    int pre_tiles, pre_k0, pre_row0, pre_head_rows, pre_scale_row, tiles_per_split;
     const __half *q16;
     const float *pre_ml, *pre_o;
     __half *out16;
-    int past_len[BRK_MAX_BATCH];
 };
 
 // Attention of every sequence's query rows over one shared prefix (prefix.cu): partials only.
@@ -301,6 +307,10 @@ cudaError_t launch_append(const AppendArgs &a, cudaStream_t s, bool pdl);
 cudaError_t launch_decode(bool q8, int head_dim, const CUtensorMap &tmk, const CUtensorMap &tmv,
                           const CUtensorMap &tms, const DecodeArgs &a, int grid_x, int grid_y, int grid_z,
                           cudaStream_t s, bool pdl);
+// Its form for the own rows of sequences that share a prefix.
+cudaError_t launch_own_rows(bool q8, int head_dim, const CUtensorMap &tmk, const CUtensorMap &tmv,
+                            const CUtensorMap &tms, const OwnArgs &a, int grid_x, int grid_y, int grid_z, cudaStream_t s,
+                            bool pdl);
 int decode_rows_per_tile();
 // How many clusters of `size` decode CTAs fit on the GPU at once (0: clusters of that size cannot
 // be launched).
