@@ -135,6 +135,22 @@ __device__ __forceinline__ float apply_act(float v) {
     return v;
 }
 
+// v[e] at out[e * n], e < count.  (A test per element is a branch each: 75 cycles a value and warp, 25
+// without.)
+__device__ __forceinline__ void store_as(__half *p, float v) { *p = __float2half_rn(v); }
+__device__ __forceinline__ void store_as(float *p, float v) { *p = v; }
+template <int CH, typename T>
+__device__ __forceinline__ void store_column(T *out, size_t n, int count, const float (&v)[CH]) {
+    if (count >= CH) {
+#pragma unroll
+        for (int e = 0; e < CH; ++e, out += n) store_as(out, v[e]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < CH; ++e)
+            if (e < count) store_as(out + e * n, v[e]);
+    }
+}
+
 // The finished values of one feature for CH tokens, at out[o + e * n] (e < count): act(v + b0)
 // * (w + b1) when GATED, else act(v + b0) + res.
 template <int ACT, bool GATED, int CH>
@@ -147,17 +163,10 @@ __device__ __forceinline__ void finish_act(const LinearArgs &a, size_t o, int co
         const float x = apply_act<ACT>(v[e] + b0);
         y[e] = GATED ? x * (w[e] + b1) : x + w[e];
     }
-    if (a.out_half) {
-        __half *out = static_cast<__half *>(a.out) + o;
-#pragma unroll
-        for (int e = 0; e < CH; ++e)
-            if (e < count) out[e * n] = __float2half_rn(y[e]);
-    } else {
-        float *out = static_cast<float *>(a.out) + o;
-#pragma unroll
-        for (int e = 0; e < CH; ++e)
-            if (e < count) out[e * n] = y[e];
-    }
+    if (a.out_half)
+        store_column<CH>(static_cast<__half *>(a.out) + o, n, count, y);
+    else
+        store_column<CH>(static_cast<float *>(a.out) + o, n, count, y);
 }
 template <bool GATED, int CH>
 __device__ __forceinline__ void finish(const LinearArgs &a, size_t o, int count, float b0, float b1, const float (&v)[CH],
@@ -488,16 +497,22 @@ __global__ void __launch_bounds__(LinearLayout<NT, MODE, PAIR>::kThreads, 1)
             const int m0 = p.mtile * nt + col0;                    // token of this thread's first column
             const int ntok = idle ? 0 : min(min(a.half_cols, nt - col0), a.M - m0);  // columns that count (may be <= 0)
             const bool whole = cs > 1 || (k0 == 0 && k1 == a.nk);
-            // A partial tile: [matrix][token / 4][128 lanes][4].
-            const size_t slot_floats = (size_t)MATS * nt * kLF;
+            // A partial tile: [matrix][token / 4][128 lanes][4], in whole chunks (nt is a multiple of 16;
+            // what a last chunk of 32 has past it is never used).
+            const size_t slot_floats = (size_t)(MATS * nt + (CH == 32 ? 16 : 0)) * kLF;
             const bool in = r < F && feat < a.n;
             const float b0 = in && a.bias[0] ? a.bias[0][feat] : 0.f;
             const float b1 = GATED && in && a.bias[1] ? a.bias[1][feat] : 0.f;
             const size_t o0 = (size_t)m0 * a.n + feat;
             auto load_res = [&](int c0, float (&res)[CH]) {
                 const float *src = a.residual + o0 + (size_t)c0 * a.n;
+                if (in && c0 + CH <= ntok) {
 #pragma unroll
-                for (int e = 0; e < CH; ++e) res[e] = in && c0 + e < ntok ? src[(size_t)e * a.n] : 0.f;
+                    for (int e = 0; e < CH; ++e, src += a.n) res[e] = *src;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < CH; ++e) res[e] = in && c0 + e < ntok ? src[(size_t)e * a.n] : 0.f;
+                }
             };
             const bool has_res = !GATED && a.residual;
             float res[CH];
@@ -578,12 +593,11 @@ __global__ void __launch_bounds__(LinearLayout<NT, MODE, PAIR>::kThreads, 1)
                 if constexpr (MATS == 2) ld_cols(buf * L::kCols + NT + col0 + c0, wr);
                 tc_wait_ld();
                 if (cs > 1) {
-                    // This CTA's part [matrix][token / 4][128 lanes][4], in the ring (its copies and the
-                    // products that read them are complete).
+                    // This CTA's part [matrix][token / 4][128 lanes][4], in whole chunks, in the ring (its
+                    // copies and the products that read them are complete).
                     float *dst = reinterpret_cast<float *>(smem) + (size_t)(col0 + c0) * kLF + lrow * 4;
 #pragma unroll
                     for (int e = 0; e < CH; e += 4) {
-                        if (c0 + e >= ntok) break;
                         *reinterpret_cast<uint4 *>(dst + e * kLF) = make_uint4(vr[e], vr[e + 1], vr[e + 2], vr[e + 3]);
                         if constexpr (MATS == 2)
                             *reinterpret_cast<uint4 *>(dst + (size_t)nt * kLF + e * kLF) =
@@ -600,21 +614,29 @@ __global__ void __launch_bounds__(LinearLayout<NT, MODE, PAIR>::kThreads, 1)
                             for (int e = 0; e < CH; ++e) sum[m][e] = 0.f;
 #pragma unroll 1
                         for (int q = c_first; q <= c_last; ++q) {
+                            if (q == worker) {
+#pragma unroll
+                                for (int e = 0; e < CH; ++e) {
+                                    sum[0][e] += __uint_as_float(vr[e]);
+                                    if constexpr (MATS == 2) sum[MATS - 1][e] += __uint_as_float(wr[e]);
+                                }
+                                continue;
+                            }
                             const int slot = range_begin(a, q) >= t0 ? 0 : 1;
                             const float *src = a.ws + ((size_t)(q * CTAS + rank) * 2 + slot) * slot_floats +
                                                (size_t)(col0 + c0) * kLF + lrow * 4;
+                            float4 x[MATS][CH / 4];
 #pragma unroll
                             for (int m = 0; m < MATS; ++m)
 #pragma unroll
-                                for (int e = 0; e < CH; e += 4) {
-                                    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-                                    if (q != worker && c0 + e < ntok)
-                                        x = __ldcg(reinterpret_cast<const float4 *>(src + (size_t)(m * nt + e) * kLF));
-                                    const uint32_t(&own)[CH] = m ? wr : vr;
-                                    sum[m][e] += q == worker ? __uint_as_float(own[e]) : x.x;
-                                    sum[m][e + 1] += q == worker ? __uint_as_float(own[e + 1]) : x.y;
-                                    sum[m][e + 2] += q == worker ? __uint_as_float(own[e + 2]) : x.z;
-                                    sum[m][e + 3] += q == worker ? __uint_as_float(own[e + 3]) : x.w;
+                                for (int e = 0; e < CH / 4; ++e)
+                                    x[m][e] = __ldcg(reinterpret_cast<const float4 *>(src + (size_t)(m * nt + 4 * e) * kLF));
+#pragma unroll
+                            for (int m = 0; m < MATS; ++m)
+#pragma unroll
+                                for (int e = 0; e < CH / 4; ++e) {
+                                    sum[m][4 * e] += x[m][e].x, sum[m][4 * e + 1] += x[m][e].y;
+                                    sum[m][4 * e + 2] += x[m][e].z, sum[m][4 * e + 3] += x[m][e].w;
                                 }
                         }
 #pragma unroll
@@ -656,7 +678,6 @@ __global__ void __launch_bounds__(LinearLayout<NT, MODE, PAIR>::kThreads, 1)
                 } else {
 #pragma unroll
                     for (int e = 0; e < CH; e += 4) {
-                        if (c0 + e >= ntok) break;
                         float *dst = part + (size_t)(c0 + e) * kLF;
                         __stcg(reinterpret_cast<uint4 *>(dst), make_uint4(vr[e], vr[e + 1], vr[e + 2], vr[e + 3]));
                         if constexpr (MATS == 2)
@@ -700,22 +721,21 @@ __global__ void __launch_bounds__(LinearLayout<NT, MODE, PAIR>::kThreads, 1)
                             float4 x[2][GATED ? 2 : 1][CH / 4];
 #pragma unroll
                             for (int h = 0; h < 2; ++h) {
-                                const bool there = q + h <= c_last;
+                                if (q + h > c_last) break;
                                 const int slot = range_begin(a, q + h) >= t0 ? 0 : 1;
                                 const float *src = a.ws + ((size_t)((q + h) * CTAS + rank) * 2 + slot) * slot_floats +
                                                    (size_t)(col0 + c0) * kLF + r * 4;
                                 const size_t other = MODE == kInterleaved ? 64 * 4 : (size_t)nt * kLF;
 #pragma unroll
                                 for (int e = 0; e < CH / 4; ++e) {
-                                    const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
-                                    x[h][0][e] = there && c0 + 4 * e < ntok ? __ldcg(reinterpret_cast<const float4 *>(src + e * 4 * kLF)) : zero;
+                                    x[h][0][e] = __ldcg(reinterpret_cast<const float4 *>(src + e * 4 * kLF));
                                     if constexpr (GATED)
-                                        x[h][1][e] =
-                                            there && c0 + 4 * e < ntok ? __ldcg(reinterpret_cast<const float4 *>(src + other + e * 4 * kLF)) : zero;
+                                        x[h][1][e] = __ldcg(reinterpret_cast<const float4 *>(src + other + e * 4 * kLF));
                                 }
                             }
 #pragma unroll
-                            for (int h = 0; h < 2; ++h)
+                            for (int h = 0; h < 2; ++h) {
+                                if (q + h > c_last) break;
 #pragma unroll
                                 for (int e = 0; e < CH / 4; ++e) {
                                     v[4 * e] += x[h][0][e].x, v[4 * e + 1] += x[h][0][e].y;
@@ -725,6 +745,7 @@ __global__ void __launch_bounds__(LinearLayout<NT, MODE, PAIR>::kThreads, 1)
                                         w[4 * e + 2] += x[h][1][e].z, w[4 * e + 3] += x[h][1][e].w;
                                     }
                                 }
+                            }
                         }
                         if (in) finish<GATED, CH>(a, o0 + (size_t)c0 * a.n, ntok - c0, b0, b1, v, w);
                     }
@@ -1073,7 +1094,7 @@ LinearPlan linear_plan(int rows, int k, int n, int mats, int sms) {
     const long long units = (p.tiles - p.tiles_whole) * p.nk;
     p.range_units = (int)(units / workers), p.range_extra = (int)(units % workers);
     p.counters = (size_t)(p.tiles - p.tiles_whole) * ctas;
-    p.ws_floats = p.tiles > p.tiles_whole ? (size_t)p.ctas * 2 * (p.pair ? 1 : mats) * p.nt * kLF : 0;
+    p.ws_floats = p.tiles > p.tiles_whole ? (size_t)p.ctas * 2 * ((p.pair ? 1 : mats) * p.nt + 16) * kLF : 0;
     return p;
 }
 
