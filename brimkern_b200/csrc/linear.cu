@@ -58,7 +58,6 @@ struct LinearLayout {
     static constexpr int kHalves = NT >= 64 ? 2 : 1;              // epilogue warps per TMEM lane quarter
     static constexpr int kEpiWarps = 4 * kHalves;
     static constexpr int kEpiCols = NT / kHalves;                 // most columns of an epilogue thread
-    static constexpr int kChunk = NT >= 64 && MODE == kLinear ? 32 : 16;  // columns handled at a time
     static constexpr int kProducer = kEpiWarps, kMma = kEpiWarps + 1;
     static constexpr int kThreads = (kEpiWarps + 2) * 32;
     static constexpr uint32_t kBarOff = kRing + kSlack;
@@ -261,7 +260,11 @@ __global__ void __launch_bounds__(LinearLayout<NT, MODE, PAIR>::kThreads, 1)
     linear_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap tw0,
                   const __grid_constant__ CUtensorMap tw1, const __grid_constant__ LinearArgs a) {
     using L = LinearLayout<NT, MODE, PAIR>;
-    constexpr int CTAS = L::kCtas, BUFS = L::kBufs, MATS = L::kMats, CH = L::kChunk;
+    constexpr int CTAS = L::kCtas, BUFS = L::kBufs, MATS = L::kMats;
+    // Columns handled at a time.  f32 outputs come with a residual's loads to hide: 32 (2048 x 2560 -> 10240
+    // 112 us, 124 with 16); fp16 outputs are bound by the epilogue's instructions, whose registers spill at
+    // 32 (3000 x 1024 -> 4096 31.5 us, 26.7 with 16).
+    constexpr int CH = DRAIN && NT >= 64 ? 32 : 16;
     constexpr int EPI = L::kEpiWarps * 32;
     constexpr bool GATED = MODE != kLinear;
     extern __shared__ uint8_t smem_raw[];
