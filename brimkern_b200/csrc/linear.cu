@@ -628,19 +628,24 @@ __global__ void __launch_bounds__(LinearLayout<NT, MODE, PAIR>::kThreads, 1)
                             const int slot = range_begin(a, q) >= t0 ? 0 : 1;
                             const float *src = a.ws + ((size_t)(q * CTAS + rank) * 2 + slot) * slot_floats +
                                                (size_t)(col0 + c0) * kLF + lrow * 4;
-                            float4 x[MATS][CH / 4];
+                            constexpr int XC = CH == 32 ? 16 : CH;  // at 32 the registers would spill
 #pragma unroll
-                            for (int m = 0; m < MATS; ++m)
+                            for (int h = 0; h < CH; h += XC) {
+                                float4 x[MATS][XC / 4];
 #pragma unroll
-                                for (int e = 0; e < CH / 4; ++e)
-                                    x[m][e] = __ldcg(reinterpret_cast<const float4 *>(src + (size_t)(m * nt + 4 * e) * kLF));
+                                for (int m = 0; m < MATS; ++m)
 #pragma unroll
-                            for (int m = 0; m < MATS; ++m)
+                                    for (int e = 0; e < XC / 4; ++e)
+                                        x[m][e] =
+                                            __ldcg(reinterpret_cast<const float4 *>(src + (size_t)(m * nt + h + 4 * e) * kLF));
 #pragma unroll
-                                for (int e = 0; e < CH / 4; ++e) {
-                                    sum[m][4 * e] += x[m][e].x, sum[m][4 * e + 1] += x[m][e].y;
-                                    sum[m][4 * e + 2] += x[m][e].z, sum[m][4 * e + 3] += x[m][e].w;
-                                }
+                                for (int m = 0; m < MATS; ++m)
+#pragma unroll
+                                    for (int e = 0; e < XC / 4; ++e) {
+                                        float *to = &sum[m][h + 4 * e];
+                                        to[0] += x[m][e].x, to[1] += x[m][e].y, to[2] += x[m][e].z, to[3] += x[m][e].w;
+                                    }
+                            }
                         }
 #pragma unroll
                         for (int e = 0; e < CH; ++e) {
