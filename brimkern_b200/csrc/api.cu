@@ -305,24 +305,27 @@ int ensure_counters(brk_ctx *ctx, size_t n) {
     return BRK_OK;
 }
 
-// The scratch of `stream`, or of the capture it is in: a workspace of at least `bytes` and
+// The scratch of `stream`, or of `stream` in the capture it is in: a workspace of at least `bytes` and
 // n_counters zeroed counters.  Growing keeps the old buffers (queued kernels and captured graphs
 // may still use them) and neither synchronises nor disturbs a capture: the allocation runs in
 // relaxed capture mode, and the counters are zeroed on a stream of the context's own.
 int get_scratch(brk_ctx *ctx, cudaStream_t stream, size_t bytes, size_t n_counters, brk_scratch **out) {
     cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
-    unsigned long long id = 0;
-    BRK_CUDA(cudaStreamGetCaptureInfo(stream, &st, &id));
+    unsigned long long id = 0, capture_id = 0;
+    BRK_CUDA(cudaStreamGetCaptureInfo(stream, &st, &capture_id));
     if (st == cudaStreamCaptureStatusInvalidated) return fail(BRK_ERR_CUDA, "the stream's capture is invalid");
     const bool capture = st == cudaStreamCaptureStatusActive;
-    if (!capture) BRK_CUDA(cudaStreamGetId(stream, &id));
+    if (capture)
+        id = reinterpret_cast<uintptr_t>(stream);  // the id may not be asked for in a capture
+    else
+        BRK_CUDA(cudaStreamGetId(stream, &id));
     brk_scratch *sc = nullptr;
     for (brk_scratch *x : ctx->scratch)
-        if (x->id == id && x->capture == capture) sc = x;
+        if (x->id == id && x->capture == capture && (!capture || x->capture_id == capture_id)) sc = x;
     if (!sc) {
         sc = new (std::nothrow) brk_scratch();
         if (!sc) return fail(BRK_ERR_CUDA, "out of host memory");
-        sc->id = id;
+        sc->id = id, sc->capture_id = capture_id;
         sc->capture = capture;
         try {
             ctx->scratch.push_back(sc);

@@ -18,7 +18,8 @@
 // streams, and graphs captured one by one, so never share it.  A buffer that has become too small
 // is kept until the context goes (queued kernels and captured graphs may still use it).
 struct brk_scratch {
-    unsigned long long id = 0;   // stream id, or capture id
+    unsigned long long id = 0;   // of the stream (capture: its handle)
+    unsigned long long capture_id = 0;
     bool capture = false;
     void *ws = nullptr;
     size_t ws_bytes = 0;

@@ -293,8 +293,9 @@ int brk_attn_combine(brk_ctx *ctx, int n_parts, int rows, int head_dim, const fl
  *   - q and out [batch][n_tokens][n_heads][head_dim], each f32 or fp16 by q_type / out_type (BRK_T_*),
  *     16-byte aligned, not overlapping.  n_tokens * (n_heads / n_kv_heads) <= 64.
  *   - Scratch (partials; for an int8 prefix its codes as fp16, 4 bytes per code of the attended
- *     rows of one layer) belongs to the stream, or to the stream capture, that the call is made on:
- *     calls on several streams, and graphs captured one after the other, may run at the same time.
+ *     rows of one layer) belongs to the stream, and to the stream capture, that the call is made on:
+ *     calls on several streams, graphs, and branches of a graph that were captured from several
+ *     streams, may run at the same time.
  *     It grows at the first call that needs more (also while capturing) and lives until
  *     brk_ctx_destroy, which must come after the last replay of such graphs. */
 int brk_attn_decode_prefix(brk_ctx *ctx, const brk_kv *prefix, int prefix_seq, int prefix_len, const brk_kv *kv,
@@ -311,7 +312,7 @@ int brk_attn_step_prefix(brk_ctx *ctx, const brk_kv *prefix, int prefix_seq, int
  * Weights are the engine's fp16 matrices [n][k] (C = A W^T), activations x fp16 [rows][k], biases
  * f32 [n] or NULL; sums in f32.  k is a multiple of 8, x and the weights 16-byte aligned; rows (0:
  * nothing is done) and n are any size.  Results do not change from run to run.  Scratch as for
- * brk_attn_decode_prefix: by stream or stream capture.  Outputs may not overlap inputs, except
+ * brk_attn_decode_prefix: by stream and stream capture.  Outputs may not overlap inputs, except
  * brk_linear's f32 out, which may be its residual.
  *   brk_linear:      out = act(x w^T + bias) + residual    (residual f32 [rows][n] or NULL)
  *                    out f32 or fp16 [rows][n] by out_type.

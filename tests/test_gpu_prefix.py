@@ -307,6 +307,45 @@ def test_captured_graphs_and_streams(eng, P):
     e.close()
 
 
+def test_branches_of_one_graph(eng):
+    """Calls captured on two streams of one capture become branches that may run at once: they share no
+    scratch either (prefix splits, split matrix products)."""
+    import torch
+    g = torch.Generator(device=eng.device).manual_seed(37)
+    Hq, Hkv, D, P, own = 32, 8, 128, 4000, [1500, 20, 700, 1]
+    prefix, kv = _fill(eng, g, Hkv, D, P, own, False, False)
+    cfg = _cfg(Hq, Hkv, D, P)
+    past = [P + n - 1 for n in own]
+    qs = [torch.randn((4, 1, Hq, D), generator=g, device=eng.device).half() for _ in range(2)]
+    x = [torch.randn((600, 2560), generator=g, device=eng.device).half() for _ in range(2)]
+    w = torch.randn((2560, 2560), generator=g, device=eng.device).half()
+    outs, ys = [torch.zeros_like(q) for q in qs], [torch.zeros_like(t) for t in x]
+
+    def work(i):
+        for _ in range(4):
+            eng.decodePrefix(prefix, P, kv, 0, cfg, qs[i], outs[i], past)
+            eng.linear(x[i], w, ys[i])
+    main, side = torch.cuda.Stream(), torch.cuda.Stream()
+    for i in range(2):
+        work(i)
+    torch.cuda.synchronize()
+    want = [t.clone() for t in outs + ys]
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr, stream=main):
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            work(1)
+        work(0)
+        main.wait_stream(side)
+    for _ in range(20):
+        for t in outs + ys:
+            t.zero_()
+        gr.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(t, v) for t, v in zip(outs + ys, want))
+    eng.ctx.check()
+
+
 def test_refusals(eng):
     """Calls the operator does not cover raise and launch nothing."""
     import torch
