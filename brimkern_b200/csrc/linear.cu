@@ -29,6 +29,12 @@
 // N(0,1) operands against 64 bits: 3.1e-6 of the result at k 2560, 1.2e-5 at 10240).  For f32
 // outputs (DRAIN) the accumulators are drained every 1024 of k and the parts added in registers;
 // fp16 outputs (half a step 4.9e-4) do not need it.
+//
+// Measured (calls replayed from a graph): gate-up 2560 -> 10240 of one token 18.9 us, 5.5 TB/s of
+// weights; of 64 tokens 25.4 us, bound by the stream and the exposed ramp and epilogue of one tile a
+// CTA; of 2048 tokens 160 us, 1340 TFLOP/s.  Linear 2048 x 10240 -> 2560 with a residual 113 us (f32)
+// and 92 (fp16, none): k steps at 85% of the tensor rate, then a join and an epilogue (9 to 12 thousand
+// cycles) that no next tile hides.
 #include <algorithm>
 
 #include "common.cuh"
