@@ -1761,7 +1761,8 @@ int check_linear(const brk_ctx *ctx, int rows, int k, int n, int act, const char
         return fail(BRK_ERR_INVALID, "%s: inner width %d (a multiple of 8, at most 2^24)", what, k);
     if (n < 1) return fail(BRK_ERR_INVALID, "%s: width %d < 1", what, n);
     if (act < BRK_ACT_NONE || act > BRK_ACT_QUICK_GELU) return fail(BRK_ERR_INVALID, "%s: activation %d", what, act);
-    if ((long long)((n + 127) / 128) * ((rows + 15) / 16) >= (1ll << 27))
+    // Features and tokens of a last tile stay in 31 bits too.
+    if (rows > (1 << 30) || n > (1 << 30) || (long long)((n + 127) / 128) * ((rows + 15) / 16) >= (1ll << 27))
         return fail(BRK_ERR_CAPACITY, "%s: %d x %d outputs", what, rows, n);
     return BRK_OK;
 }
@@ -1817,6 +1818,8 @@ int brk_linear(brk_ctx *ctx, int rows, int k, int n, const uint16_t *x, const ui
     if (!aligned16(x) || !aligned16(w)) return fail(BRK_ERR_INVALID, "x and w must be 16-byte aligned");
     const size_t esz = out_type == BRK_T_F16 ? 2 : 4, no = (size_t)rows * n * esz;
     if (reinterpret_cast<uintptr_t>(out) % esz) return fail(BRK_ERR_INVALID, "out is not aligned to its type");
+    if (reinterpret_cast<uintptr_t>(bias) % 4 || reinterpret_cast<uintptr_t>(residual) % 4)
+        return fail(BRK_ERR_INVALID, "bias and residual must be 4-byte aligned");
     if (overlap(out, no, x, (size_t)rows * k * 2) || overlap(out, no, w, (size_t)n * k * 2) ||
         overlap(out, no, bias, (size_t)n * 4) ||
         (overlap(out, no, residual, (size_t)rows * n * 4) && !(out == residual && out_type == BRK_T_F32)))
@@ -1839,6 +1842,8 @@ int brk_ffn_gate_up(brk_ctx *ctx, int rows, int d_model, int d_ff, const uint16_
     if (!aligned16(x) || !aligned16(w_gate) || !aligned16(w_up))
         return fail(BRK_ERR_INVALID, "x and the weights must be 16-byte aligned");
     if (reinterpret_cast<uintptr_t>(hidden) % 2) return fail(BRK_ERR_INVALID, "hidden is not aligned to its type");
+    if (reinterpret_cast<uintptr_t>(b_gate) % 4 || reinterpret_cast<uintptr_t>(b_up) % 4)
+        return fail(BRK_ERR_INVALID, "the biases must be 4-byte aligned");
     const size_t no = (size_t)rows * d_ff * 2, nw = (size_t)d_ff * d_model * 2;
     if (overlap(hidden, no, x, (size_t)rows * d_model * 2) || overlap(hidden, no, w_gate, nw) ||
         overlap(hidden, no, w_up, nw) || overlap(hidden, no, b_gate, (size_t)d_ff * 4) ||

@@ -26,7 +26,8 @@ def test_null_handles_are_refused():
 
 @pytest.mark.parametrize("rows,k,n,act,out_type", [
     (-1, 64, 8, 0, 0), (1, 0, 8, 0, 0), (1, 60, 8, 0, 0), (1, -8, 8, 0, 0), (1, 64, 0, 0, 0), (1, 64, -4, 0, 0),
-    (1, 64, 8, 5, 0), (1, 64, 8, -1, 0), (1, 64, 8, 0, 2), (2 ** 31 - 1, 64, 2 ** 31 - 1, 0, 0)])
+    (1, 64, 8, 5, 0), (1, 64, 8, -1, 0), (1, 64, 8, 0, 2), (2 ** 31 - 1, 64, 2 ** 31 - 1, 0, 0), (2 ** 31 - 1, 8, 1, 0, 0),
+    (1, 8, 2 ** 31 - 1, 0, 0), (1, 8, 2 ** 30 + 1, 0, 0)])
 def test_linear_scalars_are_refused(rows, k, n, act, out_type):
     """The checks run before the context or a tensor is looked at: stand-ins do."""
     stand_in = ctypes.create_string_buffer(4096)
@@ -45,8 +46,10 @@ def test_linear_pointers_are_refused():
     x, w, o = a, a + 1024, a + 8192
     for args in ((0, w, None, None, o), (x, 0, None, None, o), (x, w, None, None, 0), (x + 2, w, None, None, o),
                  (x, w + 2, None, None, o), (x, w, None, None, o + 2), (x, w, None, None, x), (x, w, None, None, w + 64),
-                 (x, w, o, None, o), (x, w, None, o + 4, o)):
+                 (x, w, o, None, o), (x, w, None, o + 4, o), (x, w, a + 16386, None, o), (x, w, None, a + 16386, o)):
         assert lib.brk_linear(a, 2, 64, 8, args[0], args[1], args[2], 0, args[3], args[4], 0, None) == L.BRK_ERR_INVALID
+    for b_gate, b_up in ((a + 16386, None), (None, a + 16385)):
+        assert lib.brk_ffn_gate_up(a, 2, 64, 8, x, w, w, b_gate, b_up, 0, o, None) == L.BRK_ERR_INVALID
 
 
 def test_zero_rows_do_nothing():
