@@ -778,6 +778,16 @@ __global__ void __launch_bounds__(decode_threads<Q8, D, F>(), DecodeCfg<Q8, D>::
         // P^T fragments -> P fragments (B operand of O^T += V^T P^T): keys 0-7 and 8-15.
         const uint32_t pb0 = movmatrix_t(pt0);
         const uint32_t pb1 = movmatrix_t(pt1);
+        // H: what the fp16 rounding of p' left off, as a second product: the probabilities then carry 22
+        // bits, where the 11 of one alone are half of a result's error (2.3e-4 beside the 2.1e-4 of an fp16
+        // output).
+        uint32_t rb0 = 0, rb1 = 0;
+        if constexpr (H) {
+            const float2 f0 = __half22float2(*reinterpret_cast<const __half2 *>(&pt0));
+            const float2 f1 = __half22float2(*reinterpret_cast<const __half2 *>(&pt1));
+            rb0 = movmatrix_t(pack_half2(p[0] - f0.x, p[1] - f0.y));
+            rb1 = movmatrix_t(pack_half2(p[2] - f1.x, p[3] - f1.y));
+        }
 
         // ---- O^T += V^T P^T over the warp's head-dim slice.
         if constexpr (Q8) {
@@ -801,10 +811,16 @@ __global__ void __launch_bounds__(decode_threads<Q8, D, F>(), DecodeCfg<Q8, D>::
                 // lo, t = 2, 3 in hi.  m-tile 2g+u takes bytes 4g+2u (its row qr) and 4g+2u+1 (row qr+8).
                 const uint32_t lo01 = prmt(vw[0][g], vw[1][g], 0x5140u), hi01 = prmt(vw[0][g], vw[1][g], 0x7362u);
                 const uint32_t lo23 = prmt(vw[2][g], vw[3][g], 0x5140u), hi23 = prmt(vw[2][g], vw[3][g], 0x7362u);
-                mma_16816(o[2 * g], codes_half2<H>(lo01, 0x4140u), codes_half2<H>(lo01, 0x4342u),
-                          codes_half2<H>(lo23, 0x4140u), codes_half2<H>(lo23, 0x4342u), pb0, pb1);
-                mma_16816(o[2 * g + 1], codes_half2<H>(hi01, 0x4140u), codes_half2<H>(hi01, 0x4342u),
-                          codes_half2<H>(hi23, 0x4140u), codes_half2<H>(hi23, 0x4342u), pb0, pb1);
+                const uint32_t a0 = codes_half2<H>(lo01, 0x4140u), a1 = codes_half2<H>(lo01, 0x4342u);
+                const uint32_t a2 = codes_half2<H>(lo23, 0x4140u), a3 = codes_half2<H>(lo23, 0x4342u);
+                const uint32_t b0 = codes_half2<H>(hi01, 0x4140u), b1 = codes_half2<H>(hi01, 0x4342u);
+                const uint32_t b2 = codes_half2<H>(hi23, 0x4140u), b3 = codes_half2<H>(hi23, 0x4342u);
+                mma_16816(o[2 * g], a0, a1, a2, a3, pb0, pb1);
+                mma_16816(o[2 * g + 1], b0, b1, b2, b3, pb0, pb1);
+                if constexpr (H) {
+                    mma_16816(o[2 * g], a0, a1, a2, a3, rb0, rb1);
+                    mma_16816(o[2 * g + 1], b0, b1, b2, b3, rb0, rb1);
+                }
             }
         } else {
             // Keys past the range end get zero V (in this warp's slice), so that 0 * (whatever
@@ -827,6 +843,7 @@ __global__ void __launch_bounds__(decode_threads<Q8, D, F>(), DecodeCfg<Q8, D>::
                 uint32_t a0, a1, a2, a3;
                 ldsm_x4_t(smem_addr(vt + (chunk >> 3) * L::kBoxBytes + sw128(vrow, chunk & 7)), a0, a1, a2, a3);
                 mma_16816(o[m], a0, a1, a2, a3, pb0, pb1);
+                if constexpr (H) mma_16816(o[m], a0, a1, a2, a3, rb0, rb1);
             }
         }
         // Every lane's reads of this slot (and the tail's zero stores) are generic-proxy accesses;
