@@ -285,7 +285,7 @@ struct DecodeArgsOf<true> {
 // it reads the prefix itself before the own rows and is the call's only launch.  int8 codes enter the
 // products exactly here (a subtraction more per pair; the plain form's bias of 1152 sums loses up to
 // 1e-3 of a score).  64 sequences of up to 512 own rows (32 / 8 heads of 128) beside a prefix of 4096:
-// 31 us with the prefix kernel, bound by the own rows' 74 MB and the SMs that the two share.
+// 32 us with the prefix kernel, bound by the own rows' 74 MB and the SMs that the two share.
 template <bool Q8, int D, bool F, bool H = false>
 __global__ void __launch_bounds__(decode_threads<Q8, D, F>(), DecodeCfg<Q8, D>::kMinBlocks)
     decode_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,

@@ -18,8 +18,9 @@
 //   - products whose tiles do not fill whole waves: the last one to two waves' tiles are dealt as
 //     (tile, k step) units in equal contiguous ranges.  A range's first and last piece may cover part
 //     of a tile's k; such pieces leave f32 partials in the workspace (the last to finish keeps its own
-//     in TMEM), and the last CTA of a tile to finish adds them in k order (the same order whoever is last: results do not change from run
-//     to run; so does the cluster's join).  The ranges come first, so that the joins run under the whole tiles.
+//     in TMEM), and the last CTA of a tile to finish adds them in k order, as the cluster's join does
+//     (the same order whoever is last: results do not change from run to run).  The ranges come first,
+//     so that the joins run under the whole tiles.
 // Gate-up (MODE): a CTA holds the gate and the up tile of the same F features in two accumulators
 // (kTwoAcc); with PAIR they are interleaved, 64 gate rows and 64 up rows in one accumulator
 // (kInterleaved), which leaves TMEM for a second set: the epilogue of a tile runs under the next

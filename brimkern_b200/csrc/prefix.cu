@@ -22,7 +22,7 @@
 //
 // Whole calls, own rows and joins included: 8 sequences (32 / 8 heads of 64) behind 131001 rows 57 us,
 // 4.7 TB/s of K and V, bound by the stream and 10 us of ramp and joins; 64 sequences (32 / 8 of 128)
-// behind 4096 rows 31 us, bound by the own rows beside it; 32 (8 / 4 of 256) with a window of 4096 22 us,
+// behind 4096 rows 32 us, bound by the own rows beside it; 32 (8 / 4 of 256) with a window of 4096 22 us,
 // bound by the one stream's softmax between its products.
 //
 // int8 prefix: the codes, as exact fp16 integers, are the operands; the K scale multiplies the
