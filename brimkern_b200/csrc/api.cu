@@ -1826,7 +1826,7 @@ int brk_linear(brk_ctx *ctx, int rows, int k, int n, const uint16_t *x, const ui
         return fail(BRK_ERR_INVALID, "out overlaps an input");
     DeviceGuard g(ctx->device);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const brk::LinearPlan plan = brk::linear_plan(rows, k, n, 1, ctx->num_sms);
+    const brk::LinearPlan plan = brk::linear_plan(rows, k, n, 1, out_type == BRK_T_F32, ctx->num_sms);
     brk_scratch *sc = nullptr;
     if ((rc = get_scratch(ctx, st, plan.ws_floats * sizeof(float), plan.counters, &sc))) return rc;
     return run_linear(ctx, plan, 1, rows, k, n, x, &w, &bias, act, residual, out, out_type, sc, st, false);
@@ -1851,7 +1851,7 @@ int brk_ffn_gate_up(brk_ctx *ctx, int rows, int d_model, int d_ff, const uint16_
         return fail(BRK_ERR_INVALID, "hidden overlaps an input");
     DeviceGuard g(ctx->device);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const brk::LinearPlan plan = brk::linear_plan(rows, d_model, d_ff, 2, ctx->num_sms);
+    const brk::LinearPlan plan = brk::linear_plan(rows, d_model, d_ff, 2, false, ctx->num_sms);
     brk_scratch *sc = nullptr;
     if ((rc = get_scratch(ctx, st, plan.ws_floats * sizeof(float), plan.counters, &sc))) return rc;
     const uint16_t *w[2] = {w_gate, w_up};
@@ -1877,8 +1877,8 @@ int brk_ffn(brk_ctx *ctx, int rows, int d_model, int d_ff, const float *h, const
         return fail(BRK_ERR_INVALID, "out overlaps an input");
     DeviceGuard g(ctx->device);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const brk::LinearPlan up = brk::linear_plan(rows, d_model, d_ff, 2, ctx->num_sms);
-    const brk::LinearPlan down = brk::linear_plan(rows, d_ff, d_model, 1, ctx->num_sms);
+    const brk::LinearPlan up = brk::linear_plan(rows, d_model, d_ff, 2, false, ctx->num_sms);
+    const brk::LinearPlan down = brk::linear_plan(rows, d_ff, d_model, 1, true, ctx->num_sms);
     const size_t counters = std::max(up.counters, down.counters);
     const size_t ws = align256(std::max(up.ws_floats, down.ws_floats) * sizeof(float));
     const size_t off_x = ws, off_h = off_x + align256((size_t)rows * d_model * 2);

@@ -12,6 +12,7 @@
 #include <vector>
 
 #include "brk_attn.h"
+#include "linear_plan.h"
 
 // Scratch of one stream (or of one stream capture) for the operators that keep theirs apart by
 // stream: partials / staging, and arrival counters that are zero between launches.  Calls on two
@@ -277,16 +278,6 @@ struct LinearArgs {
     int *err;
 };
 
-// How a linear product is cut: the kernel's token tile, tokens per tile, rows of the TMA boxes of x
-// and w, tiles, k, CTAs, workspace floats and counters.
-struct LinearPlan {
-    bool pair, ranged, flat;
-    int cs, nt_kernel, nt, x_rows, w_rows, f_rows, half_cols, tiles_m, nk, kb, stages, drain_steps, ctas;
-    long long tiles, tiles_whole;
-    int range_units, range_extra;
-    size_t ws_floats, counters;
-};
-
 struct CombineArgs {
     const float *part_ml, *part_o;
     size_t stride_ml, stride_o;  // floats between consecutive parts
@@ -363,7 +354,7 @@ cudaError_t launch_proj(int ntok, const CUtensorMap &tx, const CUtensorMap *tw, 
 
 // Linear operators (linear.cu); mats 1 or 2.  The maps: boxes of plan.x_rows (w_rows) rows and plan.kb
 // k steps over [k / 64][row][64] (plan.flat: one k step over [row][k]).
-LinearPlan linear_plan(int rows, int k, int n, int mats, int sms);
+LinearPlan linear_plan(int rows, int k, int n, int mats, bool drain, int sms);  // drain: f32 outputs
 cudaError_t launch_linear(int mats, const LinearPlan &p, const CUtensorMap &tx, const CUtensorMap *tw,
                           const LinearArgs &a, cudaStream_t s);
 // At most linear_rows_max() tokens: without tiles, maps or workspace (M, K, n, x, w, the epilogue's

@@ -40,18 +40,14 @@
 
 #include "common.cuh"
 #include "internal.h"
+#include "linear_plan.h"
 #include "tcgen05.cuh"
 
 namespace brk {
 
 namespace {
 
-constexpr int kLF = 128;         // MMA rows (TMEM lanes) per CTA
-constexpr int kLK = 64;          // k per step: one 128-byte swizzled row
-constexpr int kDrainK = 16;      // k steps per accumulator set when draining
-constexpr uint32_t kRing = 208 * 1024;   // bytes of the load ring
-constexpr uint32_t kSlack = 16 * 1024;   // behind it: the MMA's rows past F, or the gate / up swap
-constexpr int kMaxStages = 16;
+constexpr uint32_t kSlack = 16 * 1024;   // behind the ring: the MMA's rows past F, or the gate / up swap
 
 enum : int { kLinear = 0, kTwoAcc = 1, kInterleaved = 2 };
 
@@ -65,6 +61,8 @@ struct LinearLayout {
     static constexpr int kHalves = NT >= 64 ? 2 : 1;              // epilogue warps per TMEM lane quarter
     static constexpr int kEpiWarps = 4 * kHalves;
     static constexpr int kEpiCols = NT / kHalves;                 // most columns of an epilogue thread
+    template <bool DRAIN>
+    static constexpr int chunk = linear_chunk(NT, DRAIN);         // columns that it handles at a time
     static constexpr int kProducer = kEpiWarps, kMma = kEpiWarps + 1;
     static constexpr int kThreads = (kEpiWarps + 2) * 32;
     static constexpr uint32_t kBarOff = kRing + kSlack;
@@ -268,10 +266,7 @@ __global__ void __launch_bounds__(LinearLayout<NT, MODE, PAIR>::kThreads, 1)
                   const __grid_constant__ CUtensorMap tw1, const __grid_constant__ LinearArgs a) {
     using L = LinearLayout<NT, MODE, PAIR>;
     constexpr int CTAS = L::kCtas, BUFS = L::kBufs, MATS = L::kMats;
-    // Columns handled at a time.  f32 outputs come with a residual's loads to hide: 32 (2048 x 2560 -> 10240
-    // 112 us, 124 with 16); fp16 outputs are bound by the epilogue's instructions, whose registers spill at
-    // 32 (3000 x 1024 -> 4096 31.5 us, 26.7 with 16).
-    constexpr int CH = DRAIN && NT >= 64 ? 32 : 16;
+    constexpr int CH = L::template chunk<DRAIN>;  // columns handled at a time
     constexpr int EPI = L::kEpiWarps * 32;
     constexpr bool GATED = MODE != kLinear;
     extern __shared__ uint8_t smem_raw[];
@@ -968,16 +963,13 @@ cudaError_t launch_rows_t(const LinearArgs &a, cudaStream_t s) {
     return cudaLaunchKernelEx(&cfg, rows_kernel<R, WROWS, GATED>, a);
 }
 
-// f32 outputs (linear only) drain their accumulators.
 template <int NT, bool PAIR>
-cudaError_t launch_linear_t(int mats, const CUtensorMap &tx, const CUtensorMap *tw, const LinearArgs &a, int ctas,
-                            cudaStream_t s) {
-    if (mats == 2) return launch_linear_k<NT, PAIR ? kInterleaved : kTwoAcc, PAIR, false>(tx, tw, a, ctas, s);
-    return a.out_half ? launch_linear_k<NT, kLinear, PAIR, false>(tx, tw, a, ctas, s)
-                      : launch_linear_k<NT, kLinear, PAIR, true>(tx, tw, a, ctas, s);
+cudaError_t launch_linear_t(int mats, const LinearPlan &p, const CUtensorMap &tx, const CUtensorMap *tw,
+                            const LinearArgs &a, cudaStream_t s) {
+    if (mats == 2) return launch_linear_k<NT, PAIR ? kInterleaved : kTwoAcc, PAIR, false>(tx, tw, a, p.ctas, s);
+    return p.drain ? launch_linear_k<NT, kLinear, PAIR, true>(tx, tw, a, p.ctas, s)
+                   : launch_linear_k<NT, kLinear, PAIR, false>(tx, tw, a, p.ctas, s);
 }
-
-int round_up(int v, int m) { return (v + m - 1) / m * m; }
 
 }  // namespace
 
@@ -1013,104 +1005,8 @@ static int max_clusters(int size, int sms) {
     return n > 0 ? n : 0;
 }
 
-// The cheapest cut by a model in SM cycles.  A k step of a tile costs the larger of its products
-// (nt / 2 cycles, at least 32 for reading 128 rows, for each 16 of k and accumulator) and its bytes
-// through L2 (48 per cycle and SM with every SM loading); the whole product at least its weights from
-// HBM (3390 bytes a cycle).  On top: launch, ramp and the last tile's epilogue, and what joins split
-// tiles.
-LinearPlan linear_plan(int rows, int k, int n, int mats, int sms) {
-    const int nkb = (k + kLK - 1) / kLK;
-    const double hbm = 2.0 * mats * n * (double)k / 3390.0;
-    LinearPlan best;
-    double best_cost = 1e300;
-    auto consider = [&](bool pair, int tiles_m, int f, int cs, bool ranged) {
-        LinearPlan p;
-        const int unit = pair ? 32 : 16, ctas = pair ? 2 : 1;
-        p.pair = pair;
-        p.cs = cs;
-        p.tiles_m = tiles_m;
-        p.nt = round_up((rows + tiles_m - 1) / tiles_m, unit);
-        if (p.nt > 256) return;
-        p.nt_kernel = p.nt <= 16 ? 16 : p.nt <= 32 ? 32 : p.nt <= 64 ? 64 : p.nt <= 128 ? 128 : 256;
-        if (pair && p.nt_kernel < 128) p.nt_kernel = 128;
-        p.f_rows = f;
-        const int accs = pair ? 1 : mats;
-        if (cs > 1 && (uint32_t)(accs * p.nt * kLF * 4) > kRing) return;
-        const long long ftiles = (n + (long long)f * ctas - 1) / (f * ctas);
-        p.tiles = ftiles * tiles_m;
-        const long long slots = std::max(1, cs > 1 ? max_clusters(ctas * cs, sms) : sms / ctas);
-        if (cs > 1 && p.tiles > slots) return;
-        const int lanes = pair ? kLF : f * mats;  // weight rows of a k step and CTA
-        const double step = std::max(accs * 4.0 * std::max(p.nt / 2, 32), (lanes + p.nt / ctas) * 128 / 48.0);
-        const double epilogue = 800.0 + p.nt * (accs == 2 ? 60.0 : 24.0);
-        double cost;
-        if (ranged) {
-            const double join = 4000.0 + p.nt * 60.0;
-            cost = (double)p.tiles * nkb / slots * step + join + epilogue;
-        } else if (cs > 1) {
-            cost = (double)((nkb + cs - 1) / cs) * step + 3000.0 + accs * p.nt * 12.0 + epilogue / cs;
-        } else {
-            cost = (double)((p.tiles + slots - 1) / slots) * nkb * step + epilogue;
-        }
-        cost = std::max(cost, hbm) + (pair ? 5000.0 : 4000.0);
-        if (cost < best_cost) {
-            best_cost = cost;
-            p.ranged = ranged;
-            best = p;
-        }
-    };
-    const int tm0 = (rows + 255) / 256, pair_f = mats == 2 ? kLF / 2 : kLF;
-    for (int tm = tm0; tm <= tm0 + 2; ++tm) {
-        if (tm > tm0 && tm > rows) break;
-        // One CTA (cluster) per tile: the feature count that makes the tiles fill one, two, ... waves.
-        for (int cs = 1; cs <= 8; ++cs) {
-            if (cs > nkb) break;
-            const int slots = cs > 1 ? max_clusters(cs, sms) : sms;
-            for (int w = 1; w <= (cs > 1 ? 1 : 4); ++w) {
-                const long long ft = (long long)slots * w / tm;
-                if (ft < 1) continue;
-                const int f = round_up((int)((n + ft - 1) / ft), 8);
-                if (f <= kLF) {
-                    consider(false, tm, f, cs, false);
-                    break;
-                }
-            }
-        }
-        consider(false, tm, kLF, 1, true);
-        if (rows > 32) {
-            for (int cs = 1; cs <= 4 && cs <= nkb; ++cs) consider(true, tm, pair_f, cs, false);
-            consider(true, tm, pair_f, 1, true);
-        }
-    }
-    LinearPlan &p = best;
-    const int ctas = p.pair ? 2 : 1;
-    p.x_rows = p.nt / ctas;
-    p.half_cols = p.nt_kernel >= 64 ? round_up((p.nt + 1) / 2, 16) : p.nt;
-    p.w_rows = p.f_rows;
-    // k steps per stage: one TMA fetches up to eight (k a multiple of 64), a stage about 32 KB.
-    const bool by_step = k % kLK == 0 && !p.pair;
-    const int step_rows = (p.pair ? kLF : p.f_rows * mats) + p.x_rows;
-    p.kb = 1;
-    while (by_step && p.kb < 8 && 2 * p.kb * step_rows * 128 <= 40 * 1024 && nkb >= 4 * p.kb * p.cs) p.kb *= 2;
-    p.flat = p.kb == 1;
-    p.stages = std::min<int>(kMaxStages, kRing / (p.kb * step_rows * 128));
-    p.nk = (nkb + p.kb - 1) / p.kb;
-    p.drain_steps = kDrainK / p.kb;
-    // Workers: a CTA (pair, cluster) per SM (two, ...), no more than there is work for.
-    long long workers = p.cs > 1 ? p.tiles : std::max(1, sms / ctas);
-    workers = std::min<long long>(workers, p.ranged ? p.tiles * p.nk : p.tiles);
-    // Ranged: whole waves of tiles, but for the last one to two waves' (unless they divide).
-    p.tiles_whole = p.tiles;
-    if (p.ranged && p.tiles % workers) {
-        const long long waves = p.tiles / workers;
-        p.tiles_whole = waves > 0 ? (waves - 1) * workers : 0;
-    }
-    p.ctas = (int)workers * ctas * p.cs;
-    const long long units = (p.tiles - p.tiles_whole) * p.nk;
-    p.range_units = (int)(units / workers), p.range_extra = (int)(units % workers);
-    p.counters = (size_t)(p.tiles - p.tiles_whole) * ctas;
-    p.ws_floats = p.tiles > p.tiles_whole ? (size_t)p.ctas * 2 * ((p.pair ? 1 : mats) * p.nt + 16) * kLF : 0;
-    return p;
+LinearPlan linear_plan(int rows, int k, int n, int mats, bool drain, int sms) {
+    return linear_plan_for(rows, k, n, mats, drain, sms, [sms](int size) { return max_clusters(size, sms); });
 }
 
 int linear_rows_max() { return 4; }
@@ -1126,14 +1022,14 @@ cudaError_t launch_linear_rows(int mats, const LinearArgs &a, cudaStream_t s) {
 cudaError_t launch_linear(int mats, const LinearPlan &p, const CUtensorMap &tx, const CUtensorMap *tw,
                           const LinearArgs &a, cudaStream_t s) {
     if (p.pair)
-        return p.nt_kernel == 128 ? launch_linear_t<128, true>(mats, tx, tw, a, p.ctas, s)
-                                  : launch_linear_t<256, true>(mats, tx, tw, a, p.ctas, s);
+        return p.nt_kernel == 128 ? launch_linear_t<128, true>(mats, p, tx, tw, a, s)
+                                  : launch_linear_t<256, true>(mats, p, tx, tw, a, s);
     switch (p.nt_kernel) {
-        case 16: return launch_linear_t<16, false>(mats, tx, tw, a, p.ctas, s);
-        case 32: return launch_linear_t<32, false>(mats, tx, tw, a, p.ctas, s);
-        case 64: return launch_linear_t<64, false>(mats, tx, tw, a, p.ctas, s);
-        case 128: return launch_linear_t<128, false>(mats, tx, tw, a, p.ctas, s);
-        default: return launch_linear_t<256, false>(mats, tx, tw, a, p.ctas, s);
+        case 16: return launch_linear_t<16, false>(mats, p, tx, tw, a, s);
+        case 32: return launch_linear_t<32, false>(mats, p, tx, tw, a, s);
+        case 64: return launch_linear_t<64, false>(mats, p, tx, tw, a, s);
+        case 128: return launch_linear_t<128, false>(mats, p, tx, tw, a, s);
+        default: return launch_linear_t<256, false>(mats, p, tx, tw, a, s);
     }
 }
 
