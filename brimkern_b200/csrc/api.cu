@@ -271,6 +271,7 @@ int decode_split_plan(const brk_ctx *ctx, const brk_kv *kv, const brk_attn_param
             hi = kv->cap;
         }
         int lo = window > 0 ? std::max(0, past_len[b] - window + 1 - p->kv_offset) : 0;
+        if (kv->q8()) lo = lo / 4 * 4;  // as the kernel does (decode_key_range): the splits count from there
         span = std::max(span, hi - lo);
     }
     const int G = p->n_heads / p->n_kv_heads;
