@@ -164,6 +164,16 @@ __device__ __forceinline__ float ex2_fast(float x) {
     return y;
 }
 
+// What an int8 row's V scale adds to its score (log2 units) where a running maximum decides what the
+// probabilities are relative to: with it the largest probability times V scale is about 2^13, whatever
+// the size of V, and its fp16 form keeps its bits down to 2^-27 of that (2^-38 with a second term).  The
+// limits keep the sum of the bare probabilities, relative to the same, within f32.
+__device__ __forceinline__ float v_scale_log2(float scale) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(scale));
+    return fminf(fmaxf(y, -80.f), 100.f) - 13.f;
+}
+
 // Hardware reciprocal (MUFU; ~1 ulp, flushes subnormals; 1/inf = 0).
 __device__ __forceinline__ float rcp_fast(float x) {
     float y;

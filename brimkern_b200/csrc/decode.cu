@@ -730,6 +730,11 @@ __global__ void __launch_bounds__(decode_threads<Q8, D, F>(), DecodeCfg<Q8, D>::
             }
         }
         float mx[2] = {fmaxf(sacc[0], sacc[2]), fmaxf(sacc[1], sacc[3])};
+        if constexpr (Q8 && H) {
+            // The maximum of probability times V scale, which is what is rounded to fp16.
+            const float la = v_scale_log2(vsc[0]), lb = v_scale_log2(vsc[1]);
+            mx[0] = fmaxf(sacc[0] + la, sacc[2] + lb), mx[1] = fmaxf(sacc[1] + la, sacc[3] + lb);
+        }
         float muse[2];
         bool grew = false;
 #pragma unroll

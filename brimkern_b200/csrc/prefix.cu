@@ -26,7 +26,9 @@
 // bound by the one stream's softmax between its products.
 //
 // int8 prefix: the codes, as exact fp16 integers, are the operands; the K scale multiplies the
-// scores and the V scale the probabilities, so nothing is rounded that the fp16 form does not round.
+// scores and the V scale the probabilities, so nothing is rounded that the fp16 form does not round.  The
+// maximum that the probabilities are relative to counts the V scales in (v_scale_log2), so that their
+// products stay in fp16's normal range whatever the size of V (without: 1% off at |V| 0.001).
 #include <math_constants.h>
 
 #include <algorithm>
@@ -140,7 +142,7 @@ __global__ void __launch_bounds__(PrefixLayout<D>::kThreads, 1)
     constexpr int RC = kXQ / COPIES;  // MMA rows of a copy
     constexpr int KC = kXK / COPIES;  // keys of a tile that a copy takes
     // Raise the running max (and rescale O) only when a tile's max exceeds it by more than this
-    // many powers of two: P stays below 2^8, or, times an int8 row's V scale, below 4 scales.
+    // many powers of two: P stays below 2^8, or, times an int8 row's V scale, below 2^15 (v_scale_log2).
     constexpr float kRaise = Q8 ? 2.f : 8.f;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -366,9 +368,20 @@ __global__ void __launch_bounds__(PrefixLayout<D>::kThreads, 1)
                     for (int e = 0; e < KC; ++e) v[e] = kbase + e >= lo && kbase + e < ke ? v[e] : -CUDART_INF_F;
                 }
                 const float mraw = max_tree(v);
-                const float mt = mraw == -CUDART_INF_F ? -CUDART_INF_F
-                                 : cap                 ? softcap_log2(mraw, a.cap_k1, a.cap_k2)
-                                                       : mraw * a.scale_log2;
+                float mt = mraw == -CUDART_INF_F ? -CUDART_INF_F
+                           : cap                 ? softcap_log2(mraw, a.cap_k1, a.cap_k2)
+                                                 : mraw * a.scale_log2;
+                if constexpr (Q8) {
+                    // At least the maximum of probability times V scale, which is what is rounded to fp16:
+                    // with the largest scale of the keys in range (positive floats compare as their bits).
+                    unsigned top = 0u;
+#pragma unroll
+                    for (int e = 0; e < KC; e += 32) {
+                        const int x = KC < 32 ? lane % KC : e + lane;
+                        if (kbase + x < ke) top = max(top, __float_as_uint(vsc[x]));
+                    }
+                    mt += v_scale_log2(__uint_as_float(__reduce_max_sync(0xffffffffu, top)));
+                }
                 // Rows raise their maximum separately; the rescale pass is warp-collective.
                 const bool raise = mt > m_used + kRaise || (m_used == -CUDART_INF_F && mt != -CUDART_INF_F);
                 const bool rescale = raise && m_used != -CUDART_INF_F && i >= 1;
