@@ -265,6 +265,18 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
     return *reinterpret_cast<uint32_t *>(&h);
 }
 
+// lo - h[0], hi - h[1] as an fp16 pair: what pack_half2's rounding of (lo, hi) to h left off (the
+// differences are exact).
+__device__ __forceinline__ uint32_t half2_rest(float lo, float hi, uint32_t h) {
+    float r0, r1;
+    asm("{\n\t.reg .f16 a, b, m;\n\t"
+        "mov.b32 {a, b}, %2;\n\tmov.b16 m, 0xBC00;\n\t"  // -1
+        "fma.rn.f32.f16 %0, a, m, %3;\n\tfma.rn.f32.f16 %1, b, m, %4;\n\t}"
+        : "=f"(r0), "=f"(r1)
+        : "r"(h), "f"(lo), "f"(hi));
+    return pack_half2(r0, r1);
+}
+
 // Programmatic dependent launch: wait for the grids this one depends on (completion and memory
 // visibility); a no-op when the launch has no programmatic dependency.
 __device__ __forceinline__ void griddep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }

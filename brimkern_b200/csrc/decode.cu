@@ -730,9 +730,9 @@ __global__ void __launch_bounds__(decode_threads<Q8, D, F>(), DecodeCfg<Q8, D>::
             }
         }
         float mx[2] = {fmaxf(sacc[0], sacc[2]), fmaxf(sacc[1], sacc[3])};
-        if constexpr (Q8 && H) {
-            // The maximum of probability times V scale, which is what is rounded to fp16.
-            const float la = v_scale_log2(vsc[0]), lb = v_scale_log2(vsc[1]);
+        if constexpr (H) {
+            // The maximum of probability times V scale, which is what is rounded to fp16 (fp16 rows: scale 1).
+            const float la = Q8 ? v_scale_log2(vsc[0]) : -13.f, lb = Q8 ? v_scale_log2(vsc[1]) : -13.f;
             mx[0] = fmaxf(sacc[0] + la, sacc[2] + lb), mx[1] = fmaxf(sacc[1] + la, sacc[3] + lb);
         }
         float muse[2];
@@ -788,10 +788,8 @@ __global__ void __launch_bounds__(decode_threads<Q8, D, F>(), DecodeCfg<Q8, D>::
         // output).
         uint32_t rb0 = 0, rb1 = 0;
         if constexpr (H) {
-            const float2 f0 = __half22float2(*reinterpret_cast<const __half2 *>(&pt0));
-            const float2 f1 = __half22float2(*reinterpret_cast<const __half2 *>(&pt1));
-            rb0 = movmatrix_t(pack_half2(p[0] - f0.x, p[1] - f0.y));
-            rb1 = movmatrix_t(pack_half2(p[2] - f1.x, p[3] - f1.y));
+            rb0 = movmatrix_t(half2_rest(p[0], p[1], pt0));
+            rb1 = movmatrix_t(half2_rest(p[2], p[3], pt1));
         }
 
         // ---- O^T += V^T P^T over the warp's head-dim slice.

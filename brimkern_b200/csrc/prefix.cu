@@ -7,7 +7,10 @@
 // product: 4 D flops per (row, key) for 4 D bytes per key, which passes the ridge near 250 rows.
 // A CTA takes one kv head, one block of rows and one split of the keys, in 64-key tiles:
 //   S = Q K^T (M 128, N 64) in TMEM, each row's softmax by one thread (running maximum and sum in
-//   f32), P as fp16 pairs in TMEM, O += P V in TMEM.
+//   f32), P as two fp16 terms (its rounding and what that leaves off) in TMEM, O += P V in TMEM.
+// With one term the rounding of P, 2^-11 of each, is as large as an fp16 output's own (relative error
+// against 64 bits 2.9e-4, with two 2.1e-4); the second costs MMAs and conversions: 8 sequences behind 131001
+// rows 67 -> 78 us, 16 x 2 tokens over int8 rows 32.7 -> 34.1, 64 behind 4096 34 -> 35.5, the window no time.
 // Two streams of 128 rows run a tile apart so that one's exponentials overlap the other's products:
 // with more rows than one stream holds the streams are two row tiles that share every K/V tile; with
 // fewer they take alternate key tiles of the same rows.  head_dim 256 leaves TMEM for one stream.
@@ -63,9 +66,9 @@ struct PrefixLayout {
     static constexpr uint32_t kOffState = kOffScale + kStages * 2 * kXK * 4;  // [m, l][stream][128] f32
     static constexpr uint32_t kOffBar = kOffState + 2 * kStreams * kXQ * 4;
     static constexpr uint32_t kSmemBytes = 1024 + kOffBar + 36 * 8 + 16;
-    // TMEM columns: S, then P (fp16 pairs), then O from column 256 (one stream of D 256) or 192.
-    static constexpr uint32_t kColS = 0, kColP = kStreams * kXK, kColO = kStreams == 1 ? 256 : 192;
-    static_assert(kColP + kStreams * kXK / 2 <= kColO && kColO + kStreams * D <= kXTmemCols, "TMEM columns");
+    // TMEM columns: S, then P's two terms (fp16 pairs), then O from column 256.
+    static constexpr uint32_t kColS = 0, kColP = kStreams * kXK, kColR = kColP + kStreams * kXK / 2, kColO = 256;
+    static_assert(kColR + kStreams * kXK / 2 <= kColO && kColO + kStreams * D <= kXTmemCols, "TMEM columns");
     static_assert(kSmemBytes <= 232448, "more than 227 KB of shared memory per CTA");
     // The join: every stream's O [128][kJoin] f32 over q and the ring; the padding spreads the banks.
     static constexpr uint32_t kJoin = D + 4;
@@ -141,8 +144,9 @@ __global__ void __launch_bounds__(PrefixLayout<D>::kThreads, 1)
     constexpr int NS = L::kStreams;
     constexpr int RC = kXQ / COPIES;  // MMA rows of a copy
     constexpr int KC = kXK / COPIES;  // keys of a tile that a copy takes
-    // Raise the running max (and rescale O) only when a tile's max exceeds it by more than this
-    // many powers of two: P stays below 2^8, or, times an int8 row's V scale, below 2^15 (v_scale_log2).
+    // Raise the running max (and rescale O) only when a tile's max exceeds it by more than this many powers
+    // of two.  P is relative to 2^-6 of the maximum, and so stays below 2^14 (int8: times the row's V scale,
+    // below 2^15, v_scale_log2): fp16's normal range then reaches further down.
     constexpr float kRaise = Q8 ? 2.f : 8.f;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -279,9 +283,11 @@ __global__ void __launch_bounds__(PrefixLayout<D>::kThreads, 1)
                 tc_fence_after();
                 const uint32_t v_base = smem_addr(sV(st));
 #pragma unroll
-                for (int kk = 0; kk < kXK / 16; ++kk)
-                    tc_mma_ts(tmem + L::kColO + s * D, tmem + L::kColP + s * (kXK / 2) + kk * 8,
-                              sw128_desc(v_base + kk * 16 * 128, L::kKVBlock, 1024), idesc_pv, i > 0 || kk > 0);
+                for (int kk = 0; kk < kXK / 16; ++kk) {
+                    const uint64_t vd = sw128_desc(v_base + kk * 16 * 128, L::kKVBlock, 1024);
+                    tc_mma_ts(tmem + L::kColO + s * D, tmem + L::kColP + s * (kXK / 2) + kk * 8, vd, idesc_pv, i > 0 || kk > 0);
+                    tc_mma_ts(tmem + L::kColO + s * D, tmem + L::kColR + s * (kXK / 2) + kk * 8, vd, idesc_pv, true);
+                }
                 tc_commit(&bars[kXODone + s]);
                 tc_commit(&bars[kXVEmpty + st]);
                 return true;
@@ -310,6 +316,7 @@ __global__ void __launch_bounds__(PrefixLayout<D>::kThreads, 1)
         const uint32_t tS = tmem + L::kColS + s * kXK + lane_base + copy * KC;
         const uint32_t tO = tmem + L::kColO + s * D + lane_base;
         const uint32_t tP = tmem + L::kColP + s * (kXK / 2) + lane_base;
+        const uint32_t tR = tmem + L::kColR + s * (kXK / 2) + lane_base;
         // A warp without rows only keeps the barriers going.
         const bool idle = !__any_sync(0xffffffffu, row_ok);
         if (COPIES > 1 || idle) {
@@ -318,6 +325,7 @@ __global__ void __launch_bounds__(PrefixLayout<D>::kThreads, 1)
 #pragma unroll
             for (int e = 0; e < 32; ++e) zero[e] = 0u;
             tc_st32(tP, zero);
+            tc_st32(tR, zero);
             tc_wait_st();
         }
         float m_used = -CUDART_INF_F;  // the maximum that the probabilities are relative to (log2 units)
@@ -334,7 +342,7 @@ __global__ void __launch_bounds__(PrefixLayout<D>::kThreads, 1)
             }
             tc_fence_after();
             bool waited = false;
-            uint32_t pk[KC / 2];
+            uint32_t pk[KC / 2], rk[KC / 2];  // P's terms: its fp16 rounding, and what that left off
             float rsum = 0.f;
             if (idle) {
                 mbar_arrive(&bars[kXSFree + s]);
@@ -381,6 +389,8 @@ __global__ void __launch_bounds__(PrefixLayout<D>::kThreads, 1)
                         if (kbase + x < ke) top = max(top, __float_as_uint(vsc[x]));
                     }
                     mt += v_scale_log2(__uint_as_float(__reduce_max_sync(0xffffffffu, top)));
+                } else {
+                    mt -= 6.f;
                 }
                 // Rows raise their maximum separately; the rescale pass is warp-collective.
                 const bool raise = mt > m_used + kRaise || (m_used == -CUDART_INF_F && mt != -CUDART_INF_F);
@@ -444,7 +454,10 @@ __global__ void __launch_bounds__(PrefixLayout<D>::kThreads, 1)
                     }
                 }
 #pragma unroll
-                for (int u = 0; u < KC / 2; ++u) pk[u] = pack_half2(v[2 * u], v[2 * u + 1]);
+                for (int u = 0; u < KC / 2; ++u) {
+                    pk[u] = pack_half2(v[2 * u], v[2 * u + 1]);
+                    rk[u] = half2_rest(v[2 * u], v[2 * u + 1], pk[u]);
+                }
             }
             if (i >= 1 && !waited) {
                 const bool got = mbar_wait(&bars[kXODone + s], (i - 1) & 1, a.err, kErrMmaTimeout);
@@ -453,7 +466,10 @@ __global__ void __launch_bounds__(PrefixLayout<D>::kThreads, 1)
                     break;
                 }
             }
-            if (!idle) st_probs<KC / 2>(tP + copy * (KC / 2), pk);
+            if (!idle) {
+                st_probs<KC / 2>(tP + copy * (KC / 2), pk);
+                st_probs<KC / 2>(tR + copy * (KC / 2), rk);
+            }
             // Keys past the range end: zero V rows, so that 0 * (whatever the tile holds) stays 0.
             if ((s == 0 || !pair) && tail) {
                 const int key = kb + j * kXK + r;
