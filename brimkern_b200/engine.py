@@ -50,6 +50,20 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
+def _buffers_like(t: torch.Tensor, stream: Optional[torch.cuda.Stream], q_work, out):
+    """q_work and out, or in the place of None a buffer like `t` that belongs to the stream that writes
+    it: a block of another stream's could be handed out again there while it is still written.  out, which
+    the caller reads on the current stream, also waits for that one's work when it is dropped."""
+    if stream is None:
+        return torch.empty_like(t) if q_work is None else q_work, torch.empty_like(t) if out is None else out
+    with torch.cuda.stream(stream):
+        q_work = torch.empty_like(t) if q_work is None else q_work
+        new = torch.empty_like(t) if out is None else None
+    if new is not None:
+        new.record_stream(torch.cuda.current_stream(t.device))
+    return q_work, out if new is None else new
+
+
 def _positions(past_len, batch: int):
     if isinstance(past_len, (list, tuple)) and len(past_len) == batch:
         try:
@@ -582,8 +596,7 @@ class AttentionEngine:
                        kernel: str = "auto", stream=None) -> torch.Tensor:
         """The attention slice of recordLayerKV (kernels.ts:1707-1731): q/k/v projections in,
         attention output out; K/V land in the cache."""
-        q_work = torch.empty_like(q_in) if q_work is None else q_work
-        out = torch.empty_like(q_in) if out is None else out
+        q_work, out = _buffers_like(q_in, stream, q_work, out)
         B = kv.batch
         T = q_in.numel() // (B * cfg.n_heads * cfg.head_dim)
         if kernel == "auto" and self.attnDecodeOk and T * (cfg.n_heads // cfg.n_kv_heads) <= 64:
@@ -709,8 +722,7 @@ class AttentionEngine:
         projections; out f32 (default) or fp16."""
         T = self._prefix_tokens(kv, cfg, q_in, "q_in")
         n_kv = kv.batch * T * cfg.n_kv_heads * cfg.head_dim
-        q_work = torch.empty_like(q_in) if q_work is None else q_work
-        out = torch.empty_like(q_in) if out is None else out
+        q_work, out = _buffers_like(q_in, stream, q_work, out)
         ptrs = [self._tensor(t, n, _F32, None) for t, n in ((q_in, "q_in"), (k_in, "k_in"), (v_in, "v_in"), (q_work, "q_work"))]
         op = self._tensor(out, "out", _T_TYPES, None)
         for t, n, want in ((k_in, "k_in", n_kv), (v_in, "v_in", n_kv), (q_work, "q_work", q_in.numel()),
