@@ -306,72 +306,195 @@ int ensure_counters(brk_ctx *ctx, size_t n) {
     return BRK_OK;
 }
 
-// The scratch of `stream`, or of `stream` in the capture it is in: a workspace of at least `bytes` and
-// n_counters zeroed counters.  Growing keeps the old buffers (queued kernels and captured graphs
-// may still use them) and neither synchronises nor disturbs a capture: the allocation runs in
-// relaxed capture mode, and the counters are zeroed on a stream of the context's own.
-int get_scratch(brk_ctx *ctx, cudaStream_t stream, size_t bytes, size_t n_counters, brk_scratch **out) {
-    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
-    unsigned long long id = 0, capture_id = 0;
-    BRK_CUDA(cudaStreamGetCaptureInfo(stream, &st, &capture_id));
-    if (st == cudaStreamCaptureStatusInvalidated) return fail(BRK_ERR_CUDA, "the stream's capture is invalid");
-    const bool capture = st == cudaStreamCaptureStatusActive;
-    if (capture)
-        id = reinterpret_cast<uintptr_t>(stream);  // the id may not be asked for in a capture
-    else
-        BRK_CUDA(cudaStreamGetId(stream, &id));
-    brk_scratch *sc = nullptr;
-    for (brk_scratch *x : ctx->scratch)
-        if (x->id == id && x->capture == capture && (!capture || x->capture_id == capture_id)) sc = x;
-    if (!sc) {
-        sc = new (std::nothrow) brk_scratch();
-        if (!sc) return fail(BRK_ERR_CUDA, "out of host memory");
-        sc->id = id, sc->capture_id = capture_id;
-        sc->capture = capture;
-        try {
-            ctx->scratch.push_back(sc);
-        } catch (...) {
-            delete sc;
-            return fail(BRK_ERR_CUDA, "out of host memory");
+// Device memory while any thread may be capturing: the calls are allowed in relaxed mode, and touch no
+// capture.
+struct RelaxedCapture {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+    ~RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+};
+
+void free_scratch(brk_scratch *sc) {
+    cudaFree(sc->ws);
+    cudaFree(sc->counters);
+    for (void *p : sc->retired) cudaFree(p);
+    delete sc;
+}
+
+// (No CUDA call is made under the lock: CUDA's own callback takes it.)
+void free_idle_graph_scratch(brk_ctx *ctx) {
+    std::vector<brk_scratch *> gone;
+    {
+        std::lock_guard<std::mutex> lock(ctx->graph_scratch->mu);
+        gone = ctx->graph_scratch->idle;
+        ctx->graph_scratch->idle.clear();  // keeps the room that release_graph_scratch counts on
+    }
+    for (brk_scratch *sc : gone) free_scratch(sc);
+}
+
+// cudaMalloc, once more without the idle scratch of captures if there is no room.
+cudaError_t scratch_malloc(brk_ctx *ctx, void **p, size_t bytes) {
+    cudaError_t e = cudaMalloc(p, bytes);
+    if (e != cudaErrorMemoryAllocation) return e;
+    cudaGetLastError();
+    free_idle_graph_scratch(ctx);
+    return cudaMalloc(p, bytes);
+}
+
+// Sizes in steps of an eighth to a quarter, so that captures of slightly different calls can take each
+// other's scratch.
+size_t scratch_size(size_t bytes) {
+    size_t step = 256;
+    while (step * 8 < bytes) step *= 2;
+    return (bytes + step - 1) / step * step;
+}
+
+// Called by CUDA when a graph's scratch is no longer needed.
+struct GraphScratchRef {
+    std::shared_ptr<brk_graph_scratch> pool;
+    brk_scratch *sc;
+};
+void CUDART_CB release_graph_scratch(void *arg) {
+    GraphScratchRef *ref = static_cast<GraphScratchRef *>(arg);
+    {
+        std::lock_guard<std::mutex> lock(ref->pool->mu);
+        std::vector<brk_scratch *> &live = ref->pool->live;
+        if (!ref->pool->closed) {
+            live.erase(std::find(live.begin(), live.end(), ref->sc));
+            ref->pool->idle.push_back(ref->sc);  // (room for it is reserved when it becomes live)
         }
     }
+    delete ref;
+}
+
+// The scratch of `stream` in the capture `capture_id` of `graph`: the one that it has, an idle one (the
+// smallest that is large enough, else the largest), or a new one.
+int graph_scratch(brk_ctx *ctx, cudaStream_t stream, unsigned long long capture_id, cudaGraph_t graph, size_t bytes,
+                  size_t n_counters, brk_scratch **out) {
+    brk_graph_scratch &pool = *ctx->graph_scratch;
+    const unsigned long long id = reinterpret_cast<uintptr_t>(stream);  // the stream's id may not be asked for here
+    std::unique_ptr<GraphScratchRef> ref(new GraphScratchRef{ctx->graph_scratch, nullptr});
+    brk_scratch *sc = nullptr;
+    {
+        std::lock_guard<std::mutex> lock(pool.mu);
+        for (auto it = pool.live.rbegin(); it != pool.live.rend(); ++it)
+            if ((*it)->id == id && (*it)->capture_id == capture_id) {
+                *out = *it;
+                return BRK_OK;
+            }
+        pool.live.reserve(pool.live.size() + 1);
+        pool.idle.reserve(pool.idle.size() + pool.live.size() + 1);
+        auto fits = [&](const brk_scratch *x) { return x->ws_bytes >= bytes && x->counters_n >= n_counters; };
+        auto better = [&](const brk_scratch *x, const brk_scratch *y) {
+            if (fits(x) != fits(y)) return fits(x);
+            return fits(x) ? x->ws_bytes < y->ws_bytes : x->ws_bytes > y->ws_bytes;
+        };
+        const auto best = std::min_element(pool.idle.begin(), pool.idle.end(), better);
+        if (best != pool.idle.end()) {
+            sc = *best;
+            pool.idle.erase(best);
+        } else {
+            sc = new brk_scratch();
+        }
+        sc->id = id, sc->capture_id = capture_id;
+        pool.live.push_back(sc);
+    }
+    ref->sc = sc;
+    cudaUserObject_t obj = nullptr;
+    cudaError_t e = cudaUserObjectCreate(&obj, ref.get(), release_graph_scratch, 1, cudaUserObjectNoDestructorSync);
+    if (e == cudaSuccess) {
+        ref.release();
+        e = cudaGraphRetainUserObject(graph, obj, 1, cudaGraphUserObjectMove);
+    }
+    if (e != cudaSuccess) return cuda_fail(e, "scratch of a captured graph");  // (it stays live until brk_ctx_destroy)
+    // What an earlier capture outgrew.
+    if (!sc->retired.empty()) {
+        RelaxedCapture relaxed;
+        for (void *p : sc->retired) cudaFree(p);
+        sc->retired.clear();
+    }
     *out = sc;
-    if (bytes <= sc->ws_bytes && n_counters <= sc->counters_n) return BRK_OK;
-    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-    BRK_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
-    cudaError_t e = cudaSuccess;
+    return BRK_OK;
+}
+
+// The scratch of a stream outside a capture.  Streams come and go without a word, so only the kMostStreams
+// last used ones keep theirs; cudaFree waits for the kernels that may still use it.
+constexpr size_t kMostStreams = 64;
+int stream_scratch(brk_ctx *ctx, cudaStream_t stream, brk_scratch **out) {
+    unsigned long long id = 0;
+    BRK_CUDA(cudaStreamGetId(stream, &id));
+    std::vector<brk_scratch *> &list = ctx->scratch;
+    size_t i = 0;
+    while (i < list.size() && list[i]->id != id) ++i;
+    if (i == list.size()) {
+        if (list.size() >= kMostStreams) {
+            RelaxedCapture relaxed;
+            free_scratch(list.back());
+            list.pop_back();
+            i = list.size();
+        }
+        list.reserve(list.size() + 1);
+        list.push_back(new brk_scratch());
+        list.back()->id = id;
+    }
+    std::rotate(list.begin(), list.begin() + i, list.begin() + i + 1);
+    *out = list.front();
+    return BRK_OK;
+}
+
+// The scratch of `stream`, or of `stream` in the capture it is in: a workspace of at least `bytes` and
+// n_counters zeroed counters.  Growing does not disturb a capture: the allocation runs in relaxed capture
+// mode, and the counters are zeroed on a stream of the context's own.  What a capture outgrows stays with
+// its graph; a stream's old buffer goes as soon as its kernels are through.
+int get_scratch(brk_ctx *ctx, cudaStream_t stream, size_t bytes, size_t n_counters, brk_scratch **out) {
+    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    unsigned long long capture_id = 0;
+    cudaGraph_t graph = nullptr;
+    BRK_CUDA(cudaStreamGetCaptureInfo(stream, &st, &capture_id, &graph));
+    if (st == cudaStreamCaptureStatusInvalidated) return fail(BRK_ERR_CUDA, "the stream's capture is invalid");
+    const bool capture = st == cudaStreamCaptureStatusActive;
     try {
+        brk_scratch *sc = nullptr;
+        const int rc = capture ? graph_scratch(ctx, stream, capture_id, graph, bytes, n_counters, &sc)
+                               : stream_scratch(ctx, stream, &sc);
+        if (rc) return rc;
+        *out = sc;
+        if (bytes <= sc->ws_bytes && n_counters <= sc->counters_n) return BRK_OK;
+        RelaxedCapture relaxed;
+        cudaError_t e = cudaSuccess;
         sc->retired.reserve(sc->retired.size() + 2);
+        auto drop = [&](void *old) {
+            if (old && capture) sc->retired.push_back(old);
+            if (old && !capture) cudaFree(old);
+        };
         if (bytes > sc->ws_bytes) {
-            const size_t want = (std::max(bytes, 2 * sc->ws_bytes) + 255) / 256 * 256;
             void *p = nullptr;
-            e = cudaMalloc(&p, want);
+            e = scratch_malloc(ctx, &p, scratch_size(bytes));
             if (e == cudaSuccess) {
-                if (sc->ws) sc->retired.push_back(sc->ws);
+                drop(sc->ws);
                 sc->ws = p;
-                sc->ws_bytes = want;
+                sc->ws_bytes = scratch_size(bytes);
             }
         }
         if (e == cudaSuccess && n_counters > sc->counters_n) {
             const size_t want = std::max(std::max(n_counters, 2 * sc->counters_n), (size_t)4096);
             void *p = nullptr;
-            e = cudaMalloc(&p, want * sizeof(int));
+            e = scratch_malloc(ctx, &p, want * sizeof(int));
             if (e == cudaSuccess && !ctx->aux) e = cudaStreamCreateWithFlags(&ctx->aux, cudaStreamNonBlocking);
             if (e == cudaSuccess) e = cudaMemsetAsync(p, 0, want * sizeof(int), ctx->aux);
             if (e == cudaSuccess) e = cudaStreamSynchronize(ctx->aux);
             if (e == cudaSuccess) {
-                if (sc->counters) sc->retired.push_back(sc->counters);
+                drop(sc->counters);
                 sc->counters = static_cast<int *>(p);
                 sc->counters_n = want;
             } else {
                 cudaFree(p);
             }
         }
-    } catch (...) {
-        e = cudaErrorMemoryAllocation;
+        if (e != cudaSuccess) return cuda_fail(e, "scratch allocation");
+    } catch (const std::bad_alloc &) {
+        return fail(BRK_ERR_CUDA, "out of host memory");
     }
-    cudaThreadExchangeStreamCaptureMode(&mode);
-    if (e != cudaSuccess) return cuda_fail(e, "scratch allocation");
     return BRK_OK;
 }
 
@@ -562,6 +685,7 @@ int brk_ctx_create(int device, brk_ctx **out) {
     BRK_CUDA(cudaGetDeviceProperties(&prop, device));
     if (prop.major != 10) return fail(BRK_ERR_UNSUPPORTED, "device %d is sm_%d%d; this build targets sm_100a", device, prop.major, prop.minor);
     brk_ctx *c = new brk_ctx();
+    c->graph_scratch = std::make_shared<brk_graph_scratch>();
     c->device = device;
     c->num_sms = prop.multiProcessorCount;
     cudaError_t e = cudaMalloc(&c->d_err, sizeof(int));
@@ -603,12 +727,15 @@ int brk_ctx_destroy(brk_ctx *ctx) {
     cudaFree(ctx->ws);
     cudaFree(ctx->stage);
     cudaFree(ctx->act);
-    for (brk_scratch *sc : ctx->scratch) {
-        cudaFree(sc->ws);
-        cudaFree(sc->counters);
-        for (void *p : sc->retired) cudaFree(p);
-        delete sc;
+    for (brk_scratch *sc : ctx->scratch) free_scratch(sc);
+    std::vector<brk_scratch *> live;
+    {
+        std::lock_guard<std::mutex> lock(ctx->graph_scratch->mu);
+        ctx->graph_scratch->closed = true;
+        live.swap(ctx->graph_scratch->live);
     }
+    for (brk_scratch *sc : live) free_scratch(sc);
+    free_idle_graph_scratch(ctx);
     if (ctx->aux) cudaStreamDestroy(ctx->aux);
     delete ctx;
     return BRK_OK;
@@ -624,7 +751,13 @@ int brk_ctx_check(brk_ctx *ctx, void *stream) {
         BRK_CUDA(cudaMemset(ctx->d_err, 0, sizeof(int)));
         // A kernel that gave up may have left split counters mid-count: start them from zero.
         if (ctx->counters) BRK_CUDA(cudaMemset(ctx->counters, 0, ctx->counters_n * sizeof(int)));
-        for (brk_scratch *sc : ctx->scratch)
+        std::vector<brk_scratch *> all = ctx->scratch;
+        {
+            std::lock_guard<std::mutex> lock(ctx->graph_scratch->mu);
+            for (auto *list : {&ctx->graph_scratch->live, &ctx->graph_scratch->idle})
+                all.insert(all.end(), list->begin(), list->end());
+        }
+        for (brk_scratch *sc : all)
             if (sc->counters) BRK_CUDA(cudaMemset(sc->counters, 0, sc->counters_n * sizeof(int)));
         return fail(BRK_ERR_DEVICE, "a kernel gave up on a bounded wait (code %d)", err);
     }

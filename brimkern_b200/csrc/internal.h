@@ -9,24 +9,33 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <memory>
+#include <mutex>
 #include <vector>
 
 #include "brk_attn.h"
 #include "linear_plan.h"
 
-// Scratch of one stream (or of one stream capture) for the operators that keep theirs apart by
+// Scratch of one stream (or of one stream in a capture) for the operators that keep theirs apart by
 // stream: partials / staging, and arrival counters that are zero between launches.  Calls on two
-// streams, and graphs captured one by one, so never share it.  A buffer that has become too small
-// is kept until the context goes (queued kernels and captured graphs may still use it).
+// streams, and graphs captured one by one, so never share it.
 struct brk_scratch {
     unsigned long long id = 0;   // of the stream (capture: its handle)
     unsigned long long capture_id = 0;
-    bool capture = false;
     void *ws = nullptr;
     size_t ws_bytes = 0;
     int *counters = nullptr;
     size_t counters_n = 0;
-    std::vector<void *> retired;
+    std::vector<void *> retired;  // capture: buffers that became too small, which its nodes may still use
+};
+
+// The scratch of captures.  One belongs to its graph (a user object that the graph, and every executable
+// graph made from it, retains) and goes to `idle` when the last of them is gone, for later captures to
+// take.  CUDA may say so at any time and from any thread, after brk_ctx_destroy too (closed).
+struct brk_graph_scratch {
+    std::mutex mu;
+    bool closed = false;
+    std::vector<brk_scratch *> live, idle;
 };
 
 struct brk_ctx {
@@ -47,7 +56,8 @@ struct brk_ctx {
     size_t act_bytes = 0;
     uint64_t launches = 0;     // kernels launched through this context
     cudaStream_t aux = nullptr;  // zeroes new counters (never captured)
-    std::vector<brk_scratch *> scratch;
+    std::vector<brk_scratch *> scratch;  // of streams, the last used first
+    std::shared_ptr<brk_graph_scratch> graph_scratch;
 };
 
 // This rank's exchange area for sequence-sharded decode over peer memory (brk_attn_decode_push /

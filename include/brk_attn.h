@@ -292,12 +292,15 @@ int brk_attn_combine(brk_ctx *ctx, int n_parts, int rows, int head_dim, const fl
  *     must be finite (a masked row's V still meets a probability of 0 in the product).
  *   - q and out [batch][n_tokens][n_heads][head_dim], each f32 or fp16 by q_type / out_type (BRK_T_*),
  *     16-byte aligned, not overlapping.  n_tokens * (n_heads / n_kv_heads) <= 64.
- *   - Scratch (partials; for an int8 prefix its codes as fp16, 4 bytes per code of the attended
- *     rows of one layer) belongs to the stream, and to the stream capture, that the call is made on:
- *     calls on several streams, graphs, and branches of a graph that were captured from several
- *     streams, may run at the same time.
- *     It grows at the first call that needs more (also while capturing) and lives until
- *     brk_ctx_destroy, which must come after the last replay of such graphs. */
+ *   - Scratch (partials; q as fp16 when it comes in f32; for an int8 prefix its codes as fp16, 4 bytes
+ *     per pair of K and V codes of the attended rows of one layer) belongs to the stream, and to the
+ *     stream capture, that the call is made on: calls on several streams, graphs, and branches of a graph
+ *     that were captured from several streams, may run at the same time.  (Two executable graphs made
+ *     from one capture, or two child nodes of it, share theirs and may not.)
+ *     It grows at the first call that needs more (also while capturing; outside a capture the device
+ *     is synchronised).  A capture's lives as long as its graph and the executable graphs made from it,
+ *     and then serves later captures; of streams outside captures, which come and go, the 64 last used
+ *     keep theirs.  brk_ctx_destroy must come after the last replay of such graphs. */
 int brk_attn_decode_prefix(brk_ctx *ctx, const brk_kv *prefix, int prefix_seq, int prefix_len, const brk_kv *kv,
                            int layer, const brk_attn_params *p, int batch, int n_tokens, const int32_t *past_len,
                            const void *q, int q_type, void *out, int out_type, void *stream);
