@@ -271,7 +271,7 @@ struct LinearArgs {
     int f_rows;               // features per CTA and tile
     int cs;                   // parts that a cluster splits a tile's k into (1: none)
     int kb, stages, flat;     // k steps of 64 per stage; ring stages; k along the maps' x (else along z)
-    int drain_steps;          // stages' worth of k per accumulator set (f32 outputs)
+    int drain_steps;          // stages' worth of k per accumulator set (when it drains)
     int half_cols;            // tokens of a tile that an epilogue warp takes (one or two per lane quarter)
     int tiles_whole;          // the first tiles, done whole, wave by wave; the others are ranged
     int range_units, range_extra;  // (tile, stage of k) units of a worker's range; workers with one more
@@ -364,7 +364,7 @@ cudaError_t launch_proj(int ntok, const CUtensorMap &tx, const CUtensorMap *tw, 
 
 // Linear operators (linear.cu); mats 1 or 2.  The maps: boxes of plan.x_rows (w_rows) rows and plan.kb
 // k steps over [k / 64][row][64] (plan.flat: one k step over [row][k]).
-LinearPlan linear_plan(int rows, int k, int n, int mats, bool drain, int sms);  // drain: f32 outputs
+LinearPlan linear_plan(int rows, int k, int n, int mats, bool drain, int sms);  // drain: linear_drains
 cudaError_t launch_linear(int mats, const LinearPlan &p, const CUtensorMap &tx, const CUtensorMap *tw,
                           const LinearArgs &a, cudaStream_t s);
 // At most linear_rows_max() tokens: without tiles, maps or workspace (M, K, n, x, w, the epilogue's

@@ -27,9 +27,9 @@
 // tile's products, and its warps swap halves of a chunk through shared memory.
 //
 // The tensor core's f32 accumulation truncates: its error is a bias that grows with k (measured on
-// N(0,1) operands against 64 bits: 3.1e-6 of the result at k 2560, 1.2e-5 at 10240).  For f32
-// outputs (DRAIN) the accumulators are drained every 1024 of k and the parts added in registers;
-// fp16 outputs (half a step 4.9e-4) do not need it.
+// N(0,1) operands against 64 bits: 3.1e-6 of the result at k 2560, 1.2e-5 at 10240; on operands of one sign
+// 6e-5).  For f32 outputs, and wide fp16 ones (linear_drains), the accumulators are drained every 1024 of k
+// and the parts added in registers (DRAIN).
 //
 // Measured (calls replayed from a graph): gate-up 2560 -> 10240 of one token 18.9 us, 5.5 TB/s of
 // weights; of 64 tokens 25.4 us, bound by the stream and the exposed ramp and epilogue of one tile a

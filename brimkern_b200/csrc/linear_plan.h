@@ -21,6 +21,12 @@ constexpr int kMaxStages = 16;
 // with 16).
 constexpr int linear_chunk(int nt_kernel, bool drain) { return drain && nt_kernel >= 64 ? 32 : 16; }
 
+// Whether brk_linear's accumulators are drained on the way, every 1024 of k: the tensor cores' f32
+// accumulation truncates, and loses up to 5.9e-9 of the sum for each of k (operands of one sign; 6e-5 at
+// 10240, 3.9e-4 at 65536; drained 5.5e-6 at any k).  An f32 output always, an fp16 one (half a step is
+// 4.9e-4) where it would lose more than a fifth of that.
+constexpr bool linear_drains(bool f32_out, int k) { return f32_out || k > 16384; }
+
 constexpr int linear_round_up(int v, int m) { return (v + m - 1) / m * m; }
 
 // How a linear product is cut: the kernel's token tile, tokens per tile, rows of the TMA boxes of x

@@ -313,9 +313,10 @@ int brk_attn_step_prefix(brk_ctx *ctx, const brk_kv *prefix, int prefix_seq, int
 
 /* ---- linear operators on fp16 activations (the FFN of recordLayerKV, kernels.ts:1737-1744) -----
  * Weights are the engine's fp16 matrices [n][k] (C = A W^T), activations x fp16 [rows][k], biases
- * f32 [n] or NULL; sums in f32.  k is a multiple of 8, x and the weights 16-byte aligned, f32 tensors
- * 4-byte; rows (0: nothing is done) and n are any size up to 2^30.  Results do not change from run to run.  Scratch as for
- * brk_attn_decode_prefix: by stream and stream capture.  Outputs may not overlap inputs, except
+ * f32 [n] or NULL; sums in f32.  k is a multiple of 8 and at most 2^24, gate-up's 2^15 (the tensor cores'
+ * sums, where they are not drained on the way, lose up to 5.9e-9 of themselves for each of k), x and the
+ * weights 16-byte aligned, f32 tensors 4-byte; rows (0: nothing is done) and n are any size up to 2^30.
+ * Results do not change from run to run.  Scratch as for brk_attn_decode_prefix: by stream and stream capture.  Outputs may not overlap inputs, except
  * brk_linear's f32 out, which may be its residual.
  *   brk_linear:      out = act(x w^T + bias) + residual    (residual f32 [rows][n] or NULL)
  *                    out f32 or fp16 [rows][n] by out_type.

@@ -112,3 +112,23 @@ def test_ffn_block(eng, rows):
     assert_within(out, ref, tol, "ffn")
     for _ in range(10):
         assert torch.equal(eng.ffn(h, wg, wu, wd, torch.empty_like(out), ffn_norm=norm), out)
+
+
+@pytest.mark.parametrize("k", [16384, 16392, 65536])
+def test_wide_fp16_sums_lose_nothing(eng, k):
+    """Operands of one sign, whole tiles of k: the tensor cores' truncation is a bias of the sum, at most
+    k / 16 steps of 2^-23 without a drain (5.9e-9 of the sum for each of k seen: 1e-4 at the last undrained
+    width), 64 steps with one.  The mean over many outputs averages their own rounding out (2^-11 / sqrt(3 *
+    65536) = 1.1e-6)."""
+    import torch
+    g = torch.Generator(device=eng.device).manual_seed(k)
+    rows, n = 512, 9472
+    x = torch.rand((rows, k), generator=g, device=eng.device, dtype=torch.float16) / 64
+    w = torch.empty((n, k), dtype=torch.float16, device=eng.device)
+    for part in w.split(1184):
+        part.copy_(torch.rand(part.shape, generator=g, device=eng.device) * 256 / k)
+    y = eng.linear(x, w, torch.empty((rows, n), dtype=torch.float16, device=eng.device))
+    eng.ctx.check()
+    ref = x[:128].double() @ w[-512:].double().t()
+    lost = abs(((y[:128, -512:].double() - ref) / ref).mean().item())
+    assert lost <= (1.2e-4 if k <= 16384 else 64 * 2.0 ** -23 + 4 * 1.1e-6), lost
