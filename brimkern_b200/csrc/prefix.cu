@@ -750,7 +750,10 @@ PrefixPlan prefix_plan(int head_dim, int tokens, int group, int kv_heads, int nt
     const double mine = (double)units * ntiles * tile, theirs = 0.5 * own_tiles;
     const int share = std::max(1, (int)(sms * (1.0 - std::min(0.5, theirs / (mine + theirs)))));
     double best = 1e300;
-    for (int n = 1; n <= 32 && (n == 1 || 2 * n <= ntiles); ++n) {
+    // No split longer than 256 tiles, while 32 splits do: a sum in the tensor cores loses up to 2^-24 of itself
+    // with each product of 16 keys and term of P (16384 keys, V of one sign: 1.2e-4 at most; 131072 keys in one
+    // split, twice an fp16 output's half step).
+    for (int n = std::min(32, (ntiles + 255) / 256); n <= 32 && (n == 1 || 2 * n <= ntiles); ++n) {
         const int tps = (ntiles + n - 1) / n;
         if ((ntiles + tps - 1) / tps != n) continue;  // no empty split
         const double cost = (double)((units * n + share - 1) / share) * (tps + 6) + 0.25 * n;

@@ -57,3 +57,34 @@ def test_few_keys(eng, Hq, Hkv, D, P, B, q8):
         ref = torch.einsum("hgn,nhd->hgd", p, torch.cat([pv, ov])).reshape(Hq, D)
         err = (out[b, 0].double() - ref).abs() / ref
         assert err.max().item() <= 2.0 ** -17, (b, err.max().item())
+
+
+@pytest.mark.parametrize("Hq,Hkv,D,P,B,T", [(32, 8, 128, 131072, 512, 1), (8, 4, 256, 70000, 512, 1),
+                                            (21, 3, 64, 131072, 441, 4)])  # one split just fills the GPU
+def test_long_prefix_and_many_rows(eng, Hq, Hkv, D, P, B, T):
+    """Values of one sign: a tensor-core sum loses up to half a step (2^-24) of itself with each of the two
+    products of 16 keys (P's terms), so a split may not be long even when many rows fill the GPU with few:
+    2048 products of 16384 keys, 1.2e-4."""
+    import torch
+    from brimkern_b200.engine import AttnConfig, KvCache
+    dev = eng.device
+    g = torch.Generator(device=dev).manual_seed(P + D)
+    prefix, kv = KvCache(eng.ctx, 1, 1, Hkv, D, P), KvCache(eng.ctx, 1, B, Hkv, D, T)
+    for c in range(0, P, 16384):
+        n = min(16384, P - c)
+        prefix.write_rows(0, 0, c, 0.1 * torch.randn((n, Hkv, D), generator=g, device=dev),
+                          1 + torch.rand((n, Hkv, D), generator=g, device=dev))
+    for b in range(B):
+        kv.write_rows(0, b, 0, torch.zeros((T, Hkv, D), device=dev), torch.ones((T, Hkv, D), device=dev))
+    q = torch.randn((B, T, Hq, D), generator=g, device=dev).half()
+    out = torch.empty(q.shape, device=dev)
+    eng.decodePrefix(prefix, P, kv, 0, AttnConfig(Hq, Hkv, D, kv_offset=P), q, out, [P] * B)
+    eng.ctx.check()
+    k, v = prefix.read_rows(0, 0, 0, P)
+    G = Hq // Hkv
+    for b, h in ((0, 0), (B // 2, Hkv - 1), (B - 1, 0)):
+        heads = slice(h * G, (h + 1) * G)
+        z = q[b, 0, heads].double() @ k[:, h].double().t() * D ** -0.5
+        p = torch.softmax(torch.cat([z, z.new_zeros((G, 1))], 1), -1)
+        ref = p @ torch.cat([v[:, h].double(), v.new_ones((1, D)).double()])
+        assert abs(((out[b, 0, heads].double() - ref) / ref).mean().item()) <= 2048 * 2.0 ** -24
