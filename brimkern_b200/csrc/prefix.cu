@@ -313,6 +313,8 @@ __global__ void __launch_bounds__(PrefixLayout<D>::kThreads, 1)
         const bool row_ok = bt_of < nbt && bt < bt_total;
         const int cnt = tile_count(s), j0 = first_tile(s);
         const int lo = a.window > 0 && row_ok ? a.past_len[bt / a.T] + bt % a.T - a.window + 1 : INT_MIN;
+        // The first key that a row of this warp attends: what lies before it may hold anything.
+        const int warp_lo = __reduce_min_sync(0xffffffffu, row_ok ? lo : INT_MAX);
         const uint32_t tS = tmem + L::kColS + s * kXK + lane_base + copy * KC;
         const uint32_t tO = tmem + L::kColO + s * D + lane_base;
         const uint32_t tP = tmem + L::kColP + s * (kXK / 2) + lane_base;
@@ -386,7 +388,7 @@ __global__ void __launch_bounds__(PrefixLayout<D>::kThreads, 1)
 #pragma unroll
                     for (int e = 0; e < KC; e += 32) {
                         const int x = KC < 32 ? lane % KC : e + lane;
-                        if (kbase + x < ke) top = max(top, __float_as_uint(vsc[x]));
+                        if (kbase + x >= warp_lo && kbase + x < ke) top = max(top, __float_as_uint(vsc[x]));
                     }
                     mt += v_scale_log2(__uint_as_float(__reduce_max_sync(0xffffffffu, top)));
                 } else {

@@ -85,3 +85,29 @@ def test_v_of_any_size(eng, kind, Hq, Hkv, D, P, own, T, q8p, q8o, kw):
             err = (out[b, t].double() - ref).abs()
             bad = ~(err <= REL * mag)
             assert not bad.any(), (b, t, int(bad.sum()), (err / (REL * mag)).max().item())
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), 1e30])
+@pytest.mark.parametrize("P,own,W", [(8001, [3, 30, 301, 5, 6, 7], 7007), (3001, [2, 3, 4, 9], 2502), (301, [5, 9], 251)])
+def test_scales_below_every_window(eng, bad, P, own, W):
+    """Rows before the first attended one may hold anything, though loads round down to a multiple of four."""
+    import torch
+    from brimkern_b200.engine import AttnConfig, KvCache
+    dev = eng.device
+    g = torch.Generator(device=dev).manual_seed(P)
+    Hq, Hkv, D, B = 32, 8, 128, len(own)
+    rnd = lambda *s: torch.randn(s, generator=g, device=dev)  # noqa: E731
+    prefix, kv = KvCache(eng.ctx, 1, 1, Hkv, D, P, q8=True), KvCache(eng.ctx, 1, B, Hkv, D, max(own), q8=True)
+    prefix.write_rows(0, 0, 0, rnd(P, Hkv, D), rnd(P, Hkv, D))
+    for b, n in enumerate(own):
+        kv.write_rows(0, b, 0, rnd(n, Hkv, D), rnd(n, Hkv, D))
+    cfg = AttnConfig(Hq, Hkv, D, kv_offset=P, window=W)
+    q, past = rnd(B, 1, Hq, D).half(), [P + n - 1 for n in own]
+    first = min(past) - W + 1
+    assert first % 4 and first < P
+    want = eng.decodePrefix(prefix, P, kv, 0, cfg, q, torch.empty_like(q), past)
+    kc, ks, vc, vs = prefix.read_codes(0, 0, 0, first)
+    prefix.write_codes(0, 0, 0, kc, torch.full_like(ks, bad), vc, torch.full_like(vs, bad))
+    got = eng.decodePrefix(prefix, P, kv, 0, cfg, q, torch.empty_like(q), past)
+    eng.ctx.check()
+    assert torch.isfinite(want).all() and torch.equal(got, want)
