@@ -291,7 +291,8 @@ int brk_attn_combine(brk_ctx *ctx, int n_parts, int rows, int head_dim, const fl
  *     prefix may be NULL with prefix_len 0.  Rows of the prefix from the first attended position on
  *     must be finite (a masked row's V still meets a probability of 0 in the product).
  *   - q and out [batch][n_tokens][n_heads][head_dim], each f32 or fp16 by q_type / out_type (BRK_T_*),
- *     16-byte aligned, not overlapping.  n_tokens * (n_heads / n_kv_heads) <= 64.
+ *     16-byte aligned, not overlapping.  The tensor cores take q in fp16: an f32 q is rounded to it, as
+ *     brk_attn_decode's is, here by a launch of its own (a value past 65504 becomes infinite).  n_tokens * (n_heads / n_kv_heads) <= 64.
  *   - Scratch (partials; q as fp16 when it comes in f32; for an int8 prefix its codes as fp16, 4 bytes
  *     per pair of K and V codes of the attended rows of one layer) belongs to the stream, and to the
  *     stream capture, that the call is made on: calls on several streams, graphs, and branches of a graph
@@ -324,7 +325,9 @@ int brk_attn_step_prefix(brk_ctx *ctx, const brk_kv *prefix, int prefix_seq, int
  *   brk_ffn:         the whole block: out = h + ffn(rmsnorm(h, ffn_norm)), f32 [rows][d_model], with
  *                    ffn(x) = w_down (act(w_gate x) * (w_up x)); with post_norm (Gemma-2) out = h +
  *                    rmsnorm(ffn(...), post_norm).  ffn_norm NULL: no norm.  d_model and d_ff
- *                    multiples of 8.  out may not alias h. */
+ *                    multiples of 8.  out may not alias h.  The normed rows and the hidden rows
+ *                    between the products are fp16, as the products' operands: a value of theirs
+ *                    past 65504 becomes infinite, and the row with it. */
 int brk_linear(brk_ctx *ctx, int rows, int k, int n, const uint16_t *x, const uint16_t *w, const float *bias, int act,
                const float *residual, void *out, int out_type, void *stream);
 int brk_ffn_gate_up(brk_ctx *ctx, int rows, int d_model, int d_ff, const uint16_t *x, const uint16_t *w_gate,
