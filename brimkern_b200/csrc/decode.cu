@@ -284,8 +284,9 @@ struct DecodeArgsOf<true> {
 // its partials was complete before this grid could start), or, for a prefix of few bytes (a.pre_tiles),
 // it reads the prefix itself before the own rows and is the call's only launch.  int8 codes enter the
 // products exactly here (a subtraction more per pair; the plain form's bias of 1152 sums loses up to
-// 1e-3 of a score).  64 sequences of up to 512 own rows (32 / 8 heads of 128) beside a prefix of 4096:
-// 32 us with the prefix kernel, bound by the own rows' 74 MB and the SMs that the two share.
+// 1e-3 of a score).  64 sequences of up to 512 own rows (32 / 8 heads of 128; 74 MB) beside a prefix of 4096:
+// 34 us with the prefix kernel replayed from a graph, 35 eager, bound by the SMs that the two share; these
+// rows alone 19.6 us.
 template <bool Q8, int D, bool F, bool H = false>
 __global__ void __launch_bounds__(decode_threads<Q8, D, F>(), DecodeCfg<Q8, D>::kMinBlocks)
     decode_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,

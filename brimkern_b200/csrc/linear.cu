@@ -31,11 +31,11 @@
 // 6e-5).  For f32 outputs, and wide fp16 ones (linear_drains), the accumulators are drained every 1024 of k
 // and the parts added in registers (DRAIN).
 //
-// Measured (calls replayed from a graph): gate-up 2560 -> 10240 of one token 18.9 us, 5.5 TB/s of
-// weights; of 64 tokens 25.4 us, bound by the stream and the exposed ramp and epilogue of one tile a
-// CTA; of 2048 tokens 160 us, 1340 TFLOP/s.  Linear 2048 x 10240 -> 2560 with a residual 113 us (f32)
-// and 92 (fp16, none): k steps at 85% of the tensor rate, then a join and an epilogue (9 to 12 thousand
-// cycles) that no next tile hides.
+// Measured, replayed from a graph (eager, caches cold): gate-up 2560 -> 10240 of one token 18.6 us (18.9), 5.6
+// TB/s of weights; of 64 tokens 25.5 us (26.7), bound by the stream and the exposed ramp and epilogue of one
+// tile a CTA; of 2048 tokens 158 us (186, at the power cap), 1358 TFLOP/s, tensor pipe 76% active.  Linear 2048
+// x 10240 -> 2560 with a residual 109 us (129) in f32, 93 in fp16 without: tensor pipe 53% active, then a join
+// and an epilogue (9 to 12 thousand cycles) that no next tile hides.
 #include <algorithm>
 
 #include "common.cuh"

@@ -10,7 +10,8 @@
 //   f32), P as two fp16 terms (its rounding and what that leaves off) in TMEM, O += P V in TMEM.
 // With one term the rounding of P, 2^-11 of each, is as large as an fp16 output's own (relative error
 // against 64 bits 2.9e-4, with two 2.1e-4); the second costs MMAs and conversions: 8 sequences behind 131001
-// rows 67 -> 78 us, 16 x 2 tokens over int8 rows 32.7 -> 34.1, 64 behind 4096 34 -> 35.5, the window no time.
+// rows 67 -> 75-78 us (eager), 16 x 2 tokens over int8 rows 32.8 -> 34.3, 64 behind 4096 34.3 -> 35.4, the
+// window no time.
 // Two streams of 128 rows run a tile apart so that one's exponentials overlap the other's products:
 // with more rows than one stream holds the streams are two row tiles that share every K/V tile; with
 // fewer they take alternate key tiles of the same rows.  head_dim 256 leaves TMEM for one stream.
@@ -23,10 +24,11 @@
 // cluster through distributed shared memory first, for an eighth of the partials: 131 KB a CTA took
 // 5 us there.)
 //
-// Whole calls, own rows and joins included: 8 sequences (32 / 8 heads of 64) behind 131001 rows 57 us,
-// 4.7 TB/s of K and V, bound by the stream and 10 us of ramp and joins; 64 sequences (32 / 8 of 128)
-// behind 4096 rows 32 us, bound by the own rows beside it; 32 (8 / 4 of 256) with a window of 4096 22 us,
-// bound by the one stream's softmax between its products.
+// Whole calls, own rows and joins included, replayed from a graph (eager, caches cold): 8 sequences (32 /
+// 8 heads of 64) behind 131001 rows 65 us (75-78), DRAM at 4.0 TB/s and the tensor pipe 42% active: bound by a
+// tile's chain of scores, softmax and product, and 10 us of ramp and joins; 64 sequences (32 / 8 of 128) behind
+// 4096 rows 34 us (35), this kernel alone 24.7 on 64 SMs, the own rows alone 19.6 on all; 32 (8 / 4 of 256) with
+// a window of 4096 21 us (23), bound by the one stream's softmax between its products.
 //
 // int8 prefix: the codes, as exact fp16 integers, are the operands; the K scale multiplies the
 // scores and the V scale the probabilities, so nothing is rounded that the fp16 form does not round.  The
