@@ -684,8 +684,14 @@ int brk_ctx_create(int device, brk_ctx **out) {
     cudaDeviceProp prop;
     BRK_CUDA(cudaGetDeviceProperties(&prop, device));
     if (prop.major != 10) return fail(BRK_ERR_UNSUPPORTED, "device %d is sm_%d%d; this build targets sm_100a", device, prop.major, prop.minor);
-    brk_ctx *c = new brk_ctx();
-    c->graph_scratch = std::make_shared<brk_graph_scratch>();
+    std::unique_ptr<brk_ctx> fresh;
+    try {
+        fresh.reset(new brk_ctx());
+        fresh->graph_scratch = std::make_shared<brk_graph_scratch>();
+    } catch (const std::bad_alloc &) {
+        return fail(BRK_ERR_CUDA, "out of host memory");
+    }
+    brk_ctx *c = fresh.release();
     c->device = device;
     c->num_sms = prop.multiProcessorCount;
     cudaError_t e = cudaMalloc(&c->d_err, sizeof(int));
@@ -728,14 +734,15 @@ int brk_ctx_destroy(brk_ctx *ctx) {
     cudaFree(ctx->stage);
     cudaFree(ctx->act);
     for (brk_scratch *sc : ctx->scratch) free_scratch(sc);
-    std::vector<brk_scratch *> live;
+    std::vector<brk_scratch *> live, idle;
     {
         std::lock_guard<std::mutex> lock(ctx->graph_scratch->mu);
         ctx->graph_scratch->closed = true;
         live.swap(ctx->graph_scratch->live);
+        idle.swap(ctx->graph_scratch->idle);
     }
     for (brk_scratch *sc : live) free_scratch(sc);
-    free_idle_graph_scratch(ctx);
+    for (brk_scratch *sc : idle) free_scratch(sc);
     if (ctx->aux) cudaStreamDestroy(ctx->aux);
     delete ctx;
     return BRK_OK;
@@ -751,11 +758,14 @@ int brk_ctx_check(brk_ctx *ctx, void *stream) {
         BRK_CUDA(cudaMemset(ctx->d_err, 0, sizeof(int)));
         // A kernel that gave up may have left split counters mid-count: start them from zero.
         if (ctx->counters) BRK_CUDA(cudaMemset(ctx->counters, 0, ctx->counters_n * sizeof(int)));
-        std::vector<brk_scratch *> all = ctx->scratch;
-        {
+        std::vector<brk_scratch *> all;
+        try {
+            all = ctx->scratch;
             std::lock_guard<std::mutex> lock(ctx->graph_scratch->mu);
             for (auto *list : {&ctx->graph_scratch->live, &ctx->graph_scratch->idle})
                 all.insert(all.end(), list->begin(), list->end());
+        } catch (const std::bad_alloc &) {
+            return fail(BRK_ERR_CUDA, "out of host memory");
         }
         for (brk_scratch *sc : all)
             if (sc->counters) BRK_CUDA(cudaMemset(sc->counters, 0, sc->counters_n * sizeof(int)));
