@@ -719,8 +719,10 @@ class AttentionEngine:
                    stream=None) -> torch.Tensor:
         """attentionLayer over a shared prefix: the new tokens' K / V appended to `kv` (QK-norm and
         RoPE as appendKv), then decodePrefix.  q_in [B, T, Hq, D], k_in / v_in [B, T, Hkv, D] f32
-        projections; out f32 (default) or fp16."""
+        projections; out f32 (default) or fp16.  q_work and out that are not given are allocated on the
+        stream that the step runs on."""
         T = self._prefix_tokens(kv, cfg, q_in, "q_in")
+        self._tensor(q_in, "q_in", _F32, None)
         n_kv = kv.batch * T * cfg.n_kv_heads * cfg.head_dim
         q_work, out = _buffers_like(q_in, stream, q_work, out)
         ptrs = [self._tensor(t, n, _F32, None) for t, n in ((q_in, "q_in"), (k_in, "k_in"), (v_in, "v_in"), (q_work, "q_work"))]

@@ -39,7 +39,7 @@ def test_step_on_another_stream_keeps_its_buffers(eng, entry, monkeypatch):
     assert seen[0][1] == out.data_ptr()
     assert seen[0][0] not in taken and seen[0][1] not in taken
     with torch.cuda.stream(side):  # its own stream may have it again, in order
-        assert torch.empty_like(q).data_ptr() == seen[0][0]
+        assert seen[0][0] in {t.data_ptr() for t in [torch.empty_like(q) for _ in range(64)]}
     torch.cuda.synchronize()
     assert torch.equal(out, want)
     # The output is read on the current stream: dropped there, it is not handed out on the side stream
@@ -53,3 +53,18 @@ def test_step_on_another_stream_keeps_its_buffers(eng, entry, monkeypatch):
         assert seen[0][1] not in {t.data_ptr() for t in [torch.empty_like(q) for _ in range(8)]}
     torch.cuda.synchronize()
     eng.ctx.check()
+
+
+def test_step_prefix_refuses_before_it_allocates(eng):
+    """On a stream of its own too, inputs of the wrong device or type come back as the library's error."""
+    import torch
+    from brimkern_b200 import BrkError
+    from brimkern_b200.engine import AttnConfig, KvCache
+    kv = KvCache(eng.ctx, 1, 2, 2, 64, 4)
+    q, k = torch.zeros((2, 1, 4, 64), device=eng.device), torch.zeros((2, 1, 2, 64), device=eng.device)
+    before = eng.ctx.launches
+    for bad in (q.cpu(), q.half(), q.transpose(2, 3)):
+        for stream in (None, torch.cuda.Stream()):
+            with pytest.raises(BrkError):
+                eng.stepPrefix(None, 0, kv, 0, AttnConfig(4, 2, 64), bad, k, k, [0, 0], stream=stream)
+    assert eng.ctx.launches == before
